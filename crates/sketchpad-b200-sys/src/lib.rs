@@ -29,6 +29,7 @@ pub const SP_ERR_COMM: c_int = -8;
 pub const SP_F32: c_int = 0;
 pub const SP_F16: c_int = 1;
 pub const SP_BF16: c_int = 2;
+pub const SP_E4M3: c_int = 3;
 
 // sp_act
 pub const SP_ACT_NONE: c_int = 0;
@@ -210,6 +211,59 @@ extern "C" {
         bias: *const c_void, y: *mut c_void, ldy: i64, m: i64, n: i64, k: i64,
         rope_cos_sin: *const c_float, rope_positions: i64, rope_cols: i64, head_dim: i64,
         pos_offset: i64, pos_div: i64, pos_mod: i64, dtype: c_int, stream: *mut c_void
+    ) -> c_int;
+    // -- generating a token at a time: RMS norm, 4-bit linear, paged cache
+    //    (crates/sketchpad-llm; crates/sketchpad-core/src/paged_attention.rs)
+    pub fn sp_rms_norm(
+        x: *const c_void, x_row_stride: i64, residual: *const c_void, residual_row_stride:
+        i64, weight: *const c_void, y: *mut c_void, residual_out: *mut c_void, rows: i64, n:
+        i64, eps: c_float, dtype: c_int, stream: *mut c_void
+    ) -> c_int;
+    pub fn sp_rms_norm_fp8(
+        x: *const c_void, x_row_stride: i64, residual: *const c_void, residual_row_stride:
+        i64, weight: *const c_void, q: *mut c_void, scale: *mut c_float, residual_out: *mut
+        c_void, rows: i64, n: i64, eps: c_float, dtype: c_int, stream: *mut c_void
+    ) -> c_int;
+    pub fn sp_int4_packed_bytes(
+        N: i64, K: i64, group: i64, sizes: *mut i64
+    ) -> c_int;
+    pub fn sp_int4_repack(
+        qweight: *const c_void, scales: *const c_void, zeros: *const c_void, N: i64, K: i64,
+        group: i64, q_packed: *mut c_void, s_packed: *mut c_void, z_packed: *mut c_void,
+        stream: *mut c_void
+    ) -> c_int;
+    pub fn sp_int4_dequant(
+        q_packed: *const c_void, s_packed: *const c_void, z_packed: *const c_void, N: i64,
+        K: i64, group: i64, scale_dtype: c_int, out: *mut c_void, out_dtype: c_int, stream:
+        *mut c_void
+    ) -> c_int;
+    pub fn sp_int4_linear(
+        x: *const c_void, x_row_stride: i64, x_dtype: c_int, x_scale: *const c_float,
+        q_packed: *const c_void, s_packed: *const c_void, z_packed: *const c_void,
+        scale_dtype: c_int, bias: *const c_void, y: *mut c_void, M: i64, N: i64, K: i64,
+        group: i64, out_dtype: c_int, stream: *mut c_void
+    ) -> c_int;
+    pub fn sp_paged_kv_append(
+        q: *const c_void, k: *const c_void, v: *const c_void, q_out: *mut c_void, q_strides:
+        *const i64, k_in_strides: *const i64, v_in_strides: *const i64, tokens: i64, hq:
+        i64, hkv: i64, D: i64, k_cache: *mut c_void, v_cache: *mut c_void, k_scale: *const
+        c_float, v_scale: *const c_float, k_strides: *const i64, v_strides: *const i64,
+        pages: i64, page_size: i64, block_table: *const c_void, table_rows: i64, table_cols:
+        i64, table_stride: i64, seq_ids: *const c_void, positions: *const c_void,
+        rope_cos_sin: *const c_float, rope_rows: i64, dtype: c_int, cache_dtype: c_int,
+        stream: *mut c_void
+    ) -> c_int;
+    pub fn sp_paged_attention_workspace_size(
+        B: i64, hq: i64, hkv: i64
+    ) -> usize;
+    pub fn sp_paged_attention(
+        q: *const c_void, q_strides: *const i64, k_cache: *const c_void, v_cache: *const
+        c_void, k_scale: *const c_float, v_scale: *const c_float, k_strides: *const i64,
+        v_strides: *const i64, block_table: *const c_void, table_cols: i64, table_stride:
+        i64, seq_lens: *const c_void, out: *mut c_void, B: i64, hq: i64, hkv: i64, D: i64,
+        pages: i64, page_size: i64, window: i64, sinks: i64, scale: c_float, dtype: c_int,
+        cache_dtype: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut
+        c_void
     ) -> c_int;
     // -- LayerNorm (crates/sketchpad-core/src/layernorm.rs:63-73: unbiased variance)
     pub fn sp_layernorm(

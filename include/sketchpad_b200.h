@@ -36,7 +36,8 @@ typedef enum sp_status {
   SP_ERR_COMM = -8         /* NCCL missing or failed, or a communication deadline passed */
 } sp_status;
 
-typedef enum sp_dtype { SP_F32 = 0, SP_F16 = 1, SP_BF16 = 2 } sp_dtype;
+/* SP_E4M3 is taken only where an entry point says so. */
+typedef enum sp_dtype { SP_F32 = 0, SP_F16 = 1, SP_BF16 = 2, SP_E4M3 = 3 } sp_dtype;
 
 typedef enum sp_act { SP_ACT_NONE = 0, SP_ACT_SILU = 1 } sp_act;
 
@@ -430,6 +431,98 @@ int sp_model_tensor_info(void* file, int64_t index, char* name_out, size_t name_
                          uint64_t* nbytes_out);
 int sp_model_find(void* file, const char* name, int64_t* index_out);
 int sp_model_tensor_data(void* file, int64_t index, const uint8_t** data_out);
+
+/* ------------------------------------------------------------------------------------
+ * Generating a token at a time: the operators of a decoder layer over a paged cache (the
+ * reference's language models beside the denoiser: crates/sketchpad-llm, and the paged cache
+ * of crates/sketchpad-core/src/paged_attention.rs).
+ * ------------------------------------------------------------------------------------ */
+/* Root-mean-square norm:  r = T(x + residual);  y = r / sqrt(mean(r^2) + eps) * weight.
+ * x [rows, n] with row stride x_row_stride; residual (NULL: none) likewise; weight [n] (NULL:
+ * ones); y and residual_out (NULL: not kept; receives r) contiguous.  All of `dtype` (f32, f16,
+ * bf16); arithmetic in f32.  y and residual_out may be x or residual where those are
+ * contiguous.  rows = 0 is an empty call.
+ * _fp8: q [rows, n] e4m3 bytes (nearest, ties to even) and scale [rows], y ~ q * scale with
+ * scale = max|y| / 448 over the row (1 for a row of zeros, at least the smallest normal f32; a
+ * NaN in the row makes its scale and all of its q NaN). */
+int sp_rms_norm(const void* x, int64_t x_row_stride, const void* residual,
+                int64_t residual_row_stride, const void* weight, void* y, void* residual_out,
+                int64_t rows, int64_t n, float eps, int dtype, void* stream);
+int sp_rms_norm_fp8(const void* x, int64_t x_row_stride, const void* residual,
+                    int64_t residual_row_stride, const void* weight, void* q, float* scale,
+                    void* residual_out, int64_t rows, int64_t n, float eps, int dtype,
+                    void* stream);
+
+/* 4-bit weights with a scale per group of inputs, for few rows of x:
+ *   w[n, k] = scale[k / group, n] * (q[n, k] - zero[k / group, n])
+ *   y[m, n] = xs[m] * sum_k w[n, k] x[m, k] + bias[n]
+ * qweight [N, K/2] (value k in the low nibble of byte k/2 for even k, the high one for odd k),
+ * scales [K/group, N] f16 or bf16, zeros [K/group, N] bytes 0..15 or NULL (8).  group: 32, 64 or
+ * a multiple of 128 that divides K; any N.  sp_int4_repack lays a weight out once for the
+ * kernels into q_packed, s_packed, z_packed (16-byte aligned, sizes[0..2] bytes of
+ * sp_int4_packed_bytes; z_packed NULL with zeros NULL). */
+int sp_int4_packed_bytes(int64_t N, int64_t K, int64_t group, int64_t sizes[4]);
+int sp_int4_repack(const void* qweight, const void* scales, const void* zeros, int64_t N,
+                   int64_t K, int64_t group, void* q_packed, void* s_packed, void* z_packed,
+                   void* stream);
+/* The values of a laid-out weight, [N, K] of out_dtype (SP_F32: scale * (q - zero) exactly). */
+int sp_int4_dequant(const void* q_packed, const void* s_packed, const void* z_packed, int64_t N,
+                    int64_t K, int64_t group, int scale_dtype, void* out, int out_dtype,
+                    void* stream);
+/* x [M, K]: f16, bf16, or e4m3 (SP_E4M3, with x_scale [M], NULL otherwise); rows 16-byte aligned
+ * (8 for e4m3), x_row_stride a multiple of 8 elements.  bias [N] of out_dtype or NULL.  y [M, N]
+ * contiguous, out_dtype f32, f16 or bf16.  Sums are f32 and their order does not change from
+ * call to call.  Any M; the weights are read once per 32 rows of x. */
+int sp_int4_linear(const void* x, int64_t x_row_stride, int x_dtype, const float* x_scale,
+                   const void* q_packed, const void* s_packed, const void* z_packed,
+                   int scale_dtype, const void* bias, void* y, int64_t M, int64_t N, int64_t K,
+                   int64_t group, int out_dtype, void* stream);
+
+/* A paged key-value cache: k_cache, v_cache [pages, page_size, hkv, D] with element strides
+ * (innermost 1, the others multiples of 16 bytes, pointers 16-byte aligned), D a multiple of 16
+ * up to 256, f16, bf16 or e4m3 (then k_scale, v_scale [hkv] f32: value = e4m3 * scale).
+ * block_table [table_rows, table_cols] int32, row stride table_stride: the page of token t of
+ * sequence b is block_table[b, t / page_size]; an entry outside [0, pages) is a page that is
+ * not there.
+ *
+ * sp_paged_kv_append: token i (of `tokens`) of sequence seq_ids[i] at positions[i] (int32): k
+ * and v [tokens, hkv, D] enter the cache at its slot, q [tokens, hq, D] comes out in q_out
+ * (contiguous; q and q_out NULL: none).  rope_cos_sin [rope_rows, D/2, 2] f32 (cos, sin), or
+ * NULL: q and k are rotated as sp_q8_0_linear_rope rotates (pairs (2i, 2i+1), row =
+ * position).  A token whose sequence, position, page or table row does not exist is padding:
+ * nothing is stored and its q_out is zeros.  dtype: q, k, v, q_out f16 or bf16; the cache is of
+ * that type or e4m3.  Input strides (token, head, 1, unused) in elements, multiples of 8.  Two
+ * tokens of one call must not share a slot. */
+int sp_paged_kv_append(const void* q, const void* k, const void* v, void* q_out,
+                       const int64_t q_strides[4], const int64_t k_in_strides[4],
+                       const int64_t v_in_strides[4], int64_t tokens, int64_t hq, int64_t hkv,
+                       int64_t D, void* k_cache, void* v_cache, const float* k_scale,
+                       const float* v_scale, const int64_t k_strides[4],
+                       const int64_t v_strides[4], int64_t pages, int64_t page_size,
+                       const void* block_table, int64_t table_rows, int64_t table_cols,
+                       int64_t table_stride, const void* seq_ids, const void* positions,
+                       const float* rope_cos_sin, int64_t rope_rows, int dtype, int cache_dtype,
+                       void* stream);
+
+/* Attention of one new token per sequence over the cache: out[b, h] = softmax(scale q[b, h] .
+ * k_j) v_j over the visible tokens j < seq_lens[b] (int32; the new token's own k and v are in
+ * the cache, and lengths beyond the table are cut).  window > 0: only j >= seq_lens[b] - window
+ * and j < sinks.  Tokens on pages that are not there are not seen; a sequence that sees none
+ * gives zeros.  q [B, hq, D] with strides (sequence, head, 1, unused), heads 4-byte aligned;
+ * out [B, hq, D] contiguous; q and out of `dtype` (f16, bf16), the cache of that type or e4m3;
+ * query head h reads cache head h / (hq / hkv).  scale <= 0 selects 1/sqrt(D).
+ * workspace: sp_paged_attention_workspace_size() bytes, 16-byte aligned, ZERO before its first
+ * use (each call leaves its counters zero again) and not in use by another call in flight;
+ * calls of any sizes that fit may share it. */
+size_t sp_paged_attention_workspace_size(int64_t B, int64_t hq, int64_t hkv);
+int sp_paged_attention(const void* q, const int64_t q_strides[4], const void* k_cache,
+                       const void* v_cache, const float* k_scale, const float* v_scale,
+                       const int64_t k_strides[4], const int64_t v_strides[4],
+                       const void* block_table, int64_t table_cols, int64_t table_stride,
+                       const void* seq_lens, void* out, int64_t B, int64_t hq, int64_t hkv,
+                       int64_t D, int64_t pages, int64_t page_size, int64_t window, int64_t sinks,
+                       float scale, int dtype, int cache_dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

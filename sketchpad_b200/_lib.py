@@ -12,7 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsketchpad_b200.so")
 
 SP_OK = 0
-SP_F32, SP_F16, SP_BF16 = 0, 1, 2
+SP_F32, SP_F16, SP_BF16, SP_E4M3 = 0, 1, 2, 3
 SP_ACT_NONE, SP_ACT_SILU = 0, 1
 
 _STATUS = {
@@ -95,6 +95,21 @@ SIGNATURES = {
                                    _i64, _i64, _i64, _i64, _i64, _int, _vp]),
     "sp_fp8_linear_rope": (_int, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp,
                                   _i64, _i64, _i64, _i64, _i64, _i64, _int, _vp]),
+    "sp_rms_norm": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _f, _int, _vp]),
+    "sp_rms_norm_fp8": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _f, _int,
+                               _vp]),
+    "sp_int4_packed_bytes": (_int, [_i64, _i64, _i64, _i64p]),
+    "sp_int4_repack": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "sp_int4_dequant": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _int, _vp]),
+    "sp_int4_linear": (_int, [_vp, _i64, _int, _vp, _vp, _vp, _vp, _int, _vp, _vp, _i64, _i64,
+                              _i64, _i64, _int, _vp]),
+    "sp_paged_kv_append": (_int, [_vp, _vp, _vp, _vp, _i64p, _i64p, _i64p, _i64, _i64, _i64, _i64,
+                                  _vp, _vp, _vp, _vp, _i64p, _i64p, _i64, _i64, _vp, _i64, _i64,
+                                  _i64, _vp, _vp, _vp, _i64, _int, _int, _vp]),
+    "sp_paged_attention_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "sp_paged_attention": (_int, [_vp, _i64p, _vp, _vp, _vp, _vp, _i64p, _i64p, _vp, _i64, _i64,
+                                  _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f,
+                                  _int, _int, _vp, _sz, _vp]),
     "sp_layernorm": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _f, _int, _int, _vp]),
     "sp_layernorm_add": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f, _int, _int, _vp]),
     "sp_layernorm_modulate": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _f, _int, _int,

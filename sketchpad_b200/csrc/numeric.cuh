@@ -1,0 +1,40 @@
+// numeric.cuh -- element conversions shared by the token-decoding kernels (rms_norm.cu,
+// int4_linear.cu, paged_kv.cu): f32 <-> {f32, f16, bf16} and f32 -> e4m3 by value.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+namespace sp {
+
+constexpr float kE4m3Max = 448.f;
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// Two e4m3 bytes (a low) of two f32 values: round to nearest even, finite values saturate at
+// +-448, NaN stays NaN.
+__device__ __forceinline__ uint16_t e4m3x2_from_f32(float a, float b) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+
+// max of two values that keeps a NaN (fmaxf drops it)
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+}  // namespace sp

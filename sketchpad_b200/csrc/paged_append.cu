@@ -1,0 +1,184 @@
+// paged_append.cu -- the new tokens of a step enter the paged cache: rotary embedding of q and
+// k (interleaved pairs, the (cos, sin) table of the projection GEMMs' RoPE epilogue,
+// crates/sketchpad-dit/src/rope.rs:145-170) and k, v written to their slots.
+//
+//   (x0, x1) -> (x0 c - x1 s, x1 c + x0 s),  (c, s) = table[position, pair]
+//   e4m3 caches hold e4m3(value / scale[head])
+//
+// Bound by HBM for prompts (q read and written, k and v read and written once) and by latency
+// for single tokens.  One block per token: a thread owns eight values at one place of a head
+// and walks the heads, so the token's position, page and (cos, sin) pairs are loaded once for
+// all of its heads.
+#include "common.cuh"
+#include "numeric.cuh"
+#include "paged_kv.cuh"
+
+namespace sp {
+namespace {
+
+constexpr int kAppThreads = 256;
+
+struct AppendArgs {
+  PagedCache c;
+  const void* q;  // or null (hq = 0)
+  const void* k;
+  const void* v;
+  void* q_out;
+  const int32_t* seq_ids;
+  const int32_t* positions;
+  const float2* rope;  // [rope_rows, D / 2] or null
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;  // input strides, elements
+  int32_t rope_rows;
+  int32_t hq, hkv, D;
+};
+
+template <typename T>
+struct V8 {
+  T e[8];
+};
+
+// A token outside its sequence (seq id, position, page or rope row that does not exist) is
+// padding: nothing of it enters the cache, and its q comes out as zeros.
+template <typename T, bool E4M3>
+__global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendArgs a) {
+  const int64_t t = blockIdx.x;
+  const int lanes = a.D >> 3;                   // threads per head
+  const int slots = kAppThreads / lanes;        // heads in flight
+  const int lane = threadIdx.x % lanes, slot = threadIdx.x / lanes;
+  if (slot >= slots) return;
+  const int heads = a.hq + 2 * a.hkv;
+  const int32_t seq = a.seq_ids[t], pos = a.positions[t];
+  bool live = pos >= 0 && seq >= 0 && seq < a.c.table_rows;
+  if (a.rope) live = live && pos < a.rope_rows;
+  int32_t page = -1, in_page = 0;
+  if (live) {
+    const int32_t col = a.c.page_size.div(pos);
+    in_page = pos - col * a.c.page_size.d;
+    live = col < a.c.table_cols;
+    if (live) page = a.c.table[seq * a.c.table_stride + col];
+    live = live && page >= 0 && page < a.c.pages;
+  }
+  float cs[8];
+  if (a.rope && live) {
+    const float4* r = reinterpret_cast<const float4*>(a.rope + (int64_t)pos * (a.D >> 1)) + 2 * lane;
+    const float4 r0 = __ldg(r), r1 = __ldg(r + 1);
+    cs[0] = r0.x, cs[1] = r0.y, cs[2] = r0.z, cs[3] = r0.w;
+    cs[4] = r1.x, cs[5] = r1.y, cs[6] = r1.z, cs[7] = r1.w;
+  }
+  const int d0 = lane * 8;
+  for (int h = slot; h < heads; h += slots) {
+    const bool is_q = h < a.hq;
+    const bool is_k = !is_q && h < a.hq + a.hkv;
+    const int hk = h - a.hq - (is_k ? 0 : a.hkv);
+    if (!live) {
+      if (is_q)
+        reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (t * a.hq + h) * a.D + d0)[0] =
+            make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const T* src = is_q   ? static_cast<const T*>(a.q) + t * a.q_tok + h * a.q_head
+                   : is_k ? static_cast<const T*>(a.k) + t * a.k_tok + hk * a.k_head
+                          : static_cast<const T*>(a.v) + t * a.v_tok + hk * a.v_head;
+    V8<T> x;
+    *reinterpret_cast<uint4*>(&x) = *reinterpret_cast<const uint4*>(src + d0);
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f32(x.e[i]);
+    if (a.rope && (is_q || is_k)) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float x0 = f[i], x1 = f[i + 1];
+        f[i] = x0 * cs[i] - x1 * cs[i + 1];
+        f[i + 1] = x1 * cs[i] + x0 * cs[i + 1];
+      }
+    }
+    if (E4M3 && !is_q) {
+      const float s = is_k ? a.c.k_scale[hk] : a.c.v_scale[hk];
+      uint16_t o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = e4m3x2_from_f32(f[2 * i] / s, f[2 * i + 1] / s);
+      const int64_t at = is_k ? page * a.c.k_page + in_page * a.c.k_slot + hk * a.c.k_head
+                              : page * a.c.v_page + in_page * a.c.v_slot + hk * a.c.v_head;
+      uint8_t* dst = static_cast<uint8_t*>(is_k ? a.c.k : a.c.v) + at + d0;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(o[0] | (uint32_t)o[1] << 16,
+                                                  o[2] | (uint32_t)o[3] << 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x.e[i] = from_f32<T>(f[i]);
+      T* dst;
+      if (is_q) {
+        dst = static_cast<T*>(a.q_out) + (t * a.hq + h) * a.D;
+      } else {
+        const int64_t at = is_k ? page * a.c.k_page + in_page * a.c.k_slot + hk * a.c.k_head
+                                : page * a.c.v_page + in_page * a.c.v_slot + hk * a.c.v_head;
+        dst = static_cast<T*>(is_k ? a.c.k : a.c.v) + at;
+      }
+      *reinterpret_cast<uint4*>(dst + d0) = *reinterpret_cast<uint4*>(&x);
+    }
+  }
+}
+
+}  // namespace
+}  // namespace sp
+
+extern "C" int sp_paged_kv_append(const void* q, const void* k, const void* v, void* q_out,
+                                  const int64_t q_strides[4], const int64_t k_in_strides[4],
+                                  const int64_t v_in_strides[4], int64_t tokens, int64_t hq,
+                                  int64_t hkv, int64_t D, void* k_cache, void* v_cache,
+                                  const float* k_scale, const float* v_scale,
+                                  const int64_t k_strides[4], const int64_t v_strides[4],
+                                  int64_t pages, int64_t page_size, const void* block_table,
+                                  int64_t table_rows, int64_t table_cols, int64_t table_stride,
+                                  const void* seq_ids, const void* positions,
+                                  const float* rope_cos_sin, int64_t rope_rows, int dtype,
+                                  int cache_dtype, void* stream) {
+  using namespace sp;
+  clear_error();
+  AppendArgs a{};
+  if (!k_in_strides || !v_in_strides || (tokens != 0 && (!k || !v || !seq_ids || !positions)))
+    return set_error(SP_ERR_INVALID_ARG, "paged append: null pointer");
+  if ((q == nullptr) != (q_out == nullptr) || (q && (!q_strides || hq <= 0)))
+    return set_error(SP_ERR_INVALID_ARG, "paged append: q, q_out and its heads come together");
+  if (tokens < 0 || tokens > 2147483647LL || hq < 0 || hq > (1 << 20) || hkv > (1 << 20))
+    return set_error(SP_ERR_INVALID_ARG, "paged append: bad token or head count");
+  if (int rc = make_paged_cache(a.c, "paged append", k_cache, v_cache, k_scale, v_scale, k_strides,
+                                v_strides, pages, page_size, hkv, D, cache_dtype, block_table,
+                                table_rows, table_cols, table_stride))
+    return rc;
+  if (dtype != SP_F16 && dtype != SP_BF16)
+    return set_error(SP_ERR_DTYPE, "paged append: q, k and v are f16 or bf16");
+  if (cache_dtype != SP_E4M3 && cache_dtype != dtype)
+    return set_error(SP_ERR_DTYPE, "paged append: the cache is e4m3 or of the inputs' type");
+  const int64_t* ins[3] = {q ? q_strides : k_in_strides, k_in_strides, v_in_strides};
+  for (const int64_t* st : ins)
+    if (st[2] != 1 || st[0] % 8 || st[1] % 8)
+      return set_error(SP_ERR_ALIGN, "paged append: heads of q, k, v must be contiguous and "
+                       "strides multiples of 8 elements");
+  if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(q_out, 16) ||
+      !aligned(rope_cos_sin, 16) || !aligned(seq_ids, 4) || !aligned(positions, 4))
+    return set_error(SP_ERR_ALIGN, "paged append: pointers must be 16-byte aligned");
+  if (rope_cos_sin && (rope_rows <= 0 || rope_rows > 2147483647LL))
+    return set_error(SP_ERR_INVALID_ARG, "paged append: bad rope table");
+  if (tokens == 0) return SP_OK;
+  if (int rc = require_sm100()) return rc;
+  a.q = q, a.k = k, a.v = v, a.q_out = q_out;
+  a.seq_ids = static_cast<const int32_t*>(seq_ids);
+  a.positions = static_cast<const int32_t*>(positions);
+  a.rope = reinterpret_cast<const float2*>(rope_cos_sin);
+  a.rope_rows = (int32_t)rope_rows;
+  if (q) a.q_tok = q_strides[0], a.q_head = q_strides[1];
+  a.k_tok = k_in_strides[0], a.k_head = k_in_strides[1];
+  a.v_tok = v_in_strides[0], a.v_head = v_in_strides[1];
+  a.hq = q ? (int32_t)hq : 0, a.hkv = (int32_t)hkv, a.D = (int32_t)D;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const unsigned grid = (unsigned)tokens;
+  const bool f8 = cache_dtype == SP_E4M3;
+  if (dtype == SP_F16) {
+    if (f8) paged_append_kernel<__half, true><<<grid, kAppThreads, 0, s>>>(a);
+    else paged_append_kernel<__half, false><<<grid, kAppThreads, 0, s>>>(a);
+  } else {
+    if (f8) paged_append_kernel<__nv_bfloat16, true><<<grid, kAppThreads, 0, s>>>(a);
+    else paged_append_kernel<__nv_bfloat16, false><<<grid, kAppThreads, 0, s>>>(a);
+  }
+  return check_launch("paged append");
+}

@@ -1,0 +1,289 @@
+// rms_norm.cu -- root-mean-square norm of x (+ residual), output in x's type or in e4m3 with
+// one f32 scale per row.
+//
+//   r = T(x + residual)          (kept: the residual stream of the next layer)
+//   y = r / sqrt(mean(r^2) + eps) * w
+//   e4m3: s = max|y| / 448 (1 when the row is all zero), q = e4m3(y / s)
+//
+// Bound by HBM: a row is read once, held in registers across the two block reductions (sum of
+// squares, then max|y|), and written once.  One block per row: with 16-byte vectors a thread
+// holds one to eight of them, so a block has just the threads that its row needs and several
+// rows share an SM, one loading while another reduces.  All arithmetic is f32.
+#include "common.cuh"
+#include "numeric.cuh"
+
+namespace sp {
+namespace {
+
+struct RmsArgs {
+  const void* x;
+  const void* res;   // or null
+  const void* w;     // or null (all ones)
+  void* y;           // T, or e4m3 bytes
+  void* res_out;     // or null
+  float* scale;      // e4m3 only
+  int64_t x_stride, res_stride;  // elements
+  int n;
+  float eps;
+};
+
+// Sum (or NaN-keeping maximum) over the block; every thread gets it.  `slots`: 33 floats.
+template <bool MAX>
+__device__ __forceinline__ float block_reduce(float v, float* slots) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float u = __shfl_xor_sync(0xffffffffu, v, o);
+    v = MAX ? max_nan(v, u) : v + u;
+  }
+  if (nw == 1) return v;
+  if (lane == 0) slots[warp] = v;
+  __syncthreads();
+  v = lane < nw ? slots[lane] : 0.f;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float u = __shfl_xor_sync(0xffffffffu, v, o);
+    v = MAX ? max_nan(v, u) : v + u;
+  }
+  return v;
+}
+
+// The row's e4m3 scale.  Kept a normal number, so that 1 / scale is finite.
+__device__ __forceinline__ float row_scale(float amax) {
+  return amax == 0.f ? 1.f : max_nan(amax / kE4m3Max, 1.17549435e-38f);
+}
+
+// VE consecutive elements of T as one access (VE * sizeof(T) bytes: 32 as two 16-byte halves).
+template <typename T, int VE>
+struct Vec {
+  T e[VE];
+};
+template <typename T, int VE>
+__device__ __forceinline__ void load_vec(Vec<T, VE>& v, const T* p) {
+  constexpr int BYTES = VE * sizeof(T);
+  if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i)
+      reinterpret_cast<uint4*>(&v)[i] = reinterpret_cast<const uint4*>(p)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) v.e[i] = p[i];
+  }
+}
+template <typename T, int VE>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, VE>& v) {
+  constexpr int BYTES = VE * sizeof(T);
+  if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i)
+      reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(&v)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) p[i] = v.e[i];
+  }
+}
+
+// The row in registers: VPT vectors of VE elements per thread, n <= VPT * VE * blockDim.x and
+// n a multiple of VE.  A thread reads its elements before it writes them, so y may be x and
+// res_out may be x or residual.
+template <typename T, int VE, int VPT, bool FP8>
+__global__ void __launch_bounds__(1024) rms_reg_kernel(const RmsArgs a) {
+  __shared__ float sum_slots[33], max_slots[33];
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const T* res = a.res ? static_cast<const T*>(a.res) + row * a.res_stride : nullptr;
+  const T* w = static_cast<const T*>(a.w);
+  const int step = blockDim.x * VE;
+  Vec<T, VE> v[VPT], rv[VPT], wv[VPT];
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int i = threadIdx.x * VE + j * step;
+    if (i < a.n) {
+      load_vec(v[j], x + i);
+      if (res) load_vec(rv[j], res + i);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int i = threadIdx.x * VE + j * step;
+    if (i < a.n && w) load_vec(wv[j], w + i);
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int i = threadIdx.x * VE + j * step;
+    if (i < a.n) {
+#pragma unroll
+      for (int t = 0; t < VE; ++t) {
+        if (res) v[j].e[t] = from_f32<T>(to_f32(v[j].e[t]) + to_f32(rv[j].e[t]));
+        const float f = to_f32(v[j].e[t]);
+        ss += f * f;
+      }
+      if (a.res_out)
+        store_vec(static_cast<T*>(a.res_out) + row * a.n + i, v[j]);
+    }
+  }
+  const float rstd = rsqrtf(block_reduce<false>(ss, sum_slots) / (float)a.n + a.eps);
+  if constexpr (!FP8) {
+    T* y = static_cast<T*>(a.y) + row * a.n;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int i = threadIdx.x * VE + j * step;
+      if (i < a.n) {
+#pragma unroll
+        for (int t = 0; t < VE; ++t)
+          v[j].e[t] = from_f32<T>(to_f32(v[j].e[t]) * rstd * (w ? to_f32(wv[j].e[t]) : 1.f));
+        store_vec(y + i, v[j]);
+      }
+    }
+  } else {
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int i = threadIdx.x * VE + j * step;
+      if (i < a.n) {
+#pragma unroll
+        for (int t = 0; t < VE; ++t)
+          amax = max_nan(amax, fabsf(to_f32(v[j].e[t]) * rstd * (w ? to_f32(wv[j].e[t]) : 1.f)));
+      }
+    }
+    amax = block_reduce<true>(amax, max_slots);
+    const float s = row_scale(amax);
+    const float inv = 1.f / s;
+    if (threadIdx.x == 0) a.scale[row] = s;
+    uint8_t* q = static_cast<uint8_t*>(a.y) + row * a.n;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int i = threadIdx.x * VE + j * step;
+      if (i < a.n) {
+        if constexpr (VE == 8) {
+          uint16_t o[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const float f0 = to_f32(v[j].e[2 * t]) * rstd * (w ? to_f32(wv[j].e[2 * t]) : 1.f);
+            const float f1 =
+                to_f32(v[j].e[2 * t + 1]) * rstd * (w ? to_f32(wv[j].e[2 * t + 1]) : 1.f);
+            o[t] = e4m3x2_from_f32(f0 * inv, f1 * inv);
+          }
+          *reinterpret_cast<uint2*>(q + i) = make_uint2(o[0] | (uint32_t)o[1] << 16,
+                                                        o[2] | (uint32_t)o[3] << 16);
+        } else {
+#pragma unroll
+          for (int t = 0; t < VE; ++t) {
+            const float f = to_f32(v[j].e[t]) * rstd * (w ? to_f32(wv[j].e[t]) : 1.f);
+            q[i + t] = (uint8_t)e4m3x2_from_f32(f * inv, 0.f);
+          }
+        }
+      }
+    }
+  }
+}
+
+// Rows too long for the registers of a block: the row is read again for each phase (from L2).
+// r is rounded to T, so re-forming it from x and residual gives the same value; with res_out
+// given it is read back from there, since that may be the very memory of x or residual (each
+// thread reads and writes only its own elements).
+template <typename T, bool FP8>
+__global__ void __launch_bounds__(1024) rms_long_kernel(const RmsArgs a) {
+  __shared__ float sum_slots[33], max_slots[33];
+  const int64_t row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const T* res = a.res ? static_cast<const T*>(a.res) + row * a.res_stride : nullptr;
+  const T* w = static_cast<const T*>(a.w);
+  T* ro = a.res_out ? static_cast<T*>(a.res_out) + row * a.n : nullptr;
+  float ss = 0.f;
+  for (int i = threadIdx.x; i < a.n; i += blockDim.x) {
+    T v = x[i];
+    if (res) v = from_f32<T>(to_f32(v) + to_f32(res[i]));
+    if (ro) ro[i] = v;
+    ss += to_f32(v) * to_f32(v);
+  }
+  const float rstd = rsqrtf(block_reduce<false>(ss, sum_slots) / (float)a.n + a.eps);
+  auto y_at = [&](int i) {
+    T v = ro ? ro[i] : x[i];
+    if (!ro && res) v = from_f32<T>(to_f32(v) + to_f32(res[i]));
+    return to_f32(v) * rstd * (w ? to_f32(w[i]) : 1.f);
+  };
+  if constexpr (!FP8) {
+    T* y = static_cast<T*>(a.y) + row * a.n;
+    for (int i = threadIdx.x; i < a.n; i += blockDim.x) y[i] = from_f32<T>(y_at(i));
+  } else {
+    float amax = 0.f;
+    for (int i = threadIdx.x; i < a.n; i += blockDim.x) amax = max_nan(amax, fabsf(y_at(i)));
+    amax = block_reduce<true>(amax, max_slots);
+    const float s = row_scale(amax);
+    const float inv = 1.f / s;
+    if (threadIdx.x == 0) a.scale[row] = s;
+    uint8_t* q = static_cast<uint8_t*>(a.y) + row * a.n;
+    for (int i = threadIdx.x; i < a.n; i += blockDim.x)
+      q[i] = (uint8_t)e4m3x2_from_f32(y_at(i) * inv, 0.f);
+  }
+}
+
+template <typename T, bool FP8>
+int launch_rms(const RmsArgs& a, int64_t rows, cudaStream_t s) {
+  constexpr int64_t es = sizeof(T);
+  const bool vec = a.n % 8 == 0 && aligned(a.x, 16) && aligned(a.w, 16) &&
+                   aligned(a.res_out, 16) && aligned(a.y, FP8 ? 8 : 16) &&
+                   (a.x_stride * es) % 16 == 0 &&
+                   (!a.res || (aligned(a.res, 16) && (a.res_stride * es) % 16 == 0));
+  const unsigned grid = (unsigned)rows;
+  auto threads = [](int items) { return (unsigned)((items + 31) / 32 * 32); };
+  if (vec) {
+    const int nv = a.n / 8;
+    if (nv <= 512) rms_reg_kernel<T, 8, 1, FP8><<<grid, threads(nv), 0, s>>>(a);
+    else if (nv <= 1024) rms_reg_kernel<T, 8, 2, FP8><<<grid, threads((nv + 1) / 2), 0, s>>>(a);
+    else if (nv <= 4096) rms_reg_kernel<T, 8, 4, FP8><<<grid, threads((nv + 3) / 4), 0, s>>>(a);
+    else rms_long_kernel<T, FP8><<<grid, 1024, 0, s>>>(a);
+  } else {
+    if (a.n <= 1024) rms_reg_kernel<T, 1, 4, FP8><<<grid, threads((a.n + 3) / 4), 0, s>>>(a);
+    else if (a.n <= 8192) rms_reg_kernel<T, 1, 8, FP8><<<grid, threads((a.n + 7) / 8), 0, s>>>(a);
+    else rms_long_kernel<T, FP8><<<grid, 1024, 0, s>>>(a);
+  }
+  return check_launch("rms norm");
+}
+
+template <bool FP8>
+int rms_entry(const RmsArgs& a, int64_t rows, int64_t n, int dtype, void* stream) {
+  clear_error();
+  if (rows != 0 && (!a.x || !a.y || (FP8 && !a.scale)))
+    return set_error(SP_ERR_INVALID_ARG, "rms norm: null pointer");
+  if (rows < 0 || n <= 0) return set_error(SP_ERR_INVALID_ARG, "rms norm: bad shape rows=%lld n=%lld",
+                                           (long long)rows, (long long)n);
+  if (rows > 2147483647LL || n > (1LL << 30))
+    return set_error(SP_ERR_SHAPE, "rms norm: rows=%lld n=%lld too large", (long long)rows,
+                     (long long)n);
+  if (a.x_stride < n || (a.res && a.res_stride < n))
+    return set_error(SP_ERR_SHAPE, "rms norm: a row stride is below the row's %lld values",
+                     (long long)n);
+  if (!dtype_size(dtype)) return set_error(SP_ERR_DTYPE, "rms norm: unknown dtype %d", dtype);
+  if (rows == 0) return SP_OK;
+  if (int rc = require_sm100()) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case SP_F32: return launch_rms<float, FP8>(a, rows, s);
+    case SP_F16: return launch_rms<__half, FP8>(a, rows, s);
+    default: return launch_rms<__nv_bfloat16, FP8>(a, rows, s);
+  }
+}
+
+}  // namespace
+}  // namespace sp
+
+extern "C" int sp_rms_norm(const void* x, int64_t x_row_stride, const void* residual,
+                           int64_t residual_row_stride, const void* weight, void* y,
+                           void* residual_out, int64_t rows, int64_t n, float eps, int dtype,
+                           void* stream) {
+  const sp::RmsArgs a{x, residual, weight, y, residual_out, nullptr, x_row_stride,
+                      residual_row_stride, (int)n, eps};
+  return sp::rms_entry<false>(a, rows, n, dtype, stream);
+}
+
+extern "C" int sp_rms_norm_fp8(const void* x, int64_t x_row_stride, const void* residual,
+                               int64_t residual_row_stride, const void* weight, void* q,
+                               float* scale, void* residual_out, int64_t rows, int64_t n,
+                               float eps, int dtype, void* stream) {
+  const sp::RmsArgs a{x, residual, weight, q, residual_out, scale, x_row_stride,
+                      residual_row_stride, (int)n, eps};
+  return sp::rms_entry<true>(a, rows, n, dtype, stream);
+}
