@@ -243,27 +243,30 @@ extern "C" {
         scale_dtype: c_int, bias: *const c_void, y: *mut c_void, M: i64, N: i64, K: i64,
         group: i64, out_dtype: c_int, stream: *mut c_void
     ) -> c_int;
+    pub fn sp_paged_cache_create(
+        k: *mut c_void, v: *mut c_void, k_scale: *const c_float, v_scale: *const c_float,
+        k_strides: *const i64, v_strides: *const i64, pages: i64, page_size: i64, hkv: i64,
+        D: i64, dtype: c_int, cache: *mut *mut c_void
+    ) -> c_int;
+    pub fn sp_paged_cache_destroy(
+        cache: *mut c_void
+    ) -> c_int;
     pub fn sp_paged_kv_append(
-        q: *const c_void, k: *const c_void, v: *const c_void, q_out: *mut c_void, q_strides:
-        *const i64, k_in_strides: *const i64, v_in_strides: *const i64, tokens: i64, hq:
-        i64, hkv: i64, D: i64, k_cache: *mut c_void, v_cache: *mut c_void, k_scale: *const
-        c_float, v_scale: *const c_float, k_strides: *const i64, v_strides: *const i64,
-        pages: i64, page_size: i64, block_table: *const c_void, table_rows: i64, table_cols:
-        i64, table_stride: i64, seq_ids: *const c_void, positions: *const c_void,
-        rope_cos_sin: *const c_float, rope_rows: i64, dtype: c_int, cache_dtype: c_int,
-        stream: *mut c_void
+        cache: *const c_void, q: *const c_void, k: *const c_void, v: *const c_void, q_out:
+        *mut c_void, q_token_stride: i64, q_head_stride: i64, k_token_stride: i64,
+        k_head_stride: i64, v_token_stride: i64, v_head_stride: i64, tokens: i64, hq: i64,
+        block_table: *const c_void, table_rows: i64, table_cols: i64, table_stride: i64,
+        seq_ids: *const c_void, positions: *const c_void, rope_cos_sin: *const c_float,
+        rope_rows: i64, dtype: c_int, stream: *mut c_void
     ) -> c_int;
     pub fn sp_paged_attention_workspace_size(
         B: i64, hq: i64, hkv: i64
     ) -> usize;
     pub fn sp_paged_attention(
-        q: *const c_void, q_strides: *const i64, k_cache: *const c_void, v_cache: *const
-        c_void, k_scale: *const c_float, v_scale: *const c_float, k_strides: *const i64,
-        v_strides: *const i64, block_table: *const c_void, table_cols: i64, table_stride:
-        i64, seq_lens: *const c_void, out: *mut c_void, B: i64, hq: i64, hkv: i64, D: i64,
-        pages: i64, page_size: i64, window: i64, sinks: i64, scale: c_float, dtype: c_int,
-        cache_dtype: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut
-        c_void
+        cache: *const c_void, q: *const c_void, q_seq_stride: i64, q_head_stride: i64,
+        block_table: *const c_void, table_cols: i64, table_stride: i64, seq_lens: *const
+        c_void, out: *mut c_void, B: i64, hq: i64, window: i64, sinks: i64, scale: c_float,
+        dtype: c_int, workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void
     ) -> c_int;
     // -- LayerNorm (crates/sketchpad-core/src/layernorm.rs:63-73: unbiased variance)
     pub fn sp_layernorm(

@@ -478,51 +478,54 @@ int sp_int4_linear(const void* x, int64_t x_row_stride, int x_dtype, const float
                    int scale_dtype, const void* bias, void* y, int64_t M, int64_t N, int64_t K,
                    int64_t group, int out_dtype, void* stream);
 
-/* A paged key-value cache: k_cache, v_cache [pages, page_size, hkv, D] with element strides
- * (innermost 1, the others multiples of 16 bytes, pointers 16-byte aligned), D a multiple of 16
- * up to 256, f16, bf16 or e4m3 (then k_scale, v_scale [hkv] f32: value = e4m3 * scale).
+/* A paged key-value cache: k and v [pages, page_size, hkv, D] with element strides (innermost
+ * 1, the others multiples of 16 bytes, pointers 16-byte aligned), D a multiple of 16 up to 256,
+ * f16, bf16 or e4m3 (then k_scale, v_scale [hkv] f32: value = e4m3 * scale; NULL otherwise).
+ * sp_paged_cache_create checks and describes it in a host object (no device memory, no copy:
+ * k, v and the scales stay the caller's and have to outlive the handle's use), which any thread
+ * and stream may use at once; destroy takes NULL.
+ *
  * block_table [table_rows, table_cols] int32, row stride table_stride: the page of token t of
  * sequence b is block_table[b, t / page_size]; an entry outside [0, pages) is a page that is
- * not there.
- *
- * sp_paged_kv_append: token i (of `tokens`) of sequence seq_ids[i] at positions[i] (int32): k
- * and v [tokens, hkv, D] enter the cache at its slot, q [tokens, hq, D] comes out in q_out
- * (contiguous; q and q_out NULL: none).  rope_cos_sin [rope_rows, D/2, 2] f32 (cos, sin), or
- * NULL: q and k are rotated as sp_q8_0_linear_rope rotates (pairs (2i, 2i+1), row =
- * position).  A token whose sequence, position, page or table row does not exist is padding:
- * nothing is stored and its q_out is zeros.  dtype: q, k, v, q_out f16 or bf16; the cache is of
- * that type or e4m3.  Input strides (token, head, 1, unused) in elements, multiples of 8.  Two
- * tokens of one call must not share a slot. */
-int sp_paged_kv_append(const void* q, const void* k, const void* v, void* q_out,
-                       const int64_t q_strides[4], const int64_t k_in_strides[4],
-                       const int64_t v_in_strides[4], int64_t tokens, int64_t hq, int64_t hkv,
-                       int64_t D, void* k_cache, void* v_cache, const float* k_scale,
-                       const float* v_scale, const int64_t k_strides[4],
-                       const int64_t v_strides[4], int64_t pages, int64_t page_size,
-                       const void* block_table, int64_t table_rows, int64_t table_cols,
-                       int64_t table_stride, const void* seq_ids, const void* positions,
-                       const float* rope_cos_sin, int64_t rope_rows, int dtype, int cache_dtype,
-                       void* stream);
+ * not there. */
+int sp_paged_cache_create(void* k, void* v, const float* k_scale, const float* v_scale,
+                          const int64_t k_strides[4], const int64_t v_strides[4], int64_t pages,
+                          int64_t page_size, int64_t hkv, int64_t D, int dtype, void** cache);
+int sp_paged_cache_destroy(void* cache);
+
+/* The new tokens enter the cache: token i (of `tokens`) of sequence seq_ids[i] at positions[i]
+ * (int32).  k and v [tokens, hkv, D] are stored at its slot, q [tokens, hq, D] comes out in
+ * q_out (contiguous; may be q; q and q_out NULL: none).  rope_cos_sin [rope_rows, D/2, 2] f32
+ * (cos, sin), or NULL: q and k are rotated as sp_q8_0_linear_rope rotates (pairs (2i, 2i+1),
+ * table row = position).  A token whose sequence, position, page or table row does not exist is
+ * padding: nothing is stored and its q_out is zeros.  dtype: q, k, v, q_out f16 or bf16; the
+ * cache is of that type or e4m3.  Strides of q, k, v in elements, multiples of 8, heads
+ * contiguous and 16-byte aligned.  Two tokens of one call must not share a slot. */
+int sp_paged_kv_append(const void* cache, const void* q, const void* k, const void* v, void* q_out,
+                       int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                       int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                       int64_t tokens, int64_t hq, const void* block_table, int64_t table_rows,
+                       int64_t table_cols, int64_t table_stride, const void* seq_ids,
+                       const void* positions, const float* rope_cos_sin, int64_t rope_rows,
+                       int dtype, void* stream);
 
 /* Attention of one new token per sequence over the cache: out[b, h] = softmax(scale q[b, h] .
  * k_j) v_j over the visible tokens j < seq_lens[b] (int32; the new token's own k and v are in
  * the cache, and lengths beyond the table are cut).  window > 0: only j >= seq_lens[b] - window
  * and j < sinks.  Tokens on pages that are not there are not seen; a sequence that sees none
- * gives zeros.  q [B, hq, D] with strides (sequence, head, 1, unused), heads 4-byte aligned;
- * out [B, hq, D] contiguous; q and out of `dtype` (f16, bf16), the cache of that type or e4m3;
- * query head h reads cache head h / (hq / hkv).  scale <= 0 selects 1/sqrt(D).
+ * gives zeros.  q [B, hq, D] with strides (multiples of 2 elements, heads contiguous and 4-byte
+ * aligned); out [B, hq, D] contiguous; q and out of `dtype` (f16, bf16), the cache of that type
+ * or e4m3; block_table has B rows; query head h reads cache head h / (hq / hkv).  scale <= 0
+ * selects 1/sqrt(D).
  * workspace: sp_paged_attention_workspace_size() bytes, 16-byte aligned, ZERO before its first
  * use (each call leaves its counters zero again) and not in use by another call in flight;
  * calls of any sizes that fit may share it. */
 size_t sp_paged_attention_workspace_size(int64_t B, int64_t hq, int64_t hkv);
-int sp_paged_attention(const void* q, const int64_t q_strides[4], const void* k_cache,
-                       const void* v_cache, const float* k_scale, const float* v_scale,
-                       const int64_t k_strides[4], const int64_t v_strides[4],
-                       const void* block_table, int64_t table_cols, int64_t table_stride,
-                       const void* seq_lens, void* out, int64_t B, int64_t hq, int64_t hkv,
-                       int64_t D, int64_t pages, int64_t page_size, int64_t window, int64_t sinks,
-                       float scale, int dtype, int cache_dtype, void* workspace,
-                       size_t workspace_bytes, void* stream);
+int sp_paged_attention(const void* cache, const void* q, int64_t q_seq_stride,
+                       int64_t q_head_stride, const void* block_table, int64_t table_cols,
+                       int64_t table_stride, const void* seq_lens, void* out, int64_t B,
+                       int64_t hq, int64_t window, int64_t sinks, float scale, int dtype,
+                       void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

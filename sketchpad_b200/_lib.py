@@ -103,13 +103,15 @@ SIGNATURES = {
     "sp_int4_dequant": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _int, _vp]),
     "sp_int4_linear": (_int, [_vp, _i64, _int, _vp, _vp, _vp, _vp, _int, _vp, _vp, _i64, _i64,
                               _i64, _i64, _int, _vp]),
-    "sp_paged_kv_append": (_int, [_vp, _vp, _vp, _vp, _i64p, _i64p, _i64p, _i64, _i64, _i64, _i64,
-                                  _vp, _vp, _vp, _vp, _i64p, _i64p, _i64, _i64, _vp, _i64, _i64,
-                                  _i64, _vp, _vp, _vp, _i64, _int, _int, _vp]),
+    "sp_paged_cache_create": (_int, [_vp, _vp, _vp, _vp, _i64p, _i64p, _i64, _i64, _i64, _i64,
+                                     _int, ctypes.POINTER(_vp)]),
+    "sp_paged_cache_destroy": (_int, [_vp]),
+    "sp_paged_kv_append": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64,
+                                  _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _int,
+                                  _vp]),
     "sp_paged_attention_workspace_size": (_sz, [_i64, _i64, _i64]),
-    "sp_paged_attention": (_int, [_vp, _i64p, _vp, _vp, _vp, _vp, _i64p, _i64p, _vp, _i64, _i64,
-                                  _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f,
-                                  _int, _int, _vp, _sz, _vp]),
+    "sp_paged_attention": (_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64,
+                                  _i64, _i64, _f, _int, _vp, _sz, _vp]),
     "sp_layernorm": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _f, _int, _int, _vp]),
     "sp_layernorm_add": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _f, _int, _int, _vp]),
     "sp_layernorm_modulate": (_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _f, _int, _int,
@@ -147,6 +149,24 @@ def call(name: str, *args) -> int:
     if rc != SP_OK:
         raise SketchpadError(name, rc, load().sp_last_error().decode())
     return rc
+
+
+class Entry:
+    """One entry point, bound at its first call: what `call` does, without the lookups that
+    count in the call of a small operator."""
+
+    __slots__ = ("name", "_fn")
+
+    def __init__(self, name: str):
+        self.name, self._fn = name, None
+
+    def __call__(self, *args) -> None:
+        fn = self._fn
+        if fn is None:
+            fn = self._fn = getattr(load(), self.name)
+        rc = fn(*args)
+        if rc != SP_OK:
+            raise SketchpadError(self.name, rc, load().sp_last_error().decode())
 
 
 def i64_array(vals):

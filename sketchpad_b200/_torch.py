@@ -35,6 +35,30 @@ def stream_ptr(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+try:
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:  # a torch built without CUDA: the operators raise before they get here
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
+def raw_stream(index: int) -> int:
+    """The handle of the device's current stream as an int (stream_ptr builds a Stream object
+    first, 2.3 us of a small operator's call)."""
+    return _raw_stream(index)
+
+
+def cuda_index(x: torch.Tensor, *others) -> int:
+    """The device index that x and the others (None: absent) share; ValueError as require_cuda."""
+    i = x.get_device()
+    if i < 0:
+        raise ValueError("sketchpad_b200 ops take CUDA tensors (there is no CPU path)")
+    for t in others:
+        if t is not None and t.get_device() != i:
+            require_cuda(x, *others)
+    return i
+
+
 def ptr(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 

@@ -25,14 +25,16 @@ namespace sp {
 namespace {
 
 constexpr int kI4Warps = 8;
-constexpr int kI4Deep = 4;  // chunks (1 KB) in flight per warp
+constexpr int kI4Deep = 5;  // stages of a warp's ring: four chunks (1 KB) in flight
+constexpr int kMaxSmem = 200 * 1024;
+constexpr double kBlockCost = 3, kJoinCost = 2;  // see choose_split
 
 struct Int4Args {
   const void* x;         // [M, K] f16 / bf16 / e4m3
   const float* x_scale;  // [M], e4m3 only
   const uint4* q;        // [NT, C, 2, 32] 16-byte pieces
   const uint16_t* s;     // [NT, C, 8, 2, GPC]
-  const uint8_t* z;      // same, or null (8)
+  const uint8_t* z;      // [NT, C, 8, ZB] holding [2, GPC], or null (8)
   const void* bias;      // out dtype [N] or null
   void* y;               // [M, N]
   int64_t x_stride;      // elements
@@ -99,31 +101,48 @@ __device__ __forceinline__ void unpack(uint32_t (&p)[4], uint32_t w, uint32_t zo
   }
 }
 
-// The scale and zero bytes of a lane's two rows for one chunk, in one load each.
-template <int BYTES>
-struct Meta {
-  uint32_t r[(BYTES + 3) / 4];
-};
-template <int BYTES>
-__device__ __forceinline__ void load_meta(Meta<BYTES>& m, const uint8_t* p) {
-  if constexpr (BYTES == 16) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    m.r[0] = v.x, m.r[1] = v.y, m.r[2] = v.z, m.r[3] = v.w;
-  } else if constexpr (BYTES == 8) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-    m.r[0] = v.x, m.r[1] = v.y;
-  } else if constexpr (BYTES == 4) {
-    m.r[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-  } else {
-    m.r[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
-  }
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
 }
+// One asynchronous copy of 4, 8 or 16 bytes.
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES)
+                 : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void lds(uint32_t (&r)[(BYTES + 3) / 4], uint32_t addr) {
+  if constexpr (BYTES == 16)
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  else if constexpr (BYTES == 8)
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
+                 : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+  else
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(addr) : "memory");
+}
+
+// A warp's ring: per chunk in flight and lane, its 16 bytes of rows g and of rows g + 8, its
+// scales and its zeros, each lane's own (no lane reads what another one copied).
+template <int GPC, bool ZP>
+struct Ring {
+  static constexpr int SB = 4 * GPC;                      // scales of two rows
+  static constexpr int ZB = ZP ? (GPC == 1 ? 4 : 2 * GPC) : 0;
+  static constexpr int STAGE = 32 * (32 + SB + ZB);
+  static constexpr int WARP = kI4Deep * STAGE;
+  static constexpr int BLOCK = kI4Warps * WARP;
+};
+__host__ __device__ constexpr int zero_bytes(int gpc) { return gpc == 1 ? 4 : 2 * gpc; }
 
 // T: the MMA's type (x's, or f16 for e4m3 x).  NT: n-tiles of 8 rows of x.  GPC: groups per
 // chunk of 128 inputs (4: groups of 32, 2: of 64, 1: of 128 and more).
 template <typename T, bool XE4M3, int NT, int GPC, bool ZP>
-__global__ void __launch_bounds__(kI4Warps * 32) int4_linear_kernel(const Int4Args a) {
+__global__ void __launch_bounds__(kI4Warps * 32, 2) int4_linear_kernel(const Int4Args a) {
   namespace cg = cooperative_groups;
+  using R = Ring<GPC, ZP>;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float red[kI4Warps][16][8 * NT];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -135,6 +154,8 @@ __global__ void __launch_bounds__(kI4Warps * 32) int4_linear_kernel(const Int4Ar
   const int n_tiles = (a.N + 15) / 16;
   const int tile = blockIdx.x * a.wr + wr;
   const int cb = (int)((int64_t)a.C * split / S), ce = (int)((int64_t)a.C * (split + 1) / S);
+  uint8_t* xsm = smem + R::BLOCK;
+  const uint32_t ring = smem_u32(smem) + warp * R::WARP;
 
   float tot[NT][4];
 #pragma unroll
@@ -147,119 +168,121 @@ __global__ void __launch_bounds__(kI4Warps * 32) int4_linear_kernel(const Int4Ar
     const int w0 = p0 + pc * wk / WK;
     const int n_chunks = tile < n_tiles ? p0 + pc * (wk + 1) / WK - w0 : 0;
     const int64_t chunk0 = (int64_t)tile * a.C + w0;
-    const uint4* qp = a.q + chunk0 * 64 + lane;
-    const uint8_t* sp_ = reinterpret_cast<const uint8_t*>(a.s) + (chunk0 * 16 + g * 2) * GPC * 2;
-    const uint8_t* zp = ZP ? a.z + (chunk0 * 16 + g * 2) * GPC : nullptr;
-
-    uint4 w[kI4Deep][2];
-    Meta<GPC * 4> sm[kI4Deep];
-    Meta<GPC * 2> zm[kI4Deep];
-    auto fetch = [&](int u, int i) {
-      if (i < n_chunks) {
-        w[u][0] = __ldcs(qp + (int64_t)i * 64);
-        w[u][1] = __ldcs(qp + (int64_t)i * 64 + 32);
-        load_meta(sm[u], sp_ + (int64_t)i * 16 * GPC * 2);
-        if constexpr (ZP) load_meta(zm[u], zp + (int64_t)i * 16 * GPC);
+    const uint8_t* qp = reinterpret_cast<const uint8_t*>(a.q) + chunk0 * 1024 + lane * 16;
+    const uint8_t* sp_ = reinterpret_cast<const uint8_t*>(a.s) + (chunk0 * 8 + g) * R::SB;
+    const uint8_t* zp = ZP ? a.z + (chunk0 * 8 + g) * R::ZB : nullptr;
+    int copied = 0;  // chunks whose copies have been issued; the pointers stand at the next one
+    auto fetch = [&](uint32_t stage) {
+      if (copied < n_chunks) {
+        cp_async<16>(stage + lane * 16, qp);
+        cp_async<16>(stage + 512 + lane * 16, qp + 512);
+        cp_async<R::SB>(stage + 1024 + lane * R::SB, sp_);
+        if constexpr (ZP) cp_async<R::ZB>(stage + 1024 + 32 * R::SB + lane * R::ZB, zp);
+        qp += 1024;
+        sp_ += 8 * R::SB;
+        if constexpr (ZP) zp += 8 * R::ZB;
+        ++copied;
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
-    for (int u = 0; u < kI4Deep; ++u) fetch(u, u);
+    for (int u = 0; u < kI4Deep - 1; ++u) fetch(ring + u * R::STAGE);
 
-    // ---- x of this pass: row m at m * (256 pc + 64) bytes, 16-byte groups of 8 inputs, group
-    // (j, t) of a chunk (its inputs 32 j + 8 t ..) at place 4 j + t; inputs beyond K are zeros
+    // ---- x of this pass: row m at m * (256 pc + 64) bytes (64 so that two rows' 64-byte
+    // pieces fall into different halves of the banks); inputs beyond K are zeros
     const int xrow = pc * 256 + 64;
     if (p0 != cb) __syncthreads();
-    for (int i = tid; i < mrows * pc * 16; i += kI4Warps * 32) {
-      const int m = i / (pc * 16), grp = i - m * (pc * 16);
-      const int k = p0 * 128 + grp * 8;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (k < a.K) {
-        if constexpr (XE4M3) {
-          const uint2 b = __ldg(reinterpret_cast<const uint2*>(
-              static_cast<const uint8_t*>(a.x) + (int64_t)(m0 + m) * a.x_stride + k));
-          uint32_t* o = reinterpret_cast<uint32_t*>(&v);
-          const uint32_t in[2] = {b.x, b.y};
+    for (int m = 0; m < mrows; ++m)
+      for (int grp = tid; grp < pc * 16; grp += kI4Warps * 32) {
+        const int k = p0 * 128 + grp * 8;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (k < a.K) {
+          if constexpr (XE4M3) {
+            const uint2 b = __ldg(reinterpret_cast<const uint2*>(
+                static_cast<const uint8_t*>(a.x) + (int64_t)(m0 + m) * a.x_stride + k));
+            uint32_t* o = reinterpret_cast<uint32_t*>(&v);
+            const uint32_t in[2] = {b.x, b.y};
 #pragma unroll
-          for (int h = 0; h < 4; ++h)
-            asm("cvt.rn.f16x2.e4m3x2 %0, %1;"
-                : "=r"(o[h]) : "h"((uint16_t)(in[h >> 1] >> (16 * (h & 1)))));
-        } else {
-          v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) +
-                                                   (int64_t)(m0 + m) * a.x_stride + k));
+            for (int h = 0; h < 4; ++h)
+              asm("cvt.rn.f16x2.e4m3x2 %0, %1;"
+                  : "=r"(o[h]) : "h"((uint16_t)(in[h >> 1] >> (16 * (h & 1)))));
+          } else {
+            v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) +
+                                                     (int64_t)(m0 + m) * a.x_stride + k));
+          }
         }
+        *reinterpret_cast<uint4*>(xsm + m * xrow + grp * 16) = v;
       }
-      *reinterpret_cast<uint4*>(smem + m * xrow + grp * 16) = v;
-    }
     __syncthreads();
 
-    const uint8_t* xs = smem + (w0 - p0) * 256 + t4 * 16;
-    for (int i0 = 0; i0 < n_chunks; i0 += kI4Deep) {
+    // lanes beyond the last row of x repeat it: their MMA columns are never stored
+    uint32_t xa[NT];
 #pragma unroll
-      for (int u = 0; u < kI4Deep; ++u) {
-        const int i = i0 + u;
-        if (i >= n_chunks) break;
-        float acc[NT][4];
+    for (int n = 0; n < NT; ++n)
+      xa[n] = smem_u32(xsm) + min(n * 8 + g, mrows - 1) * xrow + (w0 - p0) * 256 + t4 * 16;
+    uint32_t stage = ring, refill = ring + (kI4Deep - 1) * R::STAGE;
+    for (int i = 0; i < n_chunks; ++i) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kI4Deep - 2) : "memory");
+      uint32_t w[2][4], sm[(R::SB + 3) / 4], zm[ZP ? (R::ZB + 3) / 4 : 1];
+      lds<16>(w[0], stage + lane * 16);
+      lds<16>(w[1], stage + 512 + lane * 16);
+      lds<R::SB>(sm, stage + 1024 + lane * R::SB);
+      if constexpr (ZP) lds<R::ZB>(zm, stage + 1024 + 32 * R::SB + lane * R::ZB);
+      fetch(refill);  // the stage that the previous step has read
+      refill = stage;
+      stage = stage + R::STAGE == ring + R::WARP ? ring : stage + R::STAGE;
+      float acc[NT][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          constexpr int JPG = 4 / GPC;  // words per group
-          const int grp = j / JPG;
-          if (j % JPG == 0) {
+      for (int j = 0; j < 4; ++j) {
+        constexpr int JPG = 4 / GPC;  // words per group
+        const int grp = j / JPG;
+        if (j % JPG == 0) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+            for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
+        }
+        uint32_t p[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          constexpr uint32_t magic = std::is_same_v<T, __half> ? 0x64006400u : 0x43004300u;
+          uint32_t zz = 0x00080008u;
+          if constexpr (ZP) {
+            const int at = h * GPC + grp;
+            zz = (zm[at >> 2] >> (8 * (at & 3))) & 0xffu;
+            zz |= zz << 16;
           }
-          uint32_t zoff[2], zoff16[2];
+          // -(64 + z): 0xd400 is -64 in f16, whose mantissa counts in 1/16
+          unpack<T>(p[h], w[h][j], magic | zz, 0xd400d400u + (zz << 4));
+        }
+        const uint32_t a0[4] = {p[0][0], p[1][0], p[0][1], p[1][1]};
+        const uint32_t a1[4] = {p[0][2], p[1][2], p[0][3], p[1][3]};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          uint32_t b[4];
+          lds<16>(b, xa[n] + j * 64);
+          mma_i4<T>(acc[n], a0, b[0], b[1]);
+          mma_i4<T>(acc[n], a1, b[2], b[3]);
+        }
+        if (j % JPG == JPG - 1) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            constexpr uint32_t magic = std::is_same_v<T, __half> ? 0x64006400u : 0x43004300u;
-            uint32_t z = 8;
-            if constexpr (ZP) {
-              const int at = h * GPC + grp;
-              z = (zm[u].r[at >> 2] >> (8 * (at & 3))) & 0xffu;
+            const int at = h * GPC + grp;
+            const uint32_t bits = (sm[at >> 1] >> (16 * (at & 1))) & 0xffffu;
+            const float sc = a.s_bf16 ? __uint_as_float(bits << 16)
+                                      : __half2float(__ushort_as_half((unsigned short)bits));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              tot[n][2 * h] += sc * acc[n][2 * h];
+              tot[n][2 * h + 1] += sc * acc[n][2 * h + 1];
             }
-            zoff[h] = magic | z | z << 16;
-            if constexpr (std::is_same_v<T, __half>) {
-              // -(64 + z): 0xd400 is -64, whose mantissa counts in 1/16
-              const uint32_t zz = 0xd400u + (z << 4);
-              zoff16[h] = zz | zz << 16;
-            } else {
-              zoff16[h] = 0;
-            }
-          }
-          uint32_t lo[4], hi[4];
-          const uint32_t* w0p = reinterpret_cast<const uint32_t*>(&w[u][0]);
-          const uint32_t* w1p = reinterpret_cast<const uint32_t*>(&w[u][1]);
-          unpack<T>(lo, w0p[j], zoff[0], zoff16[0]);
-          unpack<T>(hi, w1p[j], zoff[1], zoff16[1]);
-          const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]};
-          const uint32_t a1[4] = {lo[2], hi[2], lo[3], hi[3]};
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint4 b = make_uint4(0, 0, 0, 0);
-            if (n * 8 + g < mrows)
-              b = *reinterpret_cast<const uint4*>(xs + (n * 8 + g) * xrow + i * 256 + j * 64);
-            mma_i4<T>(acc[n], a0, b.x, b.y);
-            mma_i4<T>(acc[n], a1, b.z, b.w);
-          }
-          if (j % JPG == JPG - 1) {
-            float sc[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int at = h * GPC + grp;
-              const uint32_t bits = (sm[u].r[at >> 1] >> (16 * (at & 1))) & 0xffffu;
-              sc[h] = a.s_bf16 ? __uint_as_float(bits << 16)
-                               : __half2float(__ushort_as_half((unsigned short)bits));
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) tot[n][e] += sc[e >> 1] * acc[n][e];
           }
         }
-        fetch(u, i + kI4Deep);
       }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) xa[n] += 256;
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
 
   // ---- the block's warps, then the cluster's blocks, in order
@@ -338,7 +361,10 @@ __global__ void int4_repack_kernel(const uint8_t* q, const uint16_t* s, const ui
     const int64_t grp = ((chunk % C) * 128 + (gpc > 1 ? gi * group : 0)) / group;
     const bool live = row < N && grp < K / group;
     so[j] = live ? s[grp * N + row] : 0;
-    if (zo) zo[j] = live ? z[grp * N + row] & 15 : 8;
+    if (zo) {
+      const int zb = zero_bytes(gpc);
+      zo[(chunk * 8 + g) * zb + h * gpc + gi] = live ? z[grp * N + row] & 15 : 8;
+    }
   }
 }
 
@@ -355,10 +381,12 @@ __global__ void int4_dequant_kernel(const uint32_t* q, const uint16_t* s, const 
   const int j = kk >> 5, t = (kk >> 3) & 3, e = kk & 7;
   const uint32_t w = q[((chunk * 2 + h) * 32 + g * 4 + t) * 4 + j];
   const int v = (w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15;
-  const int64_t at = (chunk * 16 + g * 2 + h) * gpc + j * gpc / 4;
+  const int gi = j * gpc / 4;
+  const int64_t at = (chunk * 16 + g * 2 + h) * gpc + gi;
+  const int zero = z ? z[(chunk * 8 + g) * zero_bytes(gpc) + h * gpc + gi] : 8;
   const float sc = s_bf16 ? __uint_as_float((uint32_t)s[at] << 16)
                           : __half2float(__ushort_as_half(s[at]));
-  out[i] = from_f32<T>((float)(v - (z ? (int)z[at] : 8)) * sc);
+  out[i] = from_f32<T>((float)(v - zero) * sc);
 }
 
 struct Int4Shape {
@@ -381,31 +409,53 @@ int int4_shape(Int4Shape& sh, int64_t N, int64_t K, int64_t group) {
   return SP_OK;
 }
 
+// The shape of the launch: a.wr row tiles per block (its other warps split the inputs), S blocks
+// per cluster and a.pass_chunks chunks of x in shared memory at a time; out of all (wr, S) the
+// one with the least time by this count: waves of blocks, each as long as its busiest warp's
+// chunks plus the cost of a block's start and end (kBlockCost chunks; more for a cluster's
+// join).  `fixed`: the block's shared memory beside x.  Returns S.
+int choose_split(Int4Args& a, int tokens, int m_tiles, int fixed) {
+  const int n_tiles = (a.N + 15) / 16;
+  const int fit = ((kMaxSmem - fixed) / tokens - 64) / 256;
+  int best_s = 1;
+  double best = 1e300;
+  for (int wr = 1; wr <= kI4Warps; wr *= 2) {
+    const int wk = kI4Warps / wr;
+    for (int S = 1; S <= 8; ++S) {
+      if (S > 1 && a.C < S * wk) break;
+      const int range = (a.C + S - 1) / S;
+      const int pass = range < fit ? range : fit;
+      const int smem = fixed + tokens * (pass * 256 + 64) + 1024;
+      const int64_t slots = (int64_t)num_sms() * (2 * smem <= 227 * 1024 ? 2 : 1);
+      const int64_t blocks = (int64_t)((n_tiles + wr - 1) / wr) * S * m_tiles;
+      const int64_t waves = (blocks + slots - 1) / slots;
+      const int chunks = (range + wk - 1) / wk;
+      const double cost = (double)waves * (chunks + kBlockCost + (S > 1 ? kJoinCost : 0));
+      if (cost < best - 1e-9) best = cost, best_s = S, a.wr = wr, a.pass_chunks = pass;
+    }
+  }
+  return best_s;
+}
+
 template <typename T, bool XE4M3, int NT, int GPC, bool ZP>
 int launch_int4(Int4Args a, cudaStream_t s) {
   auto kernel = int4_linear_kernel<T, XE4M3, NT, GPC, ZP>;
-  constexpr int kMaxX = 160 * 1024;
+  using R = Ring<GPC, ZP>;
   static unsigned long long flags = 0;
   if (first_time_on_device(&flags) &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxX) !=
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           kMaxSmem - kI4Warps * 16 * 8 * NT * 4) !=
           cudaSuccess)
     return set_error(SP_ERR_LAUNCH, "int4 linear: shared memory attribute: %s",
                      cudaGetErrorString(cudaGetLastError()));
-  const int sms = num_sms();
-  const int n_tiles = (a.N + 15) / 16;
-  a.wr = NT == 1 ? 2 : 4;
-  while (a.wr > 1 && n_tiles <= a.wr / 2) a.wr /= 2;
-  const int row_blocks = (n_tiles + a.wr - 1) / a.wr;
-  int S = 1;
-  while (S < 8 && row_blocks * S < 2 * sms && a.C / (2 * S) >= kI4Warps / a.wr) S *= 2;
   const int tokens = a.M < 8 * NT ? a.M : 8 * NT;
-  const int range = (a.C + S - 1) / S;
-  const int fit = (kMaxX / tokens - 64) / 256;
-  a.pass_chunks = range < fit ? range : fit;
+  const int m_tiles = (a.M + 8 * NT - 1) / (8 * NT);
+  const int S = choose_split(a, tokens, m_tiles, R::BLOCK + kI4Warps * 16 * 8 * NT * 4);
+  const int row_blocks = ((a.N + 15) / 16 + a.wr - 1) / a.wr;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(row_blocks, S, (a.M + 8 * NT - 1) / (8 * NT));
   cfg.blockDim = dim3(kI4Warps * 32);
-  cfg.dynamicSmemBytes = (size_t)tokens * (a.pass_chunks * 256 + 64);
+  cfg.dynamicSmemBytes = R::BLOCK + (size_t)tokens * (a.pass_chunks * 256 + 64);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -450,7 +500,7 @@ extern "C" int sp_int4_packed_bytes(int64_t N, int64_t K, int64_t group, int64_t
   if (int rc = int4_shape(sh, N, K, group)) return rc;
   sizes[0] = sh.nt * sh.c * 1024;
   sizes[1] = sh.nt * sh.c * 16 * sh.gpc * 2;
-  sizes[2] = sh.nt * sh.c * 16 * sh.gpc;
+  sizes[2] = sh.nt * sh.c * 8 * zero_bytes((int)sh.gpc);
   sizes[3] = 0;
   return SP_OK;
 }

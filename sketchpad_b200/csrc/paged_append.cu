@@ -9,6 +9,8 @@
 // for single tokens.  One block per token: a thread owns eight values at one place of a head
 // and walks the heads, so the token's position, page and (cos, sin) pairs are loaded once for
 // all of its heads.
+#include <new>
+
 #include "common.cuh"
 #include "numeric.cuh"
 #include "paged_kv.cuh"
@@ -121,39 +123,82 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendA
 }  // namespace
 }  // namespace sp
 
-extern "C" int sp_paged_kv_append(const void* q, const void* k, const void* v, void* q_out,
-                                  const int64_t q_strides[4], const int64_t k_in_strides[4],
-                                  const int64_t v_in_strides[4], int64_t tokens, int64_t hq,
-                                  int64_t hkv, int64_t D, void* k_cache, void* v_cache,
-                                  const float* k_scale, const float* v_scale,
-                                  const int64_t k_strides[4], const int64_t v_strides[4],
-                                  int64_t pages, int64_t page_size, const void* block_table,
-                                  int64_t table_rows, int64_t table_cols, int64_t table_stride,
-                                  const void* seq_ids, const void* positions,
-                                  const float* rope_cos_sin, int64_t rope_rows, int dtype,
-                                  int cache_dtype, void* stream) {
+extern "C" int sp_paged_cache_create(void* k, void* v, const float* k_scale, const float* v_scale,
+                                     const int64_t k_strides[4], const int64_t v_strides[4],
+                                     int64_t pages, int64_t page_size, int64_t hkv, int64_t D,
+                                     int dtype, void** cache) {
   using namespace sp;
   clear_error();
-  AppendArgs a{};
-  if (!k_in_strides || !v_in_strides || (tokens != 0 && (!k || !v || !seq_ids || !positions)))
+  if (!cache) return set_error(SP_ERR_INVALID_ARG, "paged cache: null pointer");
+  *cache = nullptr;
+  if (!k || !v || !k_strides || !v_strides)
+    return set_error(SP_ERR_INVALID_ARG, "paged cache: null pointer");
+  if (pages <= 0 || page_size <= 0 || hkv <= 0 || D <= 0)
+    return set_error(SP_ERR_INVALID_ARG, "paged cache: non-positive size");
+  if (pages > 2147483647LL || page_size > (1LL << 30) || hkv > (1LL << 20))
+    return set_error(SP_ERR_SHAPE, "paged cache: too many pages, slots or heads");
+  if (D % 16 || D > 256)
+    return set_error(SP_ERR_SHAPE, "paged cache: head dim %lld is not a multiple of 16 up to 256",
+                     (long long)D);
+  if (dtype != SP_F16 && dtype != SP_BF16 && dtype != SP_E4M3)
+    return set_error(SP_ERR_DTYPE, "paged cache: holds f16, bf16 or e4m3");
+  if (dtype == SP_E4M3 && (!k_scale || !v_scale))
+    return set_error(SP_ERR_INVALID_ARG, "paged cache: an e4m3 cache needs its scales");
+  if (!aligned(k_scale, 4) || !aligned(v_scale, 4) || !aligned(k, 16) || !aligned(v, 16))
+    return set_error(SP_ERR_ALIGN, "paged cache: k and v must be 16-byte aligned");
+  const int64_t vec = dtype == SP_E4M3 ? 16 : 8;
+  if (k_strides[3] != 1 || v_strides[3] != 1)
+    return set_error(SP_ERR_ALIGN, "paged cache: a head's values must be contiguous");
+  for (int i = 0; i < 3; ++i)
+    if (k_strides[i] % vec || v_strides[i] % vec || k_strides[i] < 0 || v_strides[i] < 0)
+      return set_error(SP_ERR_ALIGN, "paged cache: strides must be multiples of 16 bytes");
+  CacheHandle* h = new (std::nothrow) CacheHandle{};
+  if (!h) return set_error(SP_ERR_INVALID_ARG, "paged cache: out of host memory");
+  h->c.k = k, h->c.v = v, h->c.k_scale = k_scale, h->c.v_scale = v_scale;
+  h->c.k_page = k_strides[0], h->c.k_slot = k_strides[1], h->c.k_head = k_strides[2];
+  h->c.v_page = v_strides[0], h->c.v_slot = v_strides[1], h->c.v_head = v_strides[2];
+  h->c.pages = (int32_t)pages;
+  h->c.page_size = make_fast_div((int32_t)page_size);
+  h->page_size = page_size;
+  h->hkv = (int32_t)hkv, h->D = (int32_t)D, h->dtype = dtype;
+  *cache = h;
+  return SP_OK;
+}
+
+extern "C" int sp_paged_cache_destroy(void* cache) {
+  delete static_cast<sp::CacheHandle*>(cache);
+  return SP_OK;
+}
+
+extern "C" int sp_paged_kv_append(const void* cache, const void* q, const void* k, const void* v,
+                                  void* q_out, int64_t q_token_stride, int64_t q_head_stride,
+                                  int64_t k_token_stride, int64_t k_head_stride,
+                                  int64_t v_token_stride, int64_t v_head_stride, int64_t tokens,
+                                  int64_t hq, const void* block_table, int64_t table_rows,
+                                  int64_t table_cols, int64_t table_stride, const void* seq_ids,
+                                  const void* positions, const float* rope_cos_sin,
+                                  int64_t rope_rows, int dtype, void* stream) {
+  using namespace sp;
+  clear_error();
+  const CacheHandle* h = static_cast<const CacheHandle*>(cache);
+  if (!h || (tokens != 0 && (!k || !v || !seq_ids || !positions)))
     return set_error(SP_ERR_INVALID_ARG, "paged append: null pointer");
-  if ((q == nullptr) != (q_out == nullptr) || (q && (!q_strides || hq <= 0)))
+  if ((q == nullptr) != (q_out == nullptr) || (q && hq <= 0))
     return set_error(SP_ERR_INVALID_ARG, "paged append: q, q_out and its heads come together");
-  if (tokens < 0 || tokens > 2147483647LL || hq < 0 || hq > (1 << 20) || hkv > (1 << 20))
+  if (tokens < 0 || tokens > 2147483647LL || hq < 0 || hq > (1 << 20))
     return set_error(SP_ERR_INVALID_ARG, "paged append: bad token or head count");
-  if (int rc = make_paged_cache(a.c, "paged append", k_cache, v_cache, k_scale, v_scale, k_strides,
-                                v_strides, pages, page_size, hkv, D, cache_dtype, block_table,
-                                table_rows, table_cols, table_stride))
+  AppendArgs a{};
+  if (int rc = bind_table(a.c, "paged append", h, block_table, table_rows, table_cols,
+                          table_stride))
     return rc;
   if (dtype != SP_F16 && dtype != SP_BF16)
     return set_error(SP_ERR_DTYPE, "paged append: q, k and v are f16 or bf16");
-  if (cache_dtype != SP_E4M3 && cache_dtype != dtype)
+  if (h->dtype != SP_E4M3 && h->dtype != dtype)
     return set_error(SP_ERR_DTYPE, "paged append: the cache is e4m3 or of the inputs' type");
-  const int64_t* ins[3] = {q ? q_strides : k_in_strides, k_in_strides, v_in_strides};
-  for (const int64_t* st : ins)
-    if (st[2] != 1 || st[0] % 8 || st[1] % 8)
-      return set_error(SP_ERR_ALIGN, "paged append: heads of q, k, v must be contiguous and "
-                       "strides multiples of 8 elements");
+  if ((q && (q_token_stride % 8 || q_head_stride % 8)) || k_token_stride % 8 ||
+      k_head_stride % 8 || v_token_stride % 8 || v_head_stride % 8)
+    return set_error(SP_ERR_ALIGN, "paged append: strides of q, k, v must be multiples of 8 "
+                     "elements");
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(q_out, 16) ||
       !aligned(rope_cos_sin, 16) || !aligned(seq_ids, 4) || !aligned(positions, 4))
     return set_error(SP_ERR_ALIGN, "paged append: pointers must be 16-byte aligned");
@@ -166,13 +211,13 @@ extern "C" int sp_paged_kv_append(const void* q, const void* k, const void* v, v
   a.positions = static_cast<const int32_t*>(positions);
   a.rope = reinterpret_cast<const float2*>(rope_cos_sin);
   a.rope_rows = (int32_t)rope_rows;
-  if (q) a.q_tok = q_strides[0], a.q_head = q_strides[1];
-  a.k_tok = k_in_strides[0], a.k_head = k_in_strides[1];
-  a.v_tok = v_in_strides[0], a.v_head = v_in_strides[1];
-  a.hq = q ? (int32_t)hq : 0, a.hkv = (int32_t)hkv, a.D = (int32_t)D;
+  a.q_tok = q_token_stride, a.q_head = q_head_stride;
+  a.k_tok = k_token_stride, a.k_head = k_head_stride;
+  a.v_tok = v_token_stride, a.v_head = v_head_stride;
+  a.hq = q ? (int32_t)hq : 0, a.hkv = h->hkv, a.D = h->D;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned grid = (unsigned)tokens;
-  const bool f8 = cache_dtype == SP_E4M3;
+  const bool f8 = h->dtype == SP_E4M3;
   if (dtype == SP_F16) {
     if (f8) paged_append_kernel<__half, true><<<grid, kAppThreads, 0, s>>>(a);
     else paged_append_kernel<__half, false><<<grid, kAppThreads, 0, s>>>(a);

@@ -653,40 +653,35 @@ extern "C" size_t sp_paged_attention_workspace_size(int64_t B, int64_t hq, int64
   return sp::parts_bytes() + (size_t)B * hkv * ((hq / hkv + 15) / 16) * sizeof(int32_t);
 }
 
-extern "C" int sp_paged_attention(const void* q, const int64_t q_strides[4], const void* k_cache,
-                                  const void* v_cache, const float* k_scale, const float* v_scale,
-                                  const int64_t k_strides[4], const int64_t v_strides[4],
-                                  const void* block_table, int64_t table_cols,
-                                  int64_t table_stride, const void* seq_lens, void* out, int64_t B,
-                                  int64_t hq, int64_t hkv, int64_t D, int64_t pages,
-                                  int64_t page_size, int64_t window, int64_t sinks, float scale,
-                                  int dtype, int cache_dtype, void* workspace,
-                                  size_t workspace_bytes, void* stream) {
+extern "C" int sp_paged_attention(const void* cache, const void* q, int64_t q_seq_stride,
+                                  int64_t q_head_stride, const void* block_table,
+                                  int64_t table_cols, int64_t table_stride, const void* seq_lens,
+                                  void* out, int64_t B, int64_t hq, int64_t window, int64_t sinks,
+                                  float scale, int dtype, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
   using namespace sp;
   clear_error();
-  AttnArgs a{};
-  if (!q_strides || (B != 0 && (!q || !seq_lens || !out)))
+  const CacheHandle* h = static_cast<const CacheHandle*>(cache);
+  if (!h || (B != 0 && (!q || !seq_lens || !out)))
     return set_error(SP_ERR_INVALID_ARG, "paged attention: null pointer");
-  if (B < 0 || B > 2147483647LL || hq <= 0 || hkv <= 0)
+  if (B < 0 || B > 2147483647LL || hq <= 0)
     return set_error(SP_ERR_INVALID_ARG, "paged attention: bad batch or head count");
+  const int64_t hkv = h->hkv;
   if (hq % hkv || hq > (1 << 20))
     return set_error(SP_ERR_SHAPE, "paged attention: %lld query heads do not divide over %lld cache "
                      "heads", (long long)hq, (long long)hkv);
-  if (int rc = make_paged_cache(a.c, "paged attention", const_cast<void*>(k_cache),
-                                const_cast<void*>(v_cache), k_scale, v_scale, k_strides, v_strides,
-                                pages, page_size, hkv, D, cache_dtype, block_table, B, table_cols,
-                                table_stride))
+  AttnArgs a{};
+  if (int rc = bind_table(a.c, "paged attention", h, block_table, B, table_cols, table_stride))
     return rc;
   if (window < 0 || sinks < 0 || window > 2147483647LL || sinks > 2147483647LL)
     return set_error(SP_ERR_INVALID_ARG, "paged attention: bad window or sinks");
   if (dtype != SP_F16 && dtype != SP_BF16)
     return set_error(SP_ERR_DTYPE, "paged attention: q and out are f16 or bf16");
-  if (cache_dtype != SP_E4M3 && cache_dtype != dtype)
+  if (h->dtype != SP_E4M3 && h->dtype != dtype)
     return set_error(SP_ERR_DTYPE, "paged attention: the cache is e4m3 or of q's type");
-  if (q_strides[2] != 1 || q_strides[0] % 2 || q_strides[1] % 2 || !aligned(q, 4) ||
-      !aligned(out, 16) || !aligned(seq_lens, 4))
-    return set_error(SP_ERR_ALIGN, "paged attention: q heads must be contiguous and 4-byte "
-                     "aligned, out 16-byte aligned");
+  if (q_seq_stride % 2 || q_head_stride % 2 || !aligned(q, 4) || !aligned(out, 16) ||
+      !aligned(seq_lens, 4))
+    return set_error(SP_ERR_ALIGN, "paged attention: q heads must be 4-byte aligned, out 16-byte");
   if (B == 0) return SP_OK;
   if (B * hkv * ((hq / hkv + 15) / 16) > (1LL << 30))
     return set_error(SP_ERR_SHAPE, "paged attention: too many sequences x heads");
@@ -697,15 +692,15 @@ extern "C" int sp_paged_attention(const void* q, const int64_t q_strides[4], con
     return set_error(SP_ERR_ALIGN, "paged attention: workspace must be 16-byte aligned");
   a.q = q, a.out = out;
   a.lens = static_cast<const int32_t*>(seq_lens);
-  a.q_seq = q_strides[0], a.q_head = q_strides[1];
-  a.B = (int32_t)B, a.hq = (int32_t)hq, a.hkv = (int32_t)hkv, a.D = (int32_t)D;
+  a.q_seq = q_seq_stride, a.q_head = q_head_stride;
+  a.B = (int32_t)B, a.hq = (int32_t)hq, a.hkv = (int32_t)hkv, a.D = h->D;
   a.group = (int32_t)(hq / hkv), a.row_blocks = (a.group + 15) / 16;
   a.window = (int32_t)window, a.sinks = (int32_t)sinks;
-  a.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)D)) * 1.4426950408889634f;
+  a.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)h->D)) * 1.4426950408889634f;
   a.parts = static_cast<float*>(workspace);
   a.counters = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + parts_bytes());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (cache_dtype == SP_E4M3)
+  if (h->dtype == SP_E4M3)
     return dtype == SP_F16 ? launch_attn_d<__half, true>(a, s)
                            : launch_attn_d<__nv_bfloat16, true>(a, s);
   return dtype == SP_F16 ? launch_attn_d<__half, false>(a, s)

@@ -18,7 +18,9 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._torch import dtype_code, ptr, require_cuda, stream_ptr
+from ._torch import cuda_index, dtype_code, ptr, raw_stream, require_cuda, stream_ptr
+
+_linear = _lib.Entry("sp_int4_linear")
 
 _X = {torch.float16: _lib.SP_F16, torch.bfloat16: _lib.SP_BF16,
       torch.float8_e4m3fn: _lib.SP_E4M3}
@@ -117,42 +119,53 @@ class Int4Linear:
 
         x bf16 or f16, or float8_e4m3fn with x_scale f32 [...].  The output's type is
         out_dtype, else out's, else x's (bf16 for e4m3)."""
-        dev = require_cuda(x, self.q, x_scale, out)
+        index = cuda_index(x, self.q, x_scale, out)
         N, K = self.out_features, self.in_features
         xd = _X.get(x.dtype)
         if xd is None:
             raise TypeError("x must be bf16, f16 or float8_e4m3fn")
-        if x.dim() == 0 or x.shape[-1] != K:
+        shape = x.shape
+        if not shape or shape[-1] != K:
             raise ValueError(f"x must be [..., {K}]")
-        if (xd == _lib.SP_E4M3) != (x_scale is not None):
-            raise ValueError("e4m3 activations, and only those, come with x_scale")
-        lead = x.shape[:-1]
-        if x_scale is not None and (x_scale.shape != lead or x_scale.dtype != torch.float32
-                                    or not x_scale.is_contiguous()):
-            raise ValueError(f"x_scale must be contiguous f32 {tuple(lead)}")
+        s_ptr = 0
+        if xd == _lib.SP_E4M3:
+            if x_scale is None:
+                raise ValueError("e4m3 activations come with x_scale")
+            if x_scale.shape != shape[:-1] or x_scale.dtype != torch.float32 or \
+                    not x_scale.is_contiguous():
+                raise ValueError(f"x_scale must be contiguous f32 {tuple(shape[:-1])}")
+            s_ptr, align = x_scale.data_ptr(), 8
+        elif x_scale is not None:
+            raise ValueError("only e4m3 activations come with x_scale")
+        else:
+            align = 16
         dt = out_dtype or (out.dtype if out is not None else
                            torch.bfloat16 if xd == _lib.SP_E4M3 else x.dtype)
         if out is None:
-            out = torch.empty((*lead, N), dtype=dt, device=dev)
-        elif out.dtype != dt or out.shape != (*lead, N) or not out.is_contiguous():
+            out = x.new_empty((*shape[:-1], N), dtype=dt)
+        elif out.dtype != dt or out.shape != (*shape[:-1], N) or not out.is_contiguous():
             raise ValueError(f"out must be contiguous {dt} [..., {N}]")
-        x2 = x if x.dim() == 2 else x.reshape(-1, K)
-        M, stride = x2.shape[0], x2.stride(0)
-        align = 8 if xd == _lib.SP_E4M3 else 16
-        if x2.stride(1) != 1 or stride % 8 or (stride < K and M > 1) or x2.data_ptr() % align:
-            x2 = x2.clone(memory_format=torch.contiguous_format)
-            stride = K
-        bias = self.bias
-        if bias is not None and (bias.dtype != dt or not bias.is_contiguous()):
-            bias = self._bias.get(dt)
-            if bias is None:
-                bias = self._bias[dt] = self.bias.to(dt).contiguous()
-        q, s, z, sd = self._weight_args
-        _lib.call("sp_int4_linear", x2.data_ptr(), max(stride, K), xd,
-                  0 if x_scale is None else x_scale.data_ptr(), q, s, z, sd,
-                  0 if bias is None else bias.data_ptr(), out.data_ptr(), M, N, K,
-                  self.group_size, dtype_code(dt), stream_ptr(dev))
+        M, stride, p = x.numel() // K, K, x.data_ptr()
+        if p % align or not x.is_contiguous():
+            x = x if x.dim() == 2 else x.reshape(-1, K)
+            stride, p = x.stride(0), x.data_ptr()
+            if x.stride(1) != 1 or p % align or (M > 1 and (stride % 8 or stride < K)):
+                x = x.clone(memory_format=torch.contiguous_format)
+                p, stride = x.data_ptr(), K
+            elif M <= 1:
+                stride = K
+        b_ptr = 0
+        if self.bias is not None:
+            b_ptr = self._bias_as(dt).data_ptr()
+        _linear(p, stride, xd, s_ptr, *self._weight_args, b_ptr, out.data_ptr(), M, N, K,
+                self.group_size, dtype_code(dt), raw_stream(index))
         return out
+
+    def _bias_as(self, dt: torch.dtype) -> torch.Tensor:
+        b = self._bias.get(dt)
+        if b is None:
+            b = self._bias[dt] = self.bias.to(dt).contiguous()
+        return b
 
     __call__ = forward
 

@@ -14,12 +14,17 @@ The cache holds bf16 or f16, or e4m3 values times a scale per head.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Dict, Optional
 
 import torch
 
 from . import _lib
-from ._torch import dtype_code, ptr, require_cuda, stream_ptr
+from ._torch import cuda_index, dtype_code, ptr, raw_stream, require_cuda
+
+_append = _lib.Entry("sp_paged_kv_append")
+_attend = _lib.Entry("sp_paged_attention")
+_16BIT = {torch.float16: _lib.SP_F16, torch.bfloat16: _lib.SP_BF16}
 
 
 class PagedKVCache:
@@ -48,8 +53,18 @@ class PagedKVCache:
             raise TypeError("the cache holds bf16, f16 or float8_e4m3fn")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.page_size, self.kv_heads, self.head_dim = k.shape
-        self._strides = (_lib.i64_array(k.stride()), _lib.i64_array(v.stride()))
         self._work: Dict[int, torch.Tensor] = {}
+        self._handle = ctypes.c_void_p()
+        _lib.call("sp_paged_cache_create", ptr(k), ptr(v), ptr(k_scale), ptr(v_scale),
+                  _lib.i64_array(k.stride()), _lib.i64_array(v.stride()), *k.shape, self._code,
+                  ctypes.byref(self._handle))
+
+    def __del__(self):
+        try:
+            if self._handle:
+                _lib.load().sp_paged_cache_destroy(self._handle)
+        except Exception:  # pragma: no cover - interpreter shutdown
+            pass
 
     @classmethod
     def allocate(cls, pages: int, page_size: int, kv_heads: int, head_dim: int,
@@ -62,12 +77,14 @@ class PagedKVCache:
                                    else dtype, device=device).view(dtype)
         return cls(make(), make(), k_scale, v_scale)
 
-    def _table(self, block_table: torch.Tensor) -> torch.Tensor:
+    @staticmethod
+    def _table(block_table: torch.Tensor) -> torch.Tensor:
         if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.shape[1] == 0:
             raise ValueError("block_table must be int32 [sequences, max_pages]")
-        if block_table.stride(1) != 1 or (block_table.stride(0) < block_table.shape[1]
-                                          and block_table.shape[0] > 1):
-            block_table = block_table.contiguous()
+        if not block_table.is_contiguous():
+            s0, s1 = block_table.stride()
+            if s1 != 1 or s0 < block_table.shape[1]:
+                block_table = block_table.contiguous()
         return block_table
 
     def append(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
@@ -81,42 +98,45 @@ class PagedKVCache:
         rope: f32 [positions, head_dim / 2, 2] (cos, sin) from `rope_pair_table`; k and q are
         rotated by their position (interleaved pairs).  A token whose sequence, position or page
         does not exist (a position of -1, say) is padding: nothing is stored, its q is zeros."""
-        dev = require_cuda(k, v, block_table, seq_ids, positions, q, rope, q_out, self.k)
+        index = cuda_index(k, v, block_table, seq_ids, positions, q, rope, q_out, self.k)
         T = k.shape[0]
         D, hkv = self.head_dim, self.kv_heads
-        if k.shape != (T, hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
+        dtype = k.dtype
+        if k.shape != (T, hkv, D) or v.shape != k.shape or v.dtype != dtype:
             raise ValueError(f"k and v must be [tokens, {hkv}, {D}] of one dtype")
-        if k.dtype not in (torch.bfloat16, torch.float16) or \
-                (self._code != _lib.SP_E4M3 and k.dtype != self.k.dtype):
+        code = _16BIT.get(dtype)
+        if code is None or (self._code != _lib.SP_E4M3 and code != self._code):
             raise ValueError("k and v must be of the cache's dtype (bf16 or f16 for e4m3)")
         for t in (seq_ids, positions):
             if t.shape != (T,) or t.dtype != torch.int32 or not t.is_contiguous():
                 raise ValueError(f"seq_ids and positions must be contiguous int32 [{T}]")
         table = self._table(block_table)
-        hq = 0
+        hq = q_ptr = out_ptr = q_tok = q_head = 0
         if q is not None:
             hq = q.shape[1] if q.dim() == 3 else 0
-            if hq == 0 or q.shape != (T, hq, D) or q.dtype != k.dtype:
+            if hq == 0 or q.shape != (T, hq, D) or q.dtype != dtype:
                 raise ValueError(f"q must be [{T}, heads, {D}] of k's dtype")
             if q_out is None:
-                q_out = torch.empty((T, hq, D), dtype=q.dtype, device=dev)
-            elif q_out.shape != q.shape or q_out.dtype != q.dtype or not q_out.is_contiguous():
+                q_out = q.new_empty((T, hq, D))
+            elif q_out.shape != q.shape or q_out.dtype != dtype or not q_out.is_contiguous():
                 raise ValueError("q_out must be contiguous and have q's shape and dtype")
-            q = _heads(q)
+            q, q_ptr, q_tok, q_head = _heads(q)
+            out_ptr = q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
-        k, v = _heads(k), _heads(v)
-        if rope is not None and (rope.dtype != torch.float32 or not rope.is_contiguous()
-                                 or rope.dim() != 3 or rope.shape[1:] != (D // 2, 2)):
-            raise ValueError(f"rope must be contiguous f32 [positions, {D // 2}, 2]")
-        qs = None if q is None else _lib.i64_array((*q.stride(), 0))
-        _lib.call("sp_paged_kv_append", ptr(q), ptr(k), ptr(v), ptr(q_out), qs,
-                  _lib.i64_array((*k.stride(), 0)), _lib.i64_array((*v.stride(), 0)), T, hq, hkv,
-                  D, ptr(self.k), ptr(self.v), ptr(self.k_scale), ptr(self.v_scale),
-                  *self._strides, self.pages, self.page_size, ptr(table), table.shape[0],
-                  table.shape[1], max(table.stride(0), table.shape[1]), ptr(seq_ids),
-                  ptr(positions), ptr(rope), 0 if rope is None else rope.shape[0],
-                  dtype_code(k.dtype), self._code, stream_ptr(dev))
+        k, k_ptr, k_tok, k_head = _heads(k)
+        v, v_ptr, v_tok, v_head = _heads(v)
+        rope_ptr = rope_rows = 0
+        if rope is not None:
+            if rope.dtype != torch.float32 or not rope.is_contiguous() or rope.dim() != 3 or \
+                    rope.shape[1] != D // 2 or rope.shape[2] != 2:
+                raise ValueError(f"rope must be contiguous f32 [positions, {D // 2}, 2]")
+            rope_ptr, rope_rows = rope.data_ptr(), rope.shape[0]
+        rows, cols = table.shape
+        _append(self._handle, q_ptr, k_ptr, v_ptr, out_ptr, q_tok, q_head, k_tok, k_head, v_tok,
+                v_head, T, hq, table.data_ptr(), rows, cols, max(table.stride(0), cols),
+                seq_ids.data_ptr(), positions.data_ptr(), rope_ptr, rope_rows, code,
+                raw_stream(index))
         return q_out
 
     def new_workspace(self, batch: int, heads: int) -> torch.Tensor:
@@ -133,51 +153,64 @@ class PagedKVCache:
         cache head h // (heads / kv_heads).  window: only the last `window` tokens and the first
         `sinks`.  scale: 1 / sqrt(head_dim) unless given.  A sequence of length 0, or without a
         page that is there, gives zeros."""
-        dev = require_cuda(q, block_table, seq_lens, out, workspace, self.k)
-        if q.dim() != 3 or q.shape[2] != self.head_dim or q.shape[1] == 0 or \
-                q.shape[1] % self.kv_heads:
-            raise ValueError(f"q must be [sequences, heads, {self.head_dim}] with heads a "
-                             f"multiple of {self.kv_heads}")
-        B, hq, D = q.shape
-        if q.dtype not in (torch.bfloat16, torch.float16) or \
-                (self._code != _lib.SP_E4M3 and q.dtype != self.k.dtype):
+        index = cuda_index(q, block_table, seq_lens, out, workspace, self.k)
+        D, hkv = self.head_dim, self.kv_heads
+        if q.dim() != 3:
+            raise ValueError(f"q must be [sequences, heads, {D}]")
+        B, hq, qd = q.shape
+        if qd != D or hq == 0 or hq % hkv:
+            raise ValueError(f"q must be [sequences, heads, {D}] with heads a multiple of {hkv}")
+        code = _16BIT.get(q.dtype)
+        if code is None or (self._code != _lib.SP_E4M3 and code != self._code):
             raise ValueError("q must be of the cache's dtype (bf16 or f16 for e4m3)")
-        if block_table.shape[0] != B or seq_lens.shape != (B,) or seq_lens.dtype != torch.int32 \
+        table = self._table(block_table)
+        rows, cols = table.shape
+        if rows != B or seq_lens.shape != (B,) or seq_lens.dtype != torch.int32 \
                 or not seq_lens.is_contiguous():
             raise ValueError(f"block_table must have {B} rows and seq_lens be contiguous int32 "
                              f"[{B}]")
-        if window is not None and window < 1:
+        if window is None:
+            window = 0
+        elif window < 1:
             raise ValueError("window must be at least 1")
         if sinks < 0:
             raise ValueError("sinks must not be negative")
-        table = self._table(block_table)
-        q = _heads(q)
         if out is None:
-            out = torch.empty((B, hq, D), dtype=q.dtype, device=dev)
+            out = q.new_empty((B, hq, D))
         elif out.shape != (B, hq, D) or out.dtype != q.dtype or not out.is_contiguous():
             raise ValueError(f"out must be contiguous {q.dtype} [{B}, {hq}, {D}]")
-        stream = stream_ptr(dev)
+        q, q_ptr, q_seq, q_head = _heads(q)
+        stream = raw_stream(index)
         if workspace is None:
-            need = _lib.load().sp_paged_attention_workspace_size(B, hq, self.kv_heads)
-            workspace = self._work.get(stream.value)
-            if workspace is None or workspace.numel() * 4 < need:
-                workspace = self._work[stream.value] = self.new_workspace(B, hq)
+            items = B * hkv * ((hq // hkv + 15) >> 4)  # counters of the call
+            workspace, ws_ptr, ws_bytes, most = self._work.get(stream, _NO_WORKSPACE)
+            if items > most:
+                workspace = self.new_workspace(B, hq)
+                ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * 4
+                self._work[stream] = (workspace, ws_ptr, ws_bytes, items)
         elif not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
-        _lib.call("sp_paged_attention", ptr(q), _lib.i64_array((*q.stride(), 0)), ptr(self.k),
-                  ptr(self.v), ptr(self.k_scale), ptr(self.v_scale), *self._strides, ptr(table),
-                  table.shape[1], max(table.stride(0), table.shape[1]), ptr(seq_lens), ptr(out),
-                  B, hq, self.kv_heads, D, self.pages, self.page_size, window or 0, sinks,
-                  float(scale) if scale else 0.0, dtype_code(q.dtype), self._code,
-                  ptr(workspace), workspace.numel() * workspace.element_size(), stream)
+        else:
+            ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        _attend(self._handle, q_ptr, q_seq, q_head, table.data_ptr(), cols,
+                max(table.stride(0), cols), seq_lens.data_ptr(), out.data_ptr(), B, hq, window,
+                sinks, scale or 0.0, code, ws_ptr, ws_bytes, stream)
         return out
 
 
-def _heads(t: torch.Tensor) -> torch.Tensor:
-    """t [tokens, heads, dim] with 16-byte aligned, contiguous heads (else a copy)."""
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+_NO_WORKSPACE = (None, 0, 0, 0)
+
+
+def _heads(t: torch.Tensor):
+    """(t, pointer, token stride, head stride) of t [tokens, heads, dim] with 16-byte aligned,
+    contiguous heads, or of a copy that has them."""
+    s0, s1, s2 = t.stride()
+    p = t.data_ptr()
+    if s2 != 1 or s0 % 8 or s1 % 8 or p % 16:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        s0, s1, _ = t.stride()
+        p = t.data_ptr()
+    return t, p, s0, s1
 
 
 __all__ = ["PagedKVCache"]

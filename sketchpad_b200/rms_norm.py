@@ -12,33 +12,51 @@ from typing import Optional
 import torch
 
 from . import _lib
-from ._torch import dtype_code, ptr, require_cuda, stream_ptr
+from ._torch import cuda_index, dtype_code, raw_stream
+
+_norm = _lib.Entry("sp_rms_norm")
+_norm_fp8 = _lib.Entry("sp_rms_norm_fp8")
 
 
-def _rows(t: torch.Tensor, n: int) -> torch.Tensor:
-    """t as rows of n values with one row stride (a copy only where t has no such view)."""
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= n:
-        return t
-    t = t.reshape(-1, n)
-    return t if t.stride(1) == 1 and (t.stride(0) >= n or t.shape[0] == 1) else t.contiguous()
+def _rows(t: torch.Tensor, n: int):
+    """(t, pointer, row stride) of t as rows of n values (a copy only where t has no such view)."""
+    if not t.is_contiguous():
+        if t.dim() != 2:
+            t = t.reshape(-1, n)
+        if t.stride(1) != 1 or (t.stride(0) < n and t.shape[0] > 1):
+            t = t.clone(memory_format=torch.contiguous_format)
+        return t, t.data_ptr(), max(t.stride(0), n)
+    return t, t.data_ptr(), n
 
 
 def _operands(x, weight, residual, residual_out):
-    dev = require_cuda(x, weight, residual, residual_out)
-    code = dtype_code(x.dtype)
-    if x.dim() == 0 or x.shape[-1] == 0:
+    """Checks; (device index, rows, n, x's and the residual's rows, weight's and residual_out's
+    pointers, residual_out)."""
+    index = cuda_index(x, weight, residual, residual_out)
+    shape = x.shape
+    n = shape[-1] if shape else 0
+    if n == 0:
         raise ValueError("x must have a last dimension of at least one value")
-    n = x.shape[-1]
-    if weight is not None and (weight.dtype != x.dtype or weight.shape != (n,)
-                               or weight.stride(0) != 1):
-        raise ValueError(f"weight must be [{n}], contiguous, of x's dtype")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError("residual must have x's shape and dtype")
-    if residual_out is not None and (
-            residual_out.shape != x.shape or residual_out.dtype != x.dtype
-            or not residual_out.is_contiguous()):
-        raise ValueError("residual_out must be contiguous and have x's shape and dtype")
-    return dev, code, n
+    dtype = x.dtype
+    w_ptr = ro_ptr = 0
+    if weight is not None:
+        if weight.dtype != dtype or weight.shape != (n,) or not weight.is_contiguous():
+            raise ValueError(f"weight must be [{n}], contiguous, of x's dtype")
+        w_ptr = weight.data_ptr()
+    xr = _rows(x, n)
+    rr = (None, 0, n)
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != dtype:
+            raise ValueError("residual must have x's shape and dtype")
+        rr = _rows(residual, n)
+        if residual_out is None:
+            residual_out = x.new_empty(shape)
+    if residual_out is not None:
+        if residual_out.shape != shape or residual_out.dtype != dtype or \
+                not residual_out.is_contiguous():
+            raise ValueError("residual_out must be contiguous and have x's shape and dtype")
+        ro_ptr = residual_out.data_ptr()
+    return index, x.numel() // n, n, xr, rr, w_ptr, ro_ptr, residual_out
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6, *,
@@ -48,20 +66,17 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6,
 
     Returns y, or (y, r) with a residual.  `out` and `residual_out` receive them; they may be x
     or residual themselves (the stream updated in place)."""
-    dev, code, n = _operands(x, weight, residual, residual_out)
+    code = dtype_code(x.dtype)
+    index, rows, n, xr, rr, w_ptr, ro_ptr, residual_out = _operands(x, weight, residual,
+                                                                    residual_out)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        out = x.new_empty(x.shape)
     elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous and have x's shape and dtype")
     else:
-        require_cuda(x, out)
-    if residual is not None and residual_out is None:
-        residual_out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    xr = _rows(x, n)
-    rr = None if residual is None else _rows(residual, n)
-    _lib.call("sp_rms_norm", ptr(xr), max(xr.stride(0), n), ptr(rr),
-              n if rr is None else max(rr.stride(0), n), ptr(weight), ptr(out), ptr(residual_out),
-              xr.shape[0], n, eps, code, stream_ptr(dev))
+        cuda_index(x, out)
+    _norm(xr[1], xr[2], rr[1], rr[2], w_ptr, out.data_ptr(), ro_ptr, rows, n, eps, code,
+          raw_stream(index))
     return out if residual is None else (out, residual_out)
 
 
@@ -72,16 +87,13 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1
 
     q is float8_e4m3fn of x's shape, scale f32 of its leading dimensions, y = q * scale with
     scale = max|y| / 448 over each row (1 where a row is all zeros)."""
-    dev, code, n = _operands(x, weight, residual, residual_out)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    if residual is not None and residual_out is None:
-        residual_out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    xr = _rows(x, n)
-    rr = None if residual is None else _rows(residual, n)
-    _lib.call("sp_rms_norm_fp8", ptr(xr), max(xr.stride(0), n), ptr(rr),
-              n if rr is None else max(rr.stride(0), n), ptr(weight), ptr(q), ptr(scale),
-              ptr(residual_out), xr.shape[0], n, eps, code, stream_ptr(dev))
+    code = dtype_code(x.dtype)
+    index, rows, n, xr, rr, w_ptr, ro_ptr, residual_out = _operands(x, weight, residual,
+                                                                    residual_out)
+    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    _norm_fp8(xr[1], xr[2], rr[1], rr[2], w_ptr, q.data_ptr(), scale.data_ptr(), ro_ptr, rows, n,
+              eps, code, raw_stream(index))
     return (q, scale) if residual is None else (q, scale, residual_out)
 
 
