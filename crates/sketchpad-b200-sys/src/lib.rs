@@ -237,11 +237,15 @@ extern "C" {
         K: i64, group: i64, scale_dtype: c_int, out: *mut c_void, out_dtype: c_int, stream:
         *mut c_void
     ) -> c_int;
+    pub fn sp_int4_linear_workspace_size(
+        M: i64, N: i64, K: i64, group: i64
+    ) -> usize;
     pub fn sp_int4_linear(
         x: *const c_void, x_row_stride: i64, x_dtype: c_int, x_scale: *const c_float,
         q_packed: *const c_void, s_packed: *const c_void, z_packed: *const c_void,
         scale_dtype: c_int, bias: *const c_void, y: *mut c_void, M: i64, N: i64, K: i64,
-        group: i64, out_dtype: c_int, stream: *mut c_void
+        group: i64, out_dtype: c_int, workspace: *mut c_void, workspace_bytes: usize,
+        stream: *mut c_void
     ) -> c_int;
     pub fn sp_paged_cache_create(
         k: *mut c_void, v: *mut c_void, k_scale: *const c_float, v_scale: *const c_float,

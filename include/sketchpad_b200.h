@@ -471,12 +471,18 @@ int sp_int4_dequant(const void* q_packed, const void* s_packed, const void* z_pa
                     void* stream);
 /* x [M, K]: f16, bf16, or e4m3 (SP_E4M3, with x_scale [M], NULL otherwise); rows 16-byte aligned
  * (8 for e4m3), x_row_stride a multiple of 8 elements.  bias [N] of out_dtype or NULL.  y [M, N]
- * contiguous, out_dtype f32, f16 or bf16.  Sums are f32 and their order does not change from
- * call to call.  Any M; the weights are read once per 32 rows of x. */
+ * contiguous, out_dtype f32, f16 or bf16.  N up to 2^21.  Sums are f32 and their order does not
+ * change from call to call; a row of x with an infinity or a NaN gives infinities or NaNs.  Any
+ * M; the weights are read once per 32 rows of x.
+ * workspace: sp_int4_linear_workspace_size() bytes (which grow up to M = 32), 16-byte aligned,
+ * ZERO before its first use (each call leaves its counters, the first 256 KB, zero again) and
+ * not in use by another call in flight; calls of any sizes that fit may share it. */
+size_t sp_int4_linear_workspace_size(int64_t M, int64_t N, int64_t K, int64_t group);
 int sp_int4_linear(const void* x, int64_t x_row_stride, int x_dtype, const float* x_scale,
                    const void* q_packed, const void* s_packed, const void* z_packed,
                    int scale_dtype, const void* bias, void* y, int64_t M, int64_t N, int64_t K,
-                   int64_t group, int out_dtype, void* stream);
+                   int64_t group, int out_dtype, void* workspace, size_t workspace_bytes,
+                   void* stream);
 
 /* A paged key-value cache: k and v [pages, page_size, hkv, D] with element strides (innermost
  * 1, the others multiples of 16 bytes, pointers 16-byte aligned), D a multiple of 16 up to 256,

@@ -101,8 +101,9 @@ SIGNATURES = {
     "sp_int4_packed_bytes": (_int, [_i64, _i64, _i64, _i64p]),
     "sp_int4_repack": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
     "sp_int4_dequant": (_int, [_vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _int, _vp]),
+    "sp_int4_linear_workspace_size": (_sz, [_i64, _i64, _i64, _i64]),
     "sp_int4_linear": (_int, [_vp, _i64, _int, _vp, _vp, _vp, _vp, _int, _vp, _vp, _i64, _i64,
-                              _i64, _i64, _int, _vp]),
+                              _i64, _i64, _int, _vp, _sz, _vp]),
     "sp_paged_cache_create": (_int, [_vp, _vp, _vp, _vp, _i64p, _i64p, _i64, _i64, _i64, _i64,
                                      _int, ctypes.POINTER(_vp)]),
     "sp_paged_cache_destroy": (_int, [_vp]),

@@ -59,6 +59,27 @@ def cuda_index(x: torch.Tensor, *others) -> int:
     return i
 
 
+class Workspaces:
+    """Zero-initialised device workspaces, one per (device, stream): the kernels that use them
+    leave their counters zero again, so calls in one stream's order share one.  A workspace made
+    while its stream is being captured belongs to the graph alone (its zeroing is a node of the
+    graph) and is not kept."""
+
+    def __init__(self):
+        self._kept = {}
+
+    def get(self, index: int, stream: int, nbytes: int):
+        """(tensor to hold on to until the launch, pointer, bytes) of at least nbytes."""
+        w = self._kept.get((index, stream))
+        if w is None or w[2] < nbytes:
+            n = (nbytes + 3) // 4
+            t = torch.zeros(n, dtype=torch.int32, device=torch.device("cuda", index))
+            w = (t, t.data_ptr(), n * 4)
+            if not torch.cuda.is_current_stream_capturing():
+                self._kept[index, stream] = w
+        return w
+
+
 def ptr(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 

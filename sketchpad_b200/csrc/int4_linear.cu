@@ -3,19 +3,34 @@
 //
 //   y[m, n] = xs[m] * sum_g s[g, n] * sum_{k in g} (q[n, k] - z[g, n]) x[m, k]  (+ bias[n])
 //
-// Bound by the weight bytes (HBM, or L2 where they stay there) as long as m is small.  The
-// weights are laid out once (sp_int4_repack) in the order in which a warp's m16n8k16 MMA takes
-// them as its A operand: 16 rows x 128 inputs are 1 KB, a lane's 16 bytes after 16 bytes, so
-// the weights stream in with fully used 16-byte loads, four KB in flight per warp, and never
-// pass through shared memory.  q - z is formed in the MMA's own type, exactly (small integers);
-// each group's sum over its inputs stays in the f32 accumulators, which alone are multiplied
-// by the group's scale.  x is staged in shared memory for the block's range of inputs.
+// Bound by the weight bytes (HBM, or L2 where they stay there) as long as m is small, and
+// close behind by the instructions that turn 4-bit values into MMA operands, so those are what
+// the layout and the arithmetic save on:
+//  - The weights are laid out once (sp_int4_repack) in the order in which a warp's m16n8k16 MMAs
+//    take them as their A operand: 32 rows x 128 inputs (a chunk) are 2 KB, four times a lane's
+//    16 bytes after 16 bytes.  Each lane copies the very bytes that it will use into its own
+//    slots of the warp's ring in shared memory (cp.async), so four to six KB per warp are in
+//    flight without holding registers.  32 rows, because the x operand that they share comes
+//    from shared memory, which 16 rows would keep busier than the weights keep HBM.
+//  - A 4-bit value in the low bits of an f16 is the subnormal q 2^-24, exactly, and the tensor
+//    cores take subnormals: two values per AND, no subtraction, no multiplication.  Bits 4-7
+//    are 16 q 2^-24; the inputs that meet those are staged as x / 16.  The f32 sums are scaled
+//    back by 2^24 at the end.
+//  - The zero point leaves the products: sum (q - z) x = sum q x - z sum x, where sum x of a
+//    group comes from one MMA per 16 inputs with a matrix of ones, once per block; -z sum x is
+//    what a group's accumulator starts from.  (|q x| is at most twice |(q - z) x| for a middle
+//    zero point, so the f32 sums lose a bit at most.)
+//  - x is staged in shared memory as f16, each row scaled by a power of two that brings its
+//    largest value of the block's inputs to [2^14, 2^15): exact for f16 and bf16 but for values
+//    below 2^-35 of that, and e4m3 values fit as they are.  A row with an infinity or a NaN
+//    gives infinities or NaNs.
 //
-// A block is 8 warps over WR x 16 rows and 8 / WR parts of its range of inputs; a cluster of S
-// blocks shares the rows and splits the inputs further.  Partial sums meet in shared memory,
-// then across the cluster in distributed shared memory, in a fixed order.
-#include <cooperative_groups.h>
-
+// The launch is one block of 16 warps per SM.  Where a block cannot hold all of x, the inputs
+// are cut into S slabs, each with its own blocks.  Groups of U warps take whole tiles (32 rows
+// of a slab) in turn, a group's warps every U-th chunk, and join at the tile's end in shared
+// memory; int4_plan chooses U and S for the shortest schedule.  With S > 1 a tile's slabs are
+// joined by whichever group comes last (a counter in the workspace), in slab order, so results
+// do not depend on timing.
 #include <type_traits>
 
 #include "common.cuh"
@@ -24,316 +39,511 @@
 namespace sp {
 namespace {
 
-constexpr int kI4Warps = 8;
-constexpr int kI4Deep = 5;  // stages of a warp's ring: four chunks (1 KB) in flight
-constexpr int kMaxSmem = 200 * 1024;
-constexpr double kBlockCost = 3, kJoinCost = 2;  // see choose_split
+constexpr int kI4Warps = 16;
+constexpr int kI4Deep = 3;          // stages of a warp's ring, of a chunk (2 KB) each
+constexpr int kI4Tiles = 1 << 16;   // counters of the workspace: row tiles of a launch
+constexpr int kI4Smem = 226 * 1024; // shared memory of a block (the SM's, but for 1 KB)
+constexpr double kTileCost = 0.5, kSlabCost = 1.0, kWarpTime = 9;  // see int4_plan
+constexpr int kRedRow = 36;         // row of the join: 32 values, 36 apart against bank conflicts
+constexpr int kRedBytes = kI4Warps * 8 * kRedRow * 4;
 
 struct Int4Args {
   const void* x;         // [M, K] f16 / bf16 / e4m3
   const float* x_scale;  // [M], e4m3 only
-  const uint4* q;        // [NT, C, 2, 32] 16-byte pieces
-  const uint16_t* s;     // [NT, C, 8, 2, GPC]
-  const uint8_t* z;      // [NT, C, 8, ZB] holding [2, GPC], or null (8)
+  const uint8_t* q;      // [row tiles, C, 4, 32 lanes] 16-byte pieces
+  const uint8_t* s;      // [row tiles, C, 8, 4, GPC] f16 / bf16
+  const uint8_t* z;      // same, bytes, or null (8)
   const void* bias;      // out dtype [N] or null
   void* y;               // [M, N]
+  int32_t* counters;     // [row tiles], all zero between calls
+  float* parts;          // [row tiles, S, NT, 256]
   int64_t x_stride;      // elements
   int M, N, K, C;        // C = chunks of 128 inputs
-  int wr, pass_chunks, s_bf16, out_dtype;
+  int S, cs;             // slabs, chunks of each (the last has the rest)
+  int U;                 // warps of a group
+  int x_dtype, out_dtype;
 };
 
-template <typename T>
-__device__ __forceinline__ void mma_i4(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                       uint32_t b1) {
-  if constexpr (std::is_same_v<T, __half>)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-template <uint32_t MASK, uint32_t MAGIC>
-__device__ __forceinline__ uint32_t and_or(uint32_t w) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "n"(MASK), "n"(MAGIC));
-  return r;
-}
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-  const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t bsub2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 r =
-      __hsub2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// The eight 4-bit values of w (value 2i in nibble i, value 2i+1 in nibble 4+i) minus z, as four
-// pairs of T.  `zoff` is the pair (magic + z) whose mantissa's low bits are the integer z:
-// magic is 1024 in f16 and 128 in bf16, so magic + q is q's bits under the magic exponent and
-// the subtraction is exact.  For f16, nibbles 1 and 3 stay four bits up (1024 + 16 q) and one
-// fused multiply-add by 1/16 takes them down: `zoff16` is -(64 + z).
-template <typename T>
-__device__ __forceinline__ void unpack(uint32_t (&p)[4], uint32_t w, uint32_t zoff,
-                                       uint32_t zoff16) {
-  if constexpr (std::is_same_v<T, __half>) {
-    const uint32_t v = w >> 8;
-    p[0] = hsub2(and_or<0x000f000fu, 0x64006400u>(w), zoff);
-    p[2] = hsub2(and_or<0x000f000fu, 0x64006400u>(v), zoff);
-    uint32_t a = and_or<0x00f000f0u, 0x64006400u>(w), b = and_or<0x00f000f0u, 0x64006400u>(v);
-    const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
-    const __half2 off = *reinterpret_cast<__half2*>(&zoff16);
-    __half2 r = __hfma2(*reinterpret_cast<__half2*>(&a), sixteenth, off);
-    p[1] = *reinterpret_cast<uint32_t*>(&r);
-    r = __hfma2(*reinterpret_cast<__half2*>(&b), sixteenth, off);
-    p[3] = *reinterpret_cast<uint32_t*>(&r);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      p[i] = bsub2(and_or<0x000f000fu, 0x43004300u>(w >> (4 * i)), zoff);
-  }
+// d = a b + c, 16 x 8 x 16, f16 operands, f32 sums
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]),
+        "f"(c[2]), "f"(c[3]));
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return (uint32_t)__cvta_generic_to_shared(p);
 }
-// One asynchronous copy of 4, 8 or 16 bytes.
-template <int BYTES>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES)
-                 : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// BYTES of shared memory as words.  Plain loads: the compiler moves them ahead of their use.
 template <int BYTES>
-__device__ __forceinline__ void lds(uint32_t (&r)[(BYTES + 3) / 4], uint32_t addr) {
-  if constexpr (BYTES == 16)
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
-  else if constexpr (BYTES == 8)
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
-                 : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
-  else
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r[0]) : "r"(addr) : "memory");
+__device__ __forceinline__ void lds(uint32_t (&r)[BYTES / 4], const uint8_t* p) {
+  if constexpr (BYTES >= 16) {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      r[4 * i] = v.x, r[4 * i + 1] = v.y, r[4 * i + 2] = v.z, r[4 * i + 3] = v.w;
+    }
+  } else if constexpr (BYTES == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    r[0] = v.x, r[1] = v.y;
+  } else {
+    r[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
 }
 
-// A warp's ring: per chunk in flight and lane, its 16 bytes of rows g and of rows g + 8, its
-// scales and its zeros, each lane's own (no lane reads what another one copied).
+// A warp's ring: per stage the lanes' 4 x 16 bytes, then the chunk's scales and zeros, which lanes
+// 0 .. SB / 16 - 1 and 16 .. 16 + ZB / 16 - 1 copy for all.
 template <int GPC, bool ZP>
 struct Ring {
-  static constexpr int SB = 4 * GPC;                      // scales of two rows
-  static constexpr int ZB = ZP ? (GPC == 1 ? 4 : 2 * GPC) : 0;
-  static constexpr int STAGE = 32 * (32 + SB + ZB);
+  static constexpr int SB = 64 * GPC;            // scales: 8 x 4 rows x GPC
+  static constexpr int ZB = ZP ? 32 * GPC : 0;   // zeros
+  static constexpr int STAGE = 2048 + SB + ZB;
   static constexpr int WARP = kI4Deep * STAGE;
   static constexpr int BLOCK = kI4Warps * WARP;
 };
-__host__ __device__ constexpr int zero_bytes(int gpc) { return gpc == 1 ? 4 : 2 * gpc; }
 
-// T: the MMA's type (x's, or f16 for e4m3 x).  NT: n-tiles of 8 rows of x.  GPC: groups per
-// chunk of 128 inputs (4: groups of 32, 2: of 64, 1: of 128 and more).
-template <typename T, bool XE4M3, int NT, int GPC, bool ZP>
-__global__ void __launch_bounds__(kI4Warps * 32, 2) int4_linear_kernel(const Int4Args a) {
-  namespace cg = cooperative_groups;
+// The power of two that brings a row's largest magnitude to [2^14, 2^15) (1 for rows of zeros
+// and rows with infinities or NaNs), as the exponent field of an f32.
+__device__ __forceinline__ uint32_t row_exponent(uint32_t amax_bits) {
+  const uint32_t e = amax_bits >> 23;
+  if (amax_bits == 0 || e == 255) return 127;
+  return min(268u - e, 253u);
+}
+
+// How a block's warps go over mrows rows of `groups` 16-byte groups of 8 inputs: `parts` warps
+// to a row, each lane every (32 parts)-th group, kXBatch loads at a time.
+constexpr int kXBatch = 8;
+struct XWalk {
+  int row, rows, first, step;
+  __device__ __forceinline__ XWalk(int mrows) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int parts = 1;
+    while (2 * parts * mrows <= kI4Warps) parts *= 2;
+    rows = kI4Warps / parts;
+    row = warp / parts;
+    first = warp % parts * 32 + lane;
+    step = parts * 32;
+  }
+};
+
+template <int XD>
+using XVec = std::conditional_t<XD == SP_E4M3, uint2, uint4>;
+
+template <int XD>
+__device__ __forceinline__ const XVec<XD>* x_row(const Int4Args& a, int m, int k0) {
+  return reinterpret_cast<const XVec<XD>*>(static_cast<const uint8_t*>(a.x) +
+                                           ((int64_t)m * a.x_stride + k0) * (sizeof(XVec<XD>) / 8));
+}
+template <int XD>
+__device__ __forceinline__ void x_load(XVec<XD> (&v)[kXBatch], const XVec<XD>* row, int i, int step,
+                                       int live) {
+#pragma unroll
+  for (int u = 0; u < kXBatch; ++u)
+    v[u] = i + u * step < live ? __ldg(row + i + u * step) : XVec<XD>{};
+}
+
+// The largest magnitude of a batch of 16-bit values, which order like their bits.
+__device__ __forceinline__ uint32_t x_max(const uint4 (&v)[kXBatch], uint32_t mx) {
+#pragma unroll
+  for (int u = 0; u < kXBatch; ++u) {
+    mx = __vmaxu2(mx, v[u].x & 0x7fff7fffu);
+    mx = __vmaxu2(mx, v[u].y & 0x7fff7fffu);
+    mx = __vmaxu2(mx, v[u].z & 0x7fff7fffu);
+    mx = __vmaxu2(mx, v[u].w & 0x7fff7fffu);
+  }
+  return mx;
+}
+// ... of the warp's part of a row, into the row's word of amax as f32 bits
+template <int XD>
+__device__ __forceinline__ void x_max_row(uint32_t mx, uint32_t* amax) {
+  const uint32_t h = __reduce_max_sync(0xffffffffu, max(mx & 0xffffu, mx >> 16));
+  if ((threadIdx.x & 31) == 0)
+    atomicMax(amax, XD == SP_BF16
+                        ? h << 16
+                        : __float_as_uint(__half2float(__ushort_as_half((unsigned short)h))));
+}
+
+// A batch into shared memory as f16 times the row's power of two, pairs 1 and 3 of each 16-byte
+// group also by 1/16.
+template <int XD>
+__device__ __forceinline__ void x_put(const XVec<XD> (&v)[kXBatch], float mul, uint8_t* dst, int i,
+                                      int step, int groups) {
+  const float mul16 = mul * 0.0625f;
+#pragma unroll
+  for (int u = 0; u < kXBatch; ++u) {
+    uint32_t o[4];
+    if constexpr (XD == SP_E4M3) {
+      const uint32_t in[2] = {v[u].x, v[u].y};
+      const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;"
+            : "=r"(o[h]) : "h"((uint16_t)(in[h >> 1] >> (16 * (h & 1)))));
+        if (h & 1) {
+          const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&o[h]), sixteenth);
+          o[h] = *reinterpret_cast<const uint32_t*>(&r);
+        }
+      }
+    } else {
+      const uint32_t in[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        float2 f;
+        if constexpr (XD == SP_BF16)
+          f = make_float2(__uint_as_float(in[h] << 16), __uint_as_float(in[h] & 0xffff0000u));
+        else
+          f = __half22float2(*reinterpret_cast<const __half2*>(&in[h]));
+        const float c = h & 1 ? mul16 : mul;
+        const __half2 r = __floats2half2_rn(f.x * c, f.y * c);
+        o[h] = *reinterpret_cast<const uint32_t*>(&r);
+      }
+    }
+    if (i + u * step < groups)
+      *reinterpret_cast<uint4*>(dst + (i + u * step) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// The block's slab of x into shared memory.  16-bit rows need their largest magnitude first; where
+// a lane's whole share is one batch (short slabs, up to 16 rows) it stays in registers between.
+template <int XD>
+__device__ __forceinline__ void x_stage(const Int4Args& a, int mrows, int k0, int groups, int live,
+                                        uint32_t* amax, uint8_t* xsm, int xrow) {
+  const XWalk w(mrows);
+  XVec<XD> v[kXBatch];
+  const bool once = mrows <= w.rows && groups <= w.step * kXBatch;
+  if constexpr (XD != SP_E4M3) {
+    for (int m = w.row; m < mrows; m += w.rows) {
+      uint32_t mx = 0;
+      for (int i = w.first; i < groups; i += w.step * kXBatch) {
+        x_load<XD>(v, x_row<XD>(a, m, k0), i, w.step, live);
+        mx = x_max(v, mx);
+      }
+      x_max_row<XD>(mx, amax + m);
+    }
+    __syncthreads();
+  }
+  for (int m = w.row; m < mrows; m += w.rows) {
+    const float mul = __uint_as_float(row_exponent(amax[m]) << 23);
+    for (int i = w.first; i < groups; i += w.step * kXBatch) {
+      if (XD == SP_E4M3 || !once) x_load<XD>(v, x_row<XD>(a, m, k0), i, w.step, live);
+      x_put<XD>(v, mul, xsm + m * xrow, i, w.step, groups);
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ void store_y(const Int4Args& a, int m, int n, float v) {
+  if (a.x_scale) v *= a.x_scale[m];
+  const int64_t at = (int64_t)m * a.N + n;
+  if (a.out_dtype == SP_F32) {
+    if (a.bias) v += static_cast<const float*>(a.bias)[n];
+    static_cast<float*>(a.y)[at] = v;
+  } else if (a.out_dtype == SP_F16) {
+    if (a.bias) v += __half2float(static_cast<const __half*>(a.bias)[n]);
+    static_cast<__half*>(a.y)[at] = __float2half_rn(v);
+  } else {
+    if (a.bias) v += __bfloat162float(static_cast<const __nv_bfloat16*>(a.bias)[n]);
+    static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
+  }
+}
+
+// An accumulator fragment: rows m and m + 1 of x, outputs n and n + 8.
+__device__ __forceinline__ void store_frag(const Int4Args& a, const float (&v)[4], int m, int n,
+                                           int mrows) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (m + (e & 1) < mrows && n + (e >> 1) * 8 < a.N)
+      store_y(a, m + (e & 1), n + (e >> 1) * 8, v[e]);
+}
+
+// Waits for the U warps of group `id` (a warp alone: for its lanes).
+__device__ __forceinline__ void group_sync(int id, int U) {
+  if (U == 1) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(U * 32) : "memory");
+}
+
+// NT: n-tiles of 8 rows of x.  GPC: groups per chunk of 128 inputs (4: groups of 32, 2: of 64,
+// 1: of 128 and more).  ZP: zero points (else 8).  SBF: bf16 scales (else f16).
+template <int NT, int GPC, bool ZP, bool SBF>
+__global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int4Args a) {
   using R = Ring<GPC, ZP>;
+  constexpr int TM = 8 * NT;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float red[kI4Warps][16][8 * NT];
+  __shared__ uint32_t amax[TM];
+  __shared__ float back[TM];
+  __shared__ float red[kI4Warps * 8 * kRedRow];
+  __shared__ int last_flag[kI4Warps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
-  const int S = gridDim.y, split = blockIdx.y;
-  const int m0 = blockIdx.z * 8 * NT;
-  const int mrows = min(8 * NT, a.M - m0);
-  const int WK = kI4Warps / a.wr, wr = warp % a.wr, wk = warp / a.wr;
-  const int n_tiles = (a.N + 15) / 16;
-  const int tile = blockIdx.x * a.wr + wr;
-  const int cb = (int)((int64_t)a.C * split / S), ce = (int)((int64_t)a.C * (split + 1) / S);
-  uint8_t* xsm = smem + R::BLOCK;
+  const int mrows = min(TM, a.M);
+  const int n_tiles = (a.N + 31) / 32;
+  const int U = a.U, group = warp / U, gw = warp - group * U;
+  const int slab = blockIdx.x % a.S, cb = slab * a.cs, cs = min(a.cs, a.C - cb);
+  // this group's tiles: tile0, tile0 + tile_step, ... (consecutive tiles to different blocks);
+  // this warp's chunks of each: gw, gw + U, ...
+  const int slab_blocks = (int)gridDim.x / a.S;
+  const int tile0 = blockIdx.x / a.S + group * slab_blocks;
+  const int tile_step = slab_blocks * (kI4Warps / U);
   const uint32_t ring = smem_u32(smem) + warp * R::WARP;
+  float* xsum = reinterpret_cast<float*>(smem + R::BLOCK);  // [cs, GPC, TM]
+  uint8_t* xsm = smem + R::BLOCK + cs * GPC * TM * 4;
 
-  float tot[NT][4];
+  // ---- the copy side: the next chunk to copy
+  int ft = tile0, fc = gw;
+  if (gw >= cs) ft = n_tiles;  // nothing for this warp
+  const uint8_t* qsrc = a.q + lane * 16;
+  const bool is_z = ZP && lane >= 16 && lane < 16 + R::ZB / 16;
+  const bool meta = lane < R::SB / 16 || is_z;
+  const uint8_t* msrc = is_z ? a.z + (lane - 16) * 16 : a.s + lane * 16;
+  const int mstep = is_z ? R::ZB : R::SB;
+  const uint32_t mdst = 2048 + (is_z ? R::SB + (lane - 16) * 16 : lane * 16);
+  auto fetch = [&](uint32_t stage) {
+    if (ft < n_tiles) {
+      const int64_t at = (int64_t)ft * a.C + cb + fc;
+      const uint8_t* q = qsrc + at * 2048;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cp_async16(stage + i * 512 + lane * 16, q + i * 512);
+      if (meta) cp_async16(stage + mdst, msrc + at * mstep);
+      fc += U;
+      if (fc >= cs) {
+        fc = gw;
+        ft += tile_step;
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int u = 0; u < kI4Deep - 1; ++u) fetch(ring + u * R::STAGE);
+
+  // ---- the slab of x: row m at m * (256 cs + 64) bytes (64 so that two rows' 64-byte pieces
+  // fall into different halves of the banks)
+  const int xrow = cs * 256 + 64;
+  {
+    const int k0 = cb * 128, groups16 = cs * 16, live = (min((cb + cs) * 128, a.K) - k0) / 8;
+    if (tid < TM) amax[tid] = 0;
+    __syncthreads();
+    if (a.x_dtype == SP_E4M3) x_stage<SP_E4M3>(a, mrows, k0, groups16, live, amax, xsm, xrow);
+    else if (a.x_dtype == SP_BF16) x_stage<SP_BF16>(a, mrows, k0, groups16, live, amax, xsm, xrow);
+    else x_stage<SP_F16>(a, mrows, k0, groups16, live, amax, xsm, xrow);
+    // what undoes the staged row's power of two and the weights' 2^-24
+    if (tid < TM) back[tid] = __uint_as_float((254u - row_exponent(amax[tid])) << 23) * 0x1p24f;
+  }
+
+  // lanes beyond the last row of x repeat it: their MMA columns are never stored
+  const uint8_t* xbase[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
+    xbase[n] = xsm + min(n * 8 + g, mrows - 1) * xrow + t4 * 16;
+  const float zero4[4] = {0.f, 0.f, 0.f, 0.f};
+  // ---- the groups' sums of x, in the accumulators' unit 2^-24 and times -8 (symmetric) or
+  // -1 (to be multiplied by the zero point)
+  for (int i = warp; i < cs; i += kI4Warps) {
+    const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u};  // 1, 16
+    const float unit = ZP ? -0x1p-24f : -0x1p-21f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tot[n][i] = 0.f;
-
-  for (int p0 = cb; p0 < ce; p0 += a.pass_chunks) {
-    const int pc = min(a.pass_chunks, ce - p0);
-    const int w0 = p0 + pc * wk / WK;
-    const int n_chunks = tile < n_tiles ? p0 + pc * (wk + 1) / WK - w0 : 0;
-    const int64_t chunk0 = (int64_t)tile * a.C + w0;
-    const uint8_t* qp = reinterpret_cast<const uint8_t*>(a.q) + chunk0 * 1024 + lane * 16;
-    const uint8_t* sp_ = reinterpret_cast<const uint8_t*>(a.s) + (chunk0 * 8 + g) * R::SB;
-    const uint8_t* zp = ZP ? a.z + (chunk0 * 8 + g) * R::ZB : nullptr;
-    int copied = 0;  // chunks whose copies have been issued; the pointers stand at the next one
-    auto fetch = [&](uint32_t stage) {
-      if (copied < n_chunks) {
-        cp_async<16>(stage + lane * 16, qp);
-        cp_async<16>(stage + 512 + lane * 16, qp + 512);
-        cp_async<R::SB>(stage + 1024 + lane * R::SB, sp_);
-        if constexpr (ZP) cp_async<R::ZB>(stage + 1024 + 32 * R::SB + lane * R::ZB, zp);
-        qp += 1024;
-        sp_ += 8 * R::SB;
-        if constexpr (ZP) zp += 8 * R::ZB;
-        ++copied;
+    for (int n = 0; n < NT; ++n) {
+      float acc[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        constexpr int JPG = 4 / GPC;
+        uint32_t b[4];
+        lds<16>(b, xbase[n] + i * 256 + j * 64);
+        if (j % JPG == 0) mma_f16(acc, ones, b[0], b[1], zero4);
+        else mma_f16(acc, ones, b[0], b[1], acc);
+        mma_f16(acc, ones, b[2], b[3], acc);
+        if (j % JPG == JPG - 1 && g == 0)
+          *reinterpret_cast<float2*>(xsum + (i * GPC + j / JPG) * TM + n * 8 + t4 * 2) =
+              make_float2(acc[0] * unit, acc[1] * unit);
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll
-    for (int u = 0; u < kI4Deep - 1; ++u) fetch(ring + u * R::STAGE);
+    }
+  }
+  __syncthreads();
 
-    // ---- x of this pass: row m at m * (256 pc + 64) bytes (64 so that two rows' 64-byte
-    // pieces fall into different halves of the banks); inputs beyond K are zeros
-    const int xrow = pc * 256 + 64;
-    if (p0 != cb) __syncthreads();
-    for (int m = 0; m < mrows; ++m)
-      for (int grp = tid; grp < pc * 16; grp += kI4Warps * 32) {
-        const int k = p0 * 128 + grp * 8;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (k < a.K) {
-          if constexpr (XE4M3) {
-            const uint2 b = __ldg(reinterpret_cast<const uint2*>(
-                static_cast<const uint8_t*>(a.x) + (int64_t)(m0 + m) * a.x_stride + k));
-            uint32_t* o = reinterpret_cast<uint32_t*>(&v);
-            const uint32_t in[2] = {b.x, b.y};
+  const uint8_t* ring_p = smem + warp * R::WARP;
+  uint32_t stage = 0, refill = (kI4Deep - 1) * R::STAGE;  // offsets in the ring
+  for (int tile = tile0; tile < n_tiles; tile += tile_step) {
+    float tot[2][NT][4];
 #pragma unroll
-            for (int h = 0; h < 4; ++h)
-              asm("cvt.rn.f16x2.e4m3x2 %0, %1;"
-                  : "=r"(o[h]) : "h"((uint16_t)(in[h >> 1] >> (16 * (h & 1)))));
-          } else {
-            v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) +
-                                                     (int64_t)(m0 + m) * a.x_stride + k));
-          }
-        }
-        *reinterpret_cast<uint4*>(xsm + m * xrow + grp * 16) = v;
-      }
-    __syncthreads();
+    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tot[rt][n][e] = 0.f;
+    const uint8_t* xs = reinterpret_cast<const uint8_t*>(xsum) + t4 * 8 + gw * (GPC * TM * 4);
+    uint32_t xo = gw * 256;
 
-    // lanes beyond the last row of x repeat it: their MMA columns are never stored
-    uint32_t xa[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-      xa[n] = smem_u32(xsm) + min(n * 8 + g, mrows - 1) * xrow + (w0 - p0) * 256 + t4 * 16;
-    uint32_t stage = ring, refill = ring + (kI4Deep - 1) * R::STAGE;
-    for (int i = 0; i < n_chunks; ++i) {
+    for (int c = gw; c < cs; c += U) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kI4Deep - 2) : "memory");
-      uint32_t w[2][4], sm[(R::SB + 3) / 4], zm[ZP ? (R::ZB + 3) / 4 : 1];
-      lds<16>(w[0], stage + lane * 16);
-      lds<16>(w[1], stage + 512 + lane * 16);
-      lds<R::SB>(sm, stage + 1024 + lane * R::SB);
-      if constexpr (ZP) lds<R::ZB>(zm, stage + 1024 + 32 * R::SB + lane * R::ZB);
-      fetch(refill);  // the stage that the previous step has read
+      __syncwarp();  // the lanes' copies of the scales, and their reads of the stage before
+      uint32_t w[4][4], sm[2 * GPC], zm[ZP ? GPC : 1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lds<16>(w[i], ring_p + stage + i * 512 + lane * 16);
+      lds<8 * GPC>(sm, ring_p + stage + 2048 + g * (8 * GPC));
+      if constexpr (ZP) lds<4 * GPC>(zm, ring_p + stage + 2048 + R::SB + g * (4 * GPC));
+      fetch(ring + refill);  // the stage that the previous step has read
       refill = stage;
-      stage = stage + R::STAGE == ring + R::WARP ? ring : stage + R::STAGE;
-      float acc[NT][4];
+      stage = stage + R::STAGE == R::WARP ? 0 : stage + R::STAGE;
+      float acc[2][NT][4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         constexpr int JPG = 4 / GPC;  // words per group
         const int grp = j / JPG;
+        // what the group's accumulators start from
+        float c0[2][NT][4];
         if (j % JPG == 0) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[n][e] = 0.f;
-        }
-        uint32_t p[2][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          constexpr uint32_t magic = std::is_same_v<T, __half> ? 0x64006400u : 0x43004300u;
-          uint32_t zz = 0x00080008u;
+          float z[4];
           if constexpr (ZP) {
-            const int at = h * GPC + grp;
-            zz = (zm[at >> 2] >> (8 * (at & 3))) & 0xffu;
-            zz |= zz << 16;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {  // byte -> f32 through the mantissa of 2^23
+              const int zi = r * GPC + grp;
+              z[r] = __uint_as_float(__byte_perm(zm[zi >> 2], 0x4b000000u, 0x7540 | (zi & 3))) -
+                     8388608.f;
+            }
           }
-          // -(64 + z): 0xd400 is -64 in f16, whose mantissa counts in 1/16
-          unpack<T>(p[h], w[h][j], magic | zz, 0xd400d400u + (zz << 4));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint32_t v[2];
+            lds<8>(v, xs + (grp * TM + n * 8) * 4);
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                c0[rt][n][e] = __uint_as_float(v[e & 1]);
+                if constexpr (ZP) c0[rt][n][e] *= z[rt * 2 + (e >> 1)];
+              }
+          }
         }
-        const uint32_t a0[4] = {p[0][0], p[1][0], p[0][1], p[1][1]};
-        const uint32_t a1[4] = {p[0][2], p[1][2], p[0][3], p[1][3]};
+        // nibbles 0, 1 and, eight bits down, 2, 3 of each half
+        uint32_t p[4][4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const uint32_t v = w[r][j] >> 8;
+          p[r][0] = w[r][j] & 0x000f000fu, p[r][1] = w[r][j] & 0x00f000f0u;
+          p[r][2] = v & 0x000f000fu, p[r][3] = v & 0x00f000f0u;
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           uint32_t b[4];
-          lds<16>(b, xa[n] + j * 64);
-          mma_i4<T>(acc[n], a0, b[0], b[1]);
-          mma_i4<T>(acc[n], a1, b[2], b[3]);
+          lds<16>(b, xbase[n] + xo + j * 64);
+#pragma unroll
+          for (int rt = 0; rt < 2; ++rt) {
+            const uint32_t a0[4] = {p[rt * 2][0], p[rt * 2 + 1][0], p[rt * 2][1], p[rt * 2 + 1][1]};
+            const uint32_t a1[4] = {p[rt * 2][2], p[rt * 2 + 1][2], p[rt * 2][3], p[rt * 2 + 1][3]};
+            if (j % JPG == 0) mma_f16(acc[rt][n], a0, b[0], b[1], c0[rt][n]);
+            else mma_f16(acc[rt][n], a0, b[0], b[1], acc[rt][n]);
+            mma_f16(acc[rt][n], a1, b[2], b[3], acc[rt][n]);
+          }
         }
         if (j % JPG == JPG - 1) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int at = h * GPC + grp;
-            const uint32_t bits = (sm[at >> 1] >> (16 * (at & 1))) & 0xffffu;
-            const float sc = a.s_bf16 ? __uint_as_float(bits << 16)
-                                      : __half2float(__ushort_as_half((unsigned short)bits));
+          for (int r = 0; r < 4; ++r) {
+            const int si = r * GPC + grp;
+            float sc;
+            if constexpr (SBF) {
+              sc = __uint_as_float(si & 1 ? sm[si >> 1] & 0xffff0000u : sm[si >> 1] << 16);
+            } else {
+              const __half2 two = *reinterpret_cast<const __half2*>(&sm[si >> 1]);
+              sc = si & 1 ? __high2float(two) : __low2float(two);
+            }
+            const int rt = r >> 1, h = (r & 1) * 2;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              tot[n][2 * h] += sc * acc[n][2 * h];
-              tot[n][2 * h + 1] += sc * acc[n][2 * h + 1];
+              tot[rt][n][h] += sc * acc[rt][n][h];
+              tot[rt][n][h + 1] += sc * acc[rt][n][h + 1];
             }
           }
         }
       }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) xa[n] += 256;
+      xs += U * (GPC * TM * 4);
+      xo += U * 256;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  }
 
-  // ---- the block's warps, then the cluster's blocks, in order
+    // ---- the tile's end.  A warp alone keeps its values where the MMA left them; a group's
+    // warps join eight rows of x at a time, thread gt owning values gt, gt + 32 U, ... (row
+    // o & 31 of the tile, row o >> 5 of those of x).
+    const int gt = gw * 32 + lane, own = U * 32;
+    float* gred = red + group * U * 8 * kRedRow;
+    float* parts = a.parts + (int64_t)tile * a.S * (NT * 256);
+    float* part = parts + slab * (NT * 256);
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n) {
+      if (U == 1) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) red[warp][g + (e >> 1) * 8][n * 8 + t4 * 2 + (e & 1)] = tot[n][e];
-  __syncthreads();
-  constexpr int TM = 8 * NT;
-  const int vals = a.wr * 16 * TM;
-  for (int i = tid; i < vals; i += kI4Warps * 32) {
-    const int r = i / TM, m = i % TM;
-    float v = 0.f;
-    for (int k = 0; k < WK; ++k) v += red[k * a.wr + (r >> 4)][r & 15][m];
-    red[r >> 4][r & 15][m] = v;  // only this thread reads or writes column (r, m)
-  }
-  if (S > 1) {
-    cg::this_cluster().sync();
-  } else {
-    __syncthreads();
-  }
-  // row-major over the outputs: consecutive threads write consecutive n
-  const int rows = a.wr * 16;
-  const int lo = rows * split / S, hi = rows * (split + 1) / S;
-  const int mine = hi - lo;
-  for (int i = tid; i < mine * mrows; i += kI4Warps * 32) {
-    const int m = i / mine, r = lo + i % mine;
-    const int n = blockIdx.x * rows + r;
-    float v = 0.f;
-    if (S > 1) {
-      for (int c = 0; c < S; ++c)
-        v += *cg::this_cluster().map_shared_rank(&red[r >> 4][r & 15][m], c);
-    } else {
-      v = red[r >> 4][r & 15][m];
-    }
-    if (n < a.N) {
-      if (a.x_scale) v *= a.x_scale[m0 + m];
-      const int64_t at = (int64_t)(m0 + m) * a.N + n;
-      if (a.out_dtype == SP_F32) {
-        if (a.bias) v += static_cast<const float*>(a.bias)[n];
-        static_cast<float*>(a.y)[at] = v;
-      } else if (a.out_dtype == SP_F16) {
-        if (a.bias) v += __half2float(static_cast<const __half*>(a.bias)[n]);
-        static_cast<__half*>(a.y)[at] = __float2half_rn(v);
+        for (int rt = 0; rt < 2; ++rt) {
+          const float b0 = back[n * 8 + t4 * 2], b1 = back[n * 8 + t4 * 2 + 1];
+          const float v[4] = {tot[rt][n][0] * b0, tot[rt][n][1] * b1, tot[rt][n][2] * b0,
+                              tot[rt][n][3] * b1};
+          if (a.S > 1)
+            __stcg(reinterpret_cast<float4*>(part) + (n * 2 + rt) * 32 + lane,
+                   make_float4(v[0], v[1], v[2], v[3]));
+          else
+            store_frag(a, v, n * 8 + t4 * 2, tile * 32 + rt * 16 + g, mrows);
+        }
       } else {
-        if (a.bias) v += __bfloat162float(static_cast<const __nv_bfloat16*>(a.bias)[n]);
-        static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
+        group_sync(group, U);  // the sums of before are read
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            gred[(gw * 8 + t4 * 2 + (e & 1)) * kRedRow + rt * 16 + (e >> 1) * 8 + g] =
+                tot[rt][n][e];
+        group_sync(group, U);
+        for (int o = gt; o < 256; o += own) {
+          const int m = n * 8 + (o >> 5), row = tile * 32 + (o & 31);
+          float v = 0.f;
+#pragma unroll 2
+          for (int k = 0; k < U; ++k) v += gred[(k * 8 + (o >> 5)) * kRedRow + (o & 31)];
+          v *= back[m];
+          if (a.S > 1) __stcg(part + n * 256 + o, v);
+          else if (m < mrows && row < a.N) store_y(a, m, row, v);
+        }
+      }
+    }
+    if (a.S > 1) {
+      // one thread's release covers the group's stores, which the barrier orders before it
+      group_sync(group, U);
+      if (gt == 0) {
+        int before;
+        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;"
+                     : "=r"(before) : "l"(a.counters + tile) : "memory");
+        const bool last = before == a.S - 1;
+        if (last) a.counters[tile] = 0;  // zero again for the next call
+        last_flag[group] = last;
+      }
+      group_sync(group, U);
+      if (last_flag[group]) {
+        if (U == 1) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) {
+              float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+              for (int k = 0; k < a.S; ++k) {
+                const float4 p = __ldcg(reinterpret_cast<const float4*>(parts + k * (NT * 256)) +
+                                        (n * 2 + rt) * 32 + lane);
+                v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+              }
+              store_frag(a, v, n * 8 + t4 * 2, tile * 32 + rt * 16 + g, mrows);
+            }
+        } else {
+          for (int o = gt; o < NT * 256; o += own) {
+            const int m = o >> 5, row = tile * 32 + (o & 31);
+            float v = 0.f;
+#pragma unroll 4
+            for (int k = 0; k < a.S; ++k) v += __ldcg(parts + k * (NT * 256) + o);
+            if (m < mrows && row < a.N) store_y(a, m, row, v);
+          }
+        }
       }
     }
   }
-  if (S > 1) cg::this_cluster().sync();  // the others may still read this block's sums
 }
 
 // One thread per output word of the weights, then of the scales (and zeros).
@@ -342,9 +552,9 @@ __global__ void int4_repack_kernel(const uint8_t* q, const uint16_t* s, const ui
                                    uint32_t* qo, uint16_t* so, uint8_t* zo) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i < words) {
-    const int j = i & 3, lane = (i >> 2) & 31, h = (i >> 7) & 1;
-    const int64_t chunk = i >> 8;
-    const int64_t row = chunk / C * 16 + h * 8 + (lane >> 2);
+    const int j = i & 3, lane = (i >> 2) & 31, r = (i >> 7) & 3;
+    const int64_t chunk = i >> 9;
+    const int64_t row = chunk / C * 32 + r * 8 + (lane >> 2);
     const int k = (int)(chunk % C) * 128 + j * 32 + (lane & 3) * 8;
     uint32_t v = 0;
     if (row < N && k < K)
@@ -355,16 +565,13 @@ __global__ void int4_repack_kernel(const uint8_t* q, const uint16_t* s, const ui
     qo[i] = v;
   } else if (i - words < metas) {
     const int64_t j = i - words;
-    const int gi = (int)(j % gpc), h = (int)(j / gpc) & 1, g = (int)(j / gpc / 2) & 7;
-    const int64_t chunk = j / gpc / 16;
-    const int64_t row = chunk / C * 16 + h * 8 + g;
+    const int gi = (int)(j % gpc), r = (int)(j / gpc) & 3, g = (int)(j / gpc / 4) & 7;
+    const int64_t chunk = j / gpc / 32;
+    const int64_t row = chunk / C * 32 + r * 8 + g;
     const int64_t grp = ((chunk % C) * 128 + (gpc > 1 ? gi * group : 0)) / group;
     const bool live = row < N && grp < K / group;
     so[j] = live ? s[grp * N + row] : 0;
-    if (zo) {
-      const int zb = zero_bytes(gpc);
-      zo[(chunk * 8 + g) * zb + h * gpc + gi] = live ? z[grp * N + row] & 15 : 8;
-    }
+    if (zo) zo[j] = live ? z[grp * N + row] & 15 : 8;
   }
 }
 
@@ -376,17 +583,15 @@ __global__ void int4_dequant_kernel(const uint32_t* q, const uint16_t* s, const 
   if (i >= (int64_t)N * K) return;
   const int64_t row = i / K;
   const int k = (int)(i % K), c = k >> 7, kk = k & 127;
-  const int64_t chunk = row / 16 * C + c;
-  const int g = (int)(row & 7), h = (int)(row >> 3) & 1;
+  const int64_t chunk = row / 32 * C + c;
+  const int g = (int)(row & 7), r = (int)(row >> 3) & 3;
   const int j = kk >> 5, t = (kk >> 3) & 3, e = kk & 7;
-  const uint32_t w = q[((chunk * 2 + h) * 32 + g * 4 + t) * 4 + j];
+  const uint32_t w = q[((chunk * 4 + r) * 32 + g * 4 + t) * 4 + j];
   const int v = (w >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15;
-  const int gi = j * gpc / 4;
-  const int64_t at = (chunk * 16 + g * 2 + h) * gpc + gi;
-  const int zero = z ? z[(chunk * 8 + g) * zero_bytes(gpc) + h * gpc + gi] : 8;
+  const int64_t at = (chunk * 32 + g * 4 + r) * gpc + j * gpc / 4;
   const float sc = s_bf16 ? __uint_as_float((uint32_t)s[at] << 16)
                           : __half2float(__ushort_as_half(s[at]));
-  out[i] = from_f32<T>((float)(v - zero) * sc);
+  out[i] = from_f32<T>((float)(v - (z ? (int)z[at] : 8)) * sc);
 }
 
 struct Int4Shape {
@@ -403,90 +608,89 @@ int int4_shape(Int4Shape& sh, int64_t N, int64_t K, int64_t group) {
                      (long long)K, (long long)group);
   if (N > (1LL << 30) || K > (1LL << 30))
     return set_error(SP_ERR_SHAPE, "int4 linear: N or K too large");
-  sh.nt = (N + 15) / 16;
+  sh.nt = (N + 31) / 32;
   sh.c = (K + 127) / 128;
+  if (sh.nt * sh.c > (1LL << 30))
+    return set_error(SP_ERR_SHAPE, "int4 linear: the weight is too large");
   sh.gpc = group >= 128 ? 1 : 128 / group;
   return SP_OK;
 }
 
-// The shape of the launch: a.wr row tiles per block (its other warps split the inputs), S blocks
-// per cluster and a.pass_chunks chunks of x in shared memory at a time; out of all (wr, S) the
-// one with the least time by this count: waves of blocks, each as long as its busiest warp's
-// chunks plus the cost of a block's start and end (kBlockCost chunks; more for a cluster's
-// join).  `fixed`: the block's shared memory beside x.  Returns S.
-int choose_split(Int4Args& a, int tokens, int m_tiles, int fixed) {
-  const int n_tiles = (a.N + 15) / 16;
-  const int fit = ((kMaxSmem - fixed) / tokens - 64) / 256;
-  int best_s = 1;
+struct Int4Plan {
+  int blocks, S, cs, U;
+  size_t smem, part_bytes;
+};
+// The launch of up to 32 rows: S slabs, at least as many as let a block hold its slab of x beside
+// its rings, and U warps per group, so that the schedule is shortest.  Counted in chunks of an SM
+// that is kept busy: a block's chunks, or kWarpTime times those of its busiest warp if that is
+// more (fewer than kWarpTime warps do not keep an SM busy), each tile with the cost of its join,
+// in chunks of each of its warps.
+Int4Plan int4_plan(int64_t M, int64_t N, int64_t C, int gpc, int ring_bytes) {
+  const int NT = M <= 8 ? 1 : M <= 16 ? 2 : 4;
+  const int64_t tokens = M < 8 * NT ? M : 8 * NT, n_tiles = (N + 31) / 32;
+  const int64_t per_chunk = tokens * 256 + gpc * 8 * NT * 4;
+  const int64_t fixed = 1024 + kRedBytes + ring_bytes + tokens * 64;
+  const int64_t sms = num_sms(), fit = (kI4Smem - fixed) / per_chunk;
+  const int64_t s_min = (C + fit - 1) / fit, s_max = s_min < 8 ? 16 : 2 * s_min;
+  Int4Plan p{};
   double best = 1e300;
-  for (int wr = 1; wr <= kI4Warps; wr *= 2) {
-    const int wk = kI4Warps / wr;
-    for (int S = 1; S <= 8; ++S) {
-      if (S > 1 && a.C < S * wk) break;
-      const int range = (a.C + S - 1) / S;
-      const int pass = range < fit ? range : fit;
-      const int smem = fixed + tokens * (pass * 256 + 64) + 1024;
-      const int64_t slots = (int64_t)num_sms() * (2 * smem <= 227 * 1024 ? 2 : 1);
-      const int64_t blocks = (int64_t)((n_tiles + wr - 1) / wr) * S * m_tiles;
-      const int64_t waves = (blocks + slots - 1) / slots;
-      const int chunks = (range + wk - 1) / wk;
-      const double cost = (double)waves * (chunks + kBlockCost + (S > 1 ? kJoinCost : 0));
-      if (cost < best - 1e-9) best = cost, best_s = S, a.wr = wr, a.pass_chunks = pass;
+  for (int64_t s = s_min; s <= s_max; ++s) {
+    const int64_t cs = (C + s - 1) / s, S = (C + cs - 1) / cs;
+    if (S != s) continue;  // the same cut as a smaller s
+    const int64_t per_slab = S < sms ? sms / S : 1;  // blocks
+    for (int U = 1; U <= kI4Warps; U *= 2) {
+      const int64_t groups = per_slab * (kI4Warps / U);
+      const int64_t of_block = (n_tiles + per_slab - 1) / per_slab;
+      const int64_t of_group = (n_tiles + groups - 1) / groups;
+      const double join = kTileCost + (S > 1 ? kSlabCost : 0);
+      const double warp = (double)of_group * ((cs + U - 1) / U + join);
+      const double sm = (double)of_block * (cs + join * U);
+      const double cost = sm > kWarpTime * warp ? sm : kWarpTime * warp;
+      if (cost < best - 1e-9) {
+        best = cost;
+        p.S = (int)S, p.cs = (int)cs, p.U = U;
+        p.blocks = (int)((n_tiles < per_slab ? n_tiles : per_slab) * S);
+      }
     }
   }
-  return best_s;
+  p.smem = (size_t)(ring_bytes + tokens * 64 + p.cs * per_chunk);
+  p.part_bytes = p.S > 1 ? (size_t)(n_tiles * p.S * NT) * 1024 : 0;
+  return p;
 }
 
-template <typename T, bool XE4M3, int NT, int GPC, bool ZP>
+int ring_bytes(int gpc, bool zp) {
+  return kI4Warps * kI4Deep * (2048 + 64 * gpc + (zp ? 32 * gpc : 0));
+}
+
+template <int NT, int GPC, bool ZP, bool SBF>
 int launch_int4(Int4Args a, cudaStream_t s) {
-  auto kernel = int4_linear_kernel<T, XE4M3, NT, GPC, ZP>;
-  using R = Ring<GPC, ZP>;
+  auto kernel = int4_linear_kernel<NT, GPC, ZP, SBF>;
   static unsigned long long flags = 0;
   if (first_time_on_device(&flags) &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           kMaxSmem - kI4Warps * 16 * 8 * NT * 4) !=
-          cudaSuccess)
+                           kI4Smem - 1024 - kRedBytes) != cudaSuccess)
     return set_error(SP_ERR_LAUNCH, "int4 linear: shared memory attribute: %s",
                      cudaGetErrorString(cudaGetLastError()));
-  const int tokens = a.M < 8 * NT ? a.M : 8 * NT;
-  const int m_tiles = (a.M + 8 * NT - 1) / (8 * NT);
-  const int S = choose_split(a, tokens, m_tiles, R::BLOCK + kI4Warps * 16 * 8 * NT * 4);
-  const int row_blocks = ((a.N + 15) / 16 + a.wr - 1) / a.wr;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(row_blocks, S, (a.M + 8 * NT - 1) / (8 * NT));
-  cfg.blockDim = dim3(kI4Warps * 32);
-  cfg.dynamicSmemBytes = R::BLOCK + (size_t)tokens * (a.pass_chunks * 256 + 64);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 1, attr.val.clusterDim.y = S, attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return set_error(SP_ERR_LAUNCH, "int4 linear: launch failed: %s", cudaGetErrorString(e));
-  }
-  return SP_OK;
+  const Int4Plan p = int4_plan(a.M, a.N, a.C, GPC, Ring<GPC, ZP>::BLOCK);
+  a.S = p.S, a.cs = p.cs, a.U = p.U;
+  kernel<<<p.blocks, kI4Warps * 32, p.smem, s>>>(a);
+  return check_launch("int4 linear");
 }
 
-template <typename T, bool XE4M3, int NT>
-int launch_int4_g(const Int4Args& a, int gpc, cudaStream_t s) {
-  switch (gpc * 2 + (a.z ? 1 : 0)) {
-    case 2: return launch_int4<T, XE4M3, NT, 1, false>(a, s);
-    case 3: return launch_int4<T, XE4M3, NT, 1, true>(a, s);
-    case 4: return launch_int4<T, XE4M3, NT, 2, false>(a, s);
-    case 5: return launch_int4<T, XE4M3, NT, 2, true>(a, s);
-    case 8: return launch_int4<T, XE4M3, NT, 4, false>(a, s);
-    default: return launch_int4<T, XE4M3, NT, 4, true>(a, s);
-  }
+template <int NT, int GPC>
+int launch_int4_zs(const Int4Args& a, bool sbf, cudaStream_t s) {
+  if (a.z) return sbf ? launch_int4<NT, GPC, true, true>(a, s)
+                      : launch_int4<NT, GPC, true, false>(a, s);
+  return sbf ? launch_int4<NT, GPC, false, true>(a, s) : launch_int4<NT, GPC, false, false>(a, s);
 }
 
-template <typename T, bool XE4M3>
-int launch_int4_m(const Int4Args& a, int gpc, cudaStream_t s) {
-  if (a.M <= 8) return launch_int4_g<T, XE4M3, 1>(a, gpc, s);
-  if (a.M <= 16) return launch_int4_g<T, XE4M3, 2>(a, gpc, s);
-  return launch_int4_g<T, XE4M3, 4>(a, gpc, s);
+template <int NT>
+int launch_int4_g(const Int4Args& a, int gpc, bool sbf, cudaStream_t s) {
+  switch (gpc) {
+    case 1: return launch_int4_zs<NT, 1>(a, sbf, s);
+    case 2: return launch_int4_zs<NT, 2>(a, sbf, s);
+    default: return launch_int4_zs<NT, 4>(a, sbf, s);
+  }
 }
 
 }  // namespace
@@ -498,9 +702,9 @@ extern "C" int sp_int4_packed_bytes(int64_t N, int64_t K, int64_t group, int64_t
   if (!sizes) return set_error(SP_ERR_INVALID_ARG, "int4 linear: null pointer");
   Int4Shape sh{};
   if (int rc = int4_shape(sh, N, K, group)) return rc;
-  sizes[0] = sh.nt * sh.c * 1024;
-  sizes[1] = sh.nt * sh.c * 16 * sh.gpc * 2;
-  sizes[2] = sh.nt * sh.c * 8 * zero_bytes((int)sh.gpc);
+  sizes[0] = sh.nt * sh.c * 2048;
+  sizes[1] = sh.nt * sh.c * 64 * sh.gpc;
+  sizes[2] = sh.nt * sh.c * 32 * sh.gpc;
   sizes[3] = 0;
   return SP_OK;
 }
@@ -518,7 +722,7 @@ extern "C" int sp_int4_repack(const void* qweight, const void* scales, const voi
       !aligned(z_packed, 16))
     return set_error(SP_ERR_ALIGN, "int4 repack: the packed arrays must be 16-byte aligned");
   if (int rc = require_sm100()) return rc;
-  const int64_t words = sh.nt * sh.c * 256, metas = sh.nt * sh.c * 16 * sh.gpc;
+  const int64_t words = sh.nt * sh.c * 512, metas = sh.nt * sh.c * 32 * sh.gpc;
   const int64_t blocks = (words + metas + 255) / 256;
   if (blocks > 2147483647LL) return set_error(SP_ERR_SHAPE, "int4 repack: weight too large");
   int4_repack_kernel<<<(unsigned)blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(
@@ -561,19 +765,35 @@ extern "C" int sp_int4_dequant(const void* q_packed, const void* s_packed, const
   return check_launch("int4 dequant");
 }
 
+extern "C" size_t sp_int4_linear_workspace_size(int64_t M, int64_t N, int64_t K, int64_t group) {
+  using namespace sp;
+  Int4Shape sh{};
+  if (M <= 0 || int4_shape(sh, N, K, group)) return 0;
+  if (M > 32) M = 32;
+  // with and without zero points (whose ring leaves less room for x)
+  size_t most = 0;
+  for (int zp = 0; zp < 2; ++zp) {
+    const Int4Plan p = int4_plan(M, N, sh.c, (int)sh.gpc, ring_bytes((int)sh.gpc, zp));
+    if (p.part_bytes > most) most = p.part_bytes;
+  }
+  return (size_t)kI4Tiles * sizeof(int32_t) + most;
+}
+
 extern "C" int sp_int4_linear(const void* x, int64_t x_row_stride, int x_dtype,
                               const float* x_scale, const void* q_packed, const void* s_packed,
                               const void* z_packed, int scale_dtype, const void* bias, void* y,
                               int64_t M, int64_t N, int64_t K, int64_t group, int out_dtype,
-                              void* stream) {
+                              void* workspace, size_t workspace_bytes, void* stream) {
   using namespace sp;
   clear_error();
   Int4Shape sh{};
   if (int rc = int4_shape(sh, N, K, group)) return rc;
   if (!q_packed || !s_packed || (M != 0 && (!x || !y)))
     return set_error(SP_ERR_INVALID_ARG, "int4 linear: null pointer");
-  if (M < 0 || M > 2097120)  // 65535 blocks of 32 rows
+  if (M < 0 || M > (1LL << 30))
     return set_error(SP_ERR_INVALID_ARG, "int4 linear: %lld rows", (long long)M);
+  if (sh.nt > kI4Tiles)
+    return set_error(SP_ERR_SHAPE, "int4 linear: more than %d outputs", kI4Tiles * 32);
   if (x_dtype != SP_F16 && x_dtype != SP_BF16 && x_dtype != SP_E4M3)
     return set_error(SP_ERR_DTYPE, "int4 linear: x is f16, bf16 or e4m3");
   if (M != 0 && (x_dtype == SP_E4M3) != (x_scale != nullptr))
@@ -583,23 +803,38 @@ extern "C" int sp_int4_linear(const void* x, int64_t x_row_stride, int x_dtype,
   if (x_row_stride < K) return set_error(SP_ERR_SHAPE, "int4 linear: x rows overlap");
   const int64_t xa = x_dtype == SP_E4M3 ? 8 : 16;
   if (!aligned(x, xa) || x_row_stride % 8 || !aligned(q_packed, 16) || !aligned(s_packed, 16) ||
-      !aligned(z_packed, 16))
+      !aligned(z_packed, 16) || !aligned(workspace, 16))
     return set_error(SP_ERR_ALIGN, "int4 linear: x rows must start on %lld bytes, the packed "
-                     "weights on 16", (long long)xa);
+                     "weights and the workspace on 16", (long long)xa);
   if (M == 0) return SP_OK;
   if (int rc = require_sm100()) return rc;
+  if (!workspace || workspace_bytes < sp_int4_linear_workspace_size(M, N, K, group))
+    return set_error(SP_ERR_WORKSPACE, "int4 linear: workspace missing or too small");
   Int4Args a{};
-  a.x = x, a.x_scale = x_scale, a.x_stride = x_row_stride;
-  a.q = static_cast<const uint4*>(q_packed);
-  a.s = static_cast<const uint16_t*>(s_packed);
+  a.x_stride = x_row_stride;
+  a.q = static_cast<const uint8_t*>(q_packed);
+  a.s = static_cast<const uint8_t*>(s_packed);
   a.z = static_cast<const uint8_t*>(z_packed);
-  a.bias = bias, a.y = y;
-  a.M = (int)M, a.N = (int)N, a.K = (int)K, a.C = (int)sh.c;
-  a.s_bf16 = scale_dtype == SP_BF16;
+  a.bias = bias;
+  a.counters = static_cast<int32_t*>(workspace);
+  a.parts = reinterpret_cast<float*>(a.counters + kI4Tiles);
+  a.N = (int)N, a.K = (int)K, a.C = (int)sh.c;
+  a.x_dtype = x_dtype;
   a.out_dtype = out_dtype;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool sbf = scale_dtype == SP_BF16;
   const int gpc = (int)sh.gpc;
-  if (x_dtype == SP_E4M3) return launch_int4_m<__half, true>(a, gpc, s);
-  if (x_dtype == SP_F16) return launch_int4_m<__half, false>(a, gpc, s);
-  return launch_int4_m<__nv_bfloat16, false>(a, gpc, s);
+  const int64_t xs = x_dtype == SP_E4M3 ? 1 : 2, ys = dtype_size(out_dtype);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  for (int64_t m = 0; m < M; m += 32) {  // 32 rows of x at a time
+    a.x = static_cast<const uint8_t*>(x) + m * x_row_stride * xs;
+    a.x_scale = x_scale ? x_scale + m : nullptr;
+    a.y = static_cast<uint8_t*>(y) + m * N * ys;
+    a.M = (int)(M - m < 32 ? M - m : 32);
+    int rc;
+    if (a.M <= 8) rc = launch_int4_g<1>(a, gpc, sbf, s);
+    else if (a.M <= 16) rc = launch_int4_g<2>(a, gpc, sbf, s);
+    else rc = launch_int4_g<4>(a, gpc, sbf, s);
+    if (rc) return rc;
+  }
+  return SP_OK;
 }

@@ -18,9 +18,10 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._torch import cuda_index, dtype_code, ptr, raw_stream, require_cuda, stream_ptr
+from ._torch import Workspaces, cuda_index, dtype_code, ptr, raw_stream, require_cuda, stream_ptr
 
 _linear = _lib.Entry("sp_int4_linear")
+_workspaces = Workspaces()
 
 _X = {torch.float16: _lib.SP_F16, torch.bfloat16: _lib.SP_BF16,
       torch.float8_e4m3fn: _lib.SP_E4M3}
@@ -54,7 +55,7 @@ class Int4Linear:
         self.out_features, self.in_features, self.group_size = N, K, group_size
         self.scale_dtype = scales.dtype
         self.bias = bias
-        self._bias = {}
+        self._bias, self._work_bytes = {}, {}
         self.q = torch.empty(sizes[0], dtype=torch.uint8, device=dev)
         self.scale = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
         self.zero = None if zeros is None else torch.empty(sizes[2], dtype=torch.uint8, device=dev)
@@ -114,12 +115,16 @@ class Int4Linear:
 
     def forward(self, x: torch.Tensor, x_scale: Optional[torch.Tensor] = None, *,
                 out_dtype: Optional[torch.dtype] = None,
-                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                out: Optional[torch.Tensor] = None,
+                workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
         """[..., in_features] -> [..., out_features].
 
         x bf16 or f16, or float8_e4m3fn with x_scale f32 [...].  The output's type is
-        out_dtype, else out's, else x's (bf16 for e4m3)."""
-        index = cuda_index(x, self.q, x_scale, out)
+        out_dtype, else out's, else x's (bf16 for e4m3).
+
+        The layers share one workspace per stream; a call captured into a graph that is replayed
+        beside other work of its stream needs one of its own (`workspace_size` zero bytes)."""
+        index = cuda_index(x, self.q, x_scale, out, workspace)
         N, K = self.out_features, self.in_features
         xd = _X.get(x.dtype)
         if xd is None:
@@ -157,9 +162,24 @@ class Int4Linear:
         b_ptr = 0
         if self.bias is not None:
             b_ptr = self._bias_as(dt).data_ptr()
+        raw = raw_stream(index)
+        if workspace is None:
+            tile = 8 if M <= 8 else 16 if M <= 16 else 32
+            need = self._work_bytes.get(tile)
+            if need is None:
+                need = self._work_bytes[tile] = max(self.workspace_size(m)
+                                                    for m in range(1, tile + 1))
+            work = _workspaces.get(index, raw, need)
+        else:
+            work = (workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size())
         _linear(p, stride, xd, s_ptr, *self._weight_args, b_ptr, out.data_ptr(), M, N, K,
-                self.group_size, dtype_code(dt), raw_stream(index))
+                self.group_size, dtype_code(dt), work[1], work[2], raw)
         return out
+
+    def workspace_size(self, rows: int) -> int:
+        """Bytes of a workspace (zeros, any dtype) for a call of that many rows."""
+        return _lib.load().sp_int4_linear_workspace_size(rows, self.out_features,
+                                                         self.in_features, self.group_size)
 
     def _bias_as(self, dt: torch.dtype) -> torch.Tensor:
         b = self._bias.get(dt)

@@ -15,24 +15,24 @@ The cache holds bf16 or f16, or e4m3 values times a scale per head.
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, Optional
+from typing import Dict, Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._torch import cuda_index, dtype_code, ptr, raw_stream, require_cuda
+from ._torch import Workspaces, cuda_index, dtype_code, ptr, raw_stream, require_cuda
 
 _append = _lib.Entry("sp_paged_kv_append")
 _attend = _lib.Entry("sp_paged_attention")
+_workspaces = Workspaces()
 _16BIT = {torch.float16: _lib.SP_F16, torch.bfloat16: _lib.SP_BF16}
 
 
 class PagedKVCache:
     """k and v tensors of equal shape; k_scale and v_scale f32 [kv_heads] for e4m3 ones.
 
-    The object keeps the device workspace of `attend`, one per stream that calls it (a call
-    captured into a graph that is replayed on another stream needs a `workspace` of its own:
-    `new_workspace`)."""
+    The calls of `attend` share one device workspace per stream; a call captured into a graph
+    that is replayed beside other work of its stream needs one of its own (`new_workspace`)."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None):
@@ -53,7 +53,7 @@ class PagedKVCache:
             raise TypeError("the cache holds bf16, f16 or float8_e4m3fn")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.page_size, self.kv_heads, self.head_dim = k.shape
-        self._work: Dict[int, torch.Tensor] = {}
+        self._work_bytes: Dict[Tuple[int, int], int] = {}
         self._handle = ctypes.c_void_p()
         _lib.call("sp_paged_cache_create", ptr(k), ptr(v), ptr(k_scale), ptr(v_scale),
                   _lib.i64_array(k.stride()), _lib.i64_array(v.stride()), *k.shape, self._code,
@@ -139,10 +139,14 @@ class PagedKVCache:
                 raw_stream(index))
         return q_out
 
+    def workspace_size(self, batch: int, heads: int) -> int:
+        """Bytes of the workspace of an `attend` call."""
+        return _lib.load().sp_paged_attention_workspace_size(batch, heads, self.kv_heads)
+
     def new_workspace(self, batch: int, heads: int) -> torch.Tensor:
         """A workspace for `attend` calls of up to `batch` sequences and `heads` query heads."""
-        n = _lib.load().sp_paged_attention_workspace_size(batch, heads, self.kv_heads)
-        return torch.zeros((n + 3) // 4, dtype=torch.int32, device=self.device)
+        return torch.zeros((self.workspace_size(batch, heads) + 3) // 4, dtype=torch.int32,
+                           device=self.device)
 
     def attend(self, q: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, *,
                scale: Optional[float] = None, window: Optional[int] = None, sinks: int = 0,
@@ -182,23 +186,16 @@ class PagedKVCache:
         q, q_ptr, q_seq, q_head = _heads(q)
         stream = raw_stream(index)
         if workspace is None:
-            items = B * hkv * ((hq // hkv + 15) >> 4)  # counters of the call
-            workspace, ws_ptr, ws_bytes, most = self._work.get(stream, _NO_WORKSPACE)
-            if items > most:
-                workspace = self.new_workspace(B, hq)
-                ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * 4
-                self._work[stream] = (workspace, ws_ptr, ws_bytes, items)
-        elif not workspace.is_contiguous():
-            raise ValueError("workspace must be contiguous")
+            need = self._work_bytes.get((B, hq))
+            if need is None:
+                need = self._work_bytes[B, hq] = self.workspace_size(B, hq)
+            work = _workspaces.get(index, stream, need)
         else:
-            ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+            work = (workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size())
         _attend(self._handle, q_ptr, q_seq, q_head, table.data_ptr(), cols,
                 max(table.stride(0), cols), seq_lens.data_ptr(), out.data_ptr(), B, hq, window,
-                sinks, scale or 0.0, code, ws_ptr, ws_bytes, stream)
+                sinks, scale or 0.0, code, work[1], work[2], stream)
         return out
-
-
-_NO_WORKSPACE = (None, 0, 0, 0)
 
 
 def _heads(t: torch.Tensor):
