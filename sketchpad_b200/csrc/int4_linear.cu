@@ -43,7 +43,7 @@ constexpr int kI4Warps = 16;
 constexpr int kI4Deep = 3;          // stages of a warp's ring, of a chunk (2 KB) each
 constexpr int kI4Tiles = 1 << 16;   // counters of the workspace: row tiles of a launch
 constexpr int kI4Smem = 226 * 1024; // shared memory of a block (the SM's, but for 1 KB)
-constexpr double kTileCost = 0.5, kSlabCost = 1.0, kWarpTime = 9;  // see int4_plan
+constexpr double kTileCost = 0.5, kSlabCost = 1.0, kWarpTime = 13;  // see int4_plan
 constexpr int kRedRow = 36;         // row of the join: 32 values, 36 apart against bank conflicts
 constexpr int kRedBytes = kI4Warps * 8 * kRedRow * 4;
 
@@ -80,6 +80,14 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// t[0..1] += s a[0..1], one instruction
+__device__ __forceinline__ void fma2(float* t, const float* a, float s) {
+  asm("{ .reg .b64 x, y, z;\n"
+      "mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%0, %1};\n"
+      "fma.rn.f32x2 z, x, y, z;\n mov.b64 {%0, %1}, z; }"
+      : "+f"(t[0]), "+f"(t[1]) : "f"(a[0]), "f"(a[1]), "f"(s));
+}
+
 // BYTES of shared memory as words.  Plain loads: the compiler moves them ahead of their use.
 template <int BYTES>
 __device__ __forceinline__ void lds(uint32_t (&r)[BYTES / 4], const uint8_t* p) {
@@ -118,7 +126,7 @@ __device__ __forceinline__ uint32_t row_exponent(uint32_t amax_bits) {
 
 // How a block's warps go over mrows rows of `groups` 16-byte groups of 8 inputs: `parts` warps
 // to a row, each lane every (32 parts)-th group, kXBatch loads at a time.
-constexpr int kXBatch = 8;
+constexpr int kXBatch = 12;
 struct XWalk {
   int row, rows, first, step;
   __device__ __forceinline__ XWalk(int mrows) {
@@ -291,8 +299,9 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int
   const int tile0 = blockIdx.x / a.S + group * slab_blocks;
   const int tile_step = slab_blocks * (kI4Warps / U);
   const uint32_t ring = smem_u32(smem) + warp * R::WARP;
-  float* xsum = reinterpret_cast<float*>(smem + R::BLOCK);  // [cs, GPC, TM]
-  uint8_t* xsm = smem + R::BLOCK + cs * GPC * TM * 4;
+  // the groups' sums of x, [cs, GPC, TM / 2, 4]: two rows' sums twice, an accumulator's layout
+  float* xsum = reinterpret_cast<float*>(smem + R::BLOCK);
+  uint8_t* xsm = smem + R::BLOCK + cs * GPC * TM * 8;
 
   // ---- the copy side: the next chunk to copy
   int ft = tile0, fc = gw;
@@ -358,8 +367,8 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int
         else mma_f16(acc, ones, b[0], b[1], acc);
         mma_f16(acc, ones, b[2], b[3], acc);
         if (j % JPG == JPG - 1 && g == 0)
-          *reinterpret_cast<float2*>(xsum + (i * GPC + j / JPG) * TM + n * 8 + t4 * 2) =
-              make_float2(acc[0] * unit, acc[1] * unit);
+          *reinterpret_cast<float4*>(xsum + ((i * GPC + j / JPG) * TM + n * 8 + t4 * 2) * 2) =
+              make_float4(acc[0] * unit, acc[1] * unit, acc[0] * unit, acc[1] * unit);
       }
     }
   }
@@ -375,7 +384,7 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) tot[rt][n][e] = 0.f;
-    const uint8_t* xs = reinterpret_cast<const uint8_t*>(xsum) + t4 * 8 + gw * (GPC * TM * 4);
+    const uint8_t* xs = reinterpret_cast<const uint8_t*>(xsum) + t4 * 16 + gw * (GPC * TM * 8);
     uint32_t xo = gw * 256;
 
     for (int c = gw; c < cs; c += U) {
@@ -408,13 +417,13 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            uint32_t v[2];
-            lds<8>(v, xs + (grp * TM + n * 8) * 4);
+            uint32_t v[4];
+            lds<16>(v, xs + (grp * TM + n * 8) * 8);
 #pragma unroll
             for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                c0[rt][n][e] = __uint_as_float(v[e & 1]);
+                c0[rt][n][e] = __uint_as_float(v[e]);
                 if constexpr (ZP) c0[rt][n][e] *= z[rt * 2 + (e >> 1)];
               }
           }
@@ -453,14 +462,11 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int
             }
             const int rt = r >> 1, h = (r & 1) * 2;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              tot[rt][n][h] += sc * acc[rt][n][h];
-              tot[rt][n][h + 1] += sc * acc[rt][n][h + 1];
-            }
+            for (int n = 0; n < NT; ++n) fma2(&tot[rt][n][h], &acc[rt][n][h], sc);
           }
         }
       }
-      xs += U * (GPC * TM * 4);
+      xs += U * (GPC * TM * 8);
       xo += U * 256;
     }
 
@@ -518,27 +524,27 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int
       }
       group_sync(group, U);
       if (last_flag[group]) {
-        if (U == 1) {
+        // float4 o of the tile: in the MMA's layout, or four outputs of a row of x
+        for (int o = gt; o < NT * 64; o += own) {
+          float v[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int k0 = 0; k0 < a.S; k0 += 8) {
+            float4 p[8];
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+            for (int k = 0; k < 8; ++k)
+              p[k] = k0 + k < a.S
+                         ? __ldcg(reinterpret_cast<const float4*>(parts + (k0 + k) * (NT * 256)) + o)
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-              float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-              for (int k = 0; k < a.S; ++k) {
-                const float4 p = __ldcg(reinterpret_cast<const float4*>(parts + k * (NT * 256)) +
-                                        (n * 2 + rt) * 32 + lane);
-                v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
-              }
-              store_frag(a, v, n * 8 + t4 * 2, tile * 32 + rt * 16 + g, mrows);
-            }
-        } else {
-          for (int o = gt; o < NT * 256; o += own) {
-            const int m = o >> 5, row = tile * 32 + (o & 31);
-            float v = 0.f;
-#pragma unroll 4
-            for (int k = 0; k < a.S; ++k) v += __ldcg(parts + k * (NT * 256) + o);
-            if (m < mrows && row < a.N) store_y(a, m, row, v);
+            for (int k = 0; k < 8; ++k)
+              v[0] += p[k].x, v[1] += p[k].y, v[2] += p[k].z, v[3] += p[k].w;
+          }
+          if (U == 1) {
+            store_frag(a, v, (o >> 6) * 8 + t4 * 2, tile * 32 + (o >> 5 & 1) * 16 + g, mrows);
+          } else {
+            const int m = o >> 3, row = tile * 32 + (o & 7) * 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (m < mrows && row + e < a.N) store_y(a, m, row + e, v[e]);
           }
         }
       }
@@ -628,7 +634,7 @@ struct Int4Plan {
 Int4Plan int4_plan(int64_t M, int64_t N, int64_t C, int gpc, int ring_bytes) {
   const int NT = M <= 8 ? 1 : M <= 16 ? 2 : 4;
   const int64_t tokens = M < 8 * NT ? M : 8 * NT, n_tiles = (N + 31) / 32;
-  const int64_t per_chunk = tokens * 256 + gpc * 8 * NT * 4;
+  const int64_t per_chunk = tokens * 256 + gpc * 8 * NT * 8;
   const int64_t fixed = 1024 + kRedBytes + ring_bytes + tokens * 64;
   const int64_t sms = num_sms(), fit = (kI4Smem - fixed) / per_chunk;
   const int64_t s_min = (C + fit - 1) / fit, s_max = s_min < 8 ? 16 : 2 * s_min;
