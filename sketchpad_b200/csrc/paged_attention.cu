@@ -13,10 +13,10 @@
 //
 // Inside a block the four warps work alone: each has its own ring of key / value tiles that it
 // fills with asynchronous 16-byte copies (the only loads of the kernel that wait on HBM), its
-// own running maximum, sum and output in registers, and no barrier until the part's end.  The
-// query heads of a cache head are the 16 rows of the warp's m16n8k16 MMAs (rows beyond hq / hkv
-// are zeros: the MMAs are far from the bound).  Positions are counted over visible tokens only,
-// so a window costs no masked work.
+// own running maximum, sum and output in registers, and no barrier until an item's end.  The
+// copies run ahead over the items' ends.  The query heads of a cache head are the 16 rows of
+// the warp's m16n8k16 MMAs (rows beyond hq / hkv are zeros: the MMAs are far from the bound).
+// Positions are counted over visible tokens only, so a window costs no masked work.
 #include <type_traits>
 
 #include "common.cuh"
@@ -27,6 +27,7 @@ namespace sp {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kMinSteps = 4;  // steps of a block's share at least: fewer parts to join
 
 struct AttnArgs {
   PagedCache c;
@@ -34,6 +35,7 @@ struct AttnArgs {
   void* out;
   const int32_t* lens;
   int64_t q_seq, q_head;  // strides, elements
+  uint32_t k_page, k_slot, k_head, v_page, v_slot, v_head;  // strides, 16 bytes
   int32_t B, hq, hkv, D;
   int32_t group;       // hq / hkv
   int32_t row_blocks;  // ceil(group / 16)
@@ -125,71 +127,81 @@ struct Geo {
   static constexpr int ROW = DP * ES;          // bytes
   static constexpr int CHUNKS = ROW / 16;
   static constexpr int TILE = TOK * ROW;       // k or v
-  static constexpr int STAGES = DP > 128 ? 3 : DP > 64 ? 3 : 4;
+  static constexpr int STAGES = DP > 64 ? 3 : 4;
   static constexpr int RING = STAGES * 2 * TILE;  // per warp
   static constexpr int STEP = kWarps * TOK;       // tokens per block step
-  static constexpr int PART = 16 * (DP + 2);      // floats per warp when the block joins
-  static constexpr int SMEM = kWarps * RING > kWarps * PART * 4 ? kWarps * RING : kWarps * PART * 4;
+  static constexpr int JOIN = kWarps * 8 * DP * 4;  // the warps' outputs, eight rows at a time
+  static constexpr int SMEM = kWarps * RING + JOIN;
+  static constexpr int PER_SM = DP > 128 ? 1 : DP > 64 ? 2 : 3;  // blocks
   static constexpr uint32_t KEY = CHUNKS >= 8 ? 7 : CHUNKS - 1;
   __device__ static uint32_t at(int row, int chunk) {
     return (uint32_t)(row * ROW + ((chunk ^ (row & KEY)) << 4));
   }
 };
 
+// A place in the list of steps: step `step` of `steps` of cache head hk, row block rb, of
+// sequence b.
+struct Cursor {
+  int b, hk, rb, step, steps;
+  Visible vis;
+};
+
 template <typename T, bool E4M3, int DP>
-__global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, Geo<T, E4M3, DP>::PER_SM)
+    paged_attn_kernel(const AttnArgs a) {
   using G = Geo<T, E4M3, DP>;
   using MT = std::conditional_t<E4M3, __half, T>;  // MMA type
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t scan_slots[kWarps + 1];
+  __shared__ int64_t scan_slots[kWarps];
   __shared__ int32_t find_seq;
   __shared__ int64_t find_unit;
   __shared__ int last_flag;
   __shared__ float join_m[kWarps][16], join_l[kWarps][16];
+  __shared__ uint32_t seen[kWarps][G::STAGES];  // bit r: row r of the stage's tile is visible
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   const int nblk = gridDim.x;
   const int items_per_seq = a.hkv * a.row_blocks;
   const int64_t capacity = (int64_t)a.c.table_cols * a.c.page_size.d;
-  auto steps_of = [&](int b) -> int64_t {
-    return (visible_of(a, b, capacity).count + G::STEP - 1) / G::STEP;
-  };
+  auto steps_of = [&](const Visible& v) { return (v.count + G::STEP - 1) / G::STEP; };
 
-  // sequences that show nothing come out as zeros
+  // ---- the number of steps; sequences that show nothing come out as zeros
+  int64_t mine = 0;
+  for (int b = tid; b < a.B; b += kWarps * 32) mine += steps_of(visible_of(a, b, capacity));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) scan_slots[warp] = mine;
   for (int b = blockIdx.x; b < a.B; b += nblk)
     if (visible_of(a, b, capacity).count == 0) {
       T* o = static_cast<T*>(a.out) + (int64_t)b * a.hq * a.D;
       for (int i = tid * 8; i < a.hq * a.D; i += kWarps * 32 * 8)
         *reinterpret_cast<uint4*>(o + i) = make_uint4(0, 0, 0, 0);
     }
-
-  // ---- this block's share [unit, unit_end) of the list of steps
-  int64_t mine = 0;
-  for (int b = tid; b < a.B; b += kWarps * 32) mine += steps_of(b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) scan_slots[warp] = mine;
   __syncthreads();
   int64_t total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) total += scan_slots[w];
   total *= items_per_seq;
   if (total == 0) return;
-  const int64_t users = min((int64_t)nblk, total);  // blocks with work
+
+  // ---- this block's share [unit, unit_end) of the list
+  const int64_t users = min((int64_t)nblk, (total + kMinSteps - 1) / kMinSteps);
   if (blockIdx.x >= users) return;
   auto share_start = [&](int64_t c) { return total * c / users; };
   auto block_of = [&](int64_t u) { return ((u + 1) * users - 1) / total; };
-  int64_t unit = share_start(blockIdx.x);
-  const int64_t unit_end = share_start(blockIdx.x + 1);
+  const int64_t unit0 = share_start(blockIdx.x);
+  const int n_steps = (int)(share_start(blockIdx.x + 1) - unit0);
 
-  // ---- the sequence that holds `unit`: scan the lengths a block's width at a time
-  int64_t seq_unit = 0;  // first unit of sequence `b`
-  int b = 0;
+  // ---- the sequence that holds unit0: scan the lengths a block's width at a time
+  int64_t seq_unit = 0;  // first unit of the sequence
+  Cursor cc{};           // where the computation is
   {
     int64_t before = 0;
     for (int base = 0; base < a.B; base += kWarps * 32) {
-      const int64_t n = base + tid < a.B ? steps_of(base + tid) * items_per_seq : 0;
+      const int64_t n =
+          base + tid < a.B ? (int64_t)steps_of(visible_of(a, base + tid, capacity)) * items_per_seq
+                           : 0;
       int64_t inc = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -207,43 +219,128 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const AttnArgs 
         chunk += scan_slots[w];
       }
       const int64_t lo = off + inc - n;
-      if (unit >= lo && unit < lo + n) {
+      if (unit0 >= lo && unit0 < lo + n) {
         find_seq = base + tid;
         find_unit = lo;
       }
       __syncthreads();
       if (find_seq >= 0) {
-        b = find_seq;
+        cc.b = find_seq;
         seq_unit = find_unit;
         break;
       }
       before += chunk;
     }
+    cc.vis = visible_of(a, cc.b, capacity);
+    cc.steps = steps_of(cc.vis);
+    const int rel = (int)((unit0 - seq_unit) / cc.steps);  // head-major within the sequence
+    cc.step = (int)(unit0 - seq_unit - (int64_t)rel * cc.steps);
+    cc.hk = rel / a.row_blocks;
+    cc.rb = rel - cc.hk * a.row_blocks;
   }
+  // To the next step of the list (only while one is left).  True at an item's end.
+  auto advance = [&](Cursor& c) {
+    if (++c.step < c.steps) return false;
+    c.step = 0;
+    if (++c.rb == a.row_blocks) {
+      c.rb = 0;
+      if (++c.hk == a.hkv) {
+        c.hk = 0;
+        do {
+          ++c.b;
+          if (c.b >= a.B) break;
+          c.vis = visible_of(a, c.b, capacity);
+          c.steps = steps_of(c.vis);
+        } while (c.steps == 0);
+      }
+    }
+    return true;
+  };
 
+  // ---- the copy side of the ring: the lane's rows of a tile, their pages read one step ahead
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * G::RING;
   const int lr = lane >> 2, lc = lane & 3;  // copy: row lr + 8 i, chunks lc + 4 i
   const int chunks = a.D * G::ES / 16;      // live chunks of a row
-
-  while (unit < unit_end) {
-    const Visible vis = visible_of(a, b, capacity);
-    const int64_t steps = (vis.count + G::STEP - 1) / G::STEP;
-    if (steps == 0) {
-      ++b;
-      continue;
+  constexpr int RPL = G::TOK / 8;           // rows per lane
+  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k);
+  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v);
+  Cursor lk = cc;
+  int looked = 0, lk_head = 0;
+  int32_t page[RPL], slot[RPL];
+  auto lookup = [&]() {
+    if (looked < n_steps) {
+      lk_head = lk.hk;
+      const int32_t* row = a.c.table + lk.b * a.c.table_stride;
+#pragma unroll
+      for (int i = 0; i < RPL; ++i) {
+        page[i] = -1;
+        const int32_t v = lk.step * G::STEP + warp * G::TOK + lr + 8 * i;
+        if (v < lk.vis.count) {
+          const int32_t tok = v < lk.vis.head ? v : v + lk.vis.skip;
+          const int32_t col = a.c.page_size.div(tok);
+          slot[i] = tok - col * a.c.page_size.d;
+          page[i] = __ldg(row + col);
+        }
+      }
+      advance(lk);
     }
-    const int item = (int)((unit - seq_unit) / steps);  // head-major within the sequence
-    const int64_t item_unit = seq_unit + item * steps;
-    const int64_t stop = min(unit_end, item_unit + steps);
-    const int hk = item / a.row_blocks, rb = item % a.row_blocks;
-    const int rows = min(16, a.group - rb * 16);
-    const int head0 = hk * a.group + rb * 16;
+    ++looked;
+  };
+  auto fill = [&](int stage) {
+    const uint32_t kt = ring + stage * (2 * G::TILE), vt = kt + G::TILE;
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < RPL; ++i) {
+      const bool live = (uint32_t)page[i] < (uint32_t)a.c.pages;
+      const int row = lr + 8 * i;
+      // one bit per row out of the four equal ones of its lanes
+      uint32_t x = __ballot_sync(0xffffffffu, live) & 0x11111111u;
+      x = (x | x >> 3) & 0x03030303u;
+      x = (x | x >> 6) & 0x000f000fu;
+      x = (x | x >> 12) & 0xffu;
+      bits |= x << (8 * i);
+      const uint8_t* ks = kb;
+      const uint8_t* vs = vb;
+      if (live) {
+        ks += ((uint64_t)(uint32_t)page[i] * a.k_page +
+               (uint32_t)(slot[i] * a.k_slot + lk_head * a.k_head)) << 4;
+        vs += ((uint64_t)(uint32_t)page[i] * a.v_page +
+               (uint32_t)(slot[i] * a.v_slot + lk_head * a.v_head)) << 4;
+      }
+#pragma unroll
+      for (int c = 0; c < G::CHUNKS; c += 4) {
+        const bool on = live && c + lc < chunks;
+        cp16(kt + G::at(row, c + lc), ks + (on ? (c + lc) * 16 : 0), on);
+      }
+#pragma unroll
+      for (int c = 0; c < G::CHUNKS; c += 4) {
+        const bool on = live && c + lc < chunks;
+        cp16(vt + G::at(row, c + lc), vs + (on ? (c + lc) * 16 : 0), on);
+      }
+    }
+    if (lane == 0) seen[warp][stage] = bits;
+  };
 
-    // ---- q: the 16 rows of the A operand, from global memory straight into fragments
-    uint32_t qf[DP / 16][4];
-    float rscale[2] = {a.scale_log2, a.scale_log2};
-    {
-      const T* q0 = static_cast<const T*>(a.q) + b * a.q_seq + head0 * a.q_head;
+  lookup();
+#pragma unroll
+  for (int s = 0; s < G::STAGES - 1; ++s) {
+    if (s < n_steps) fill(s);
+    lookup();
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  uint32_t qf[DP / 16][4];
+  float rscale[2], m[2], l[2], o[DP / 8][4];
+  int64_t item_unit = unit0 - cc.step;  // the item's first unit
+  bool fresh = true;
+  int stage = 0, refill = G::STAGES - 1;
+  for (int s = 0; s < n_steps; ++s) {
+    const int rows = min(16, a.group - cc.rb * 16);
+    const int head0 = cc.hk * a.group + cc.rb * 16;
+    if (fresh) {
+      // ---- a new item: q, the 16 rows of the A operand, from global memory into fragments
+      fresh = false;
+      const T* q0 = static_cast<const T*>(a.q) + cc.b * a.q_seq + head0 * a.q_head;
       float qmax[2] = {0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < DP / 16; ++ks)
@@ -269,6 +366,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const AttnArgs 
             qmax[i & 1] = fmaxf(qmax[i & 1], fmaxf(fabsf(to_f32(e[0])), fabsf(to_f32(e[1]))));
           }
         }
+      rscale[0] = rscale[1] = a.scale_log2;
       if constexpr (E4M3) {
         // q in f16, each row scaled by a power of two so that its largest value is in [1, 2):
         // exact but for values below 2^-24 of that, and bf16's range fits
@@ -283,7 +381,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const AttnArgs 
           const uint32_t e = (__float_as_uint(qmax[r]) >> 23) & 0xff;
           const bool plain = e >= 1 && e <= 252;
           mul[r] = plain ? __uint_as_float((254 - e) << 23) : 1.f;
-          rscale[r] *= a.c.k_scale[hk] * (plain ? __uint_as_float(e << 23) : 1.f);
+          rscale[r] *= a.c.k_scale[cc.hk] * (plain ? __uint_as_float(e << 23) : 1.f);
         }
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks)
@@ -293,331 +391,261 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attn_kernel(const AttnArgs 
             qf[ks][i] = pack2<__half>(to_f32(e[0]) * mul[i & 1], to_f32(e[1]) * mul[i & 1]);
           }
       }
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
     }
 
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    float o[DP / 8][4];
-#pragma unroll
-    for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+    asm volatile("cp.async.wait_group %0;" ::"n"(G::STAGES - 2) : "memory");
+    __syncwarp();
+    // refill the stage that the previous step has read
+    if (s + G::STAGES - 1 < n_steps) fill(refill);
+    lookup();
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    const uint32_t kt = ring + stage * (2 * G::TILE), vt = kt + G::TILE;
+    const uint32_t bits = seen[warp][stage];
+    refill = stage;
+    stage = stage + 1 == G::STAGES ? 0 : stage + 1;
 
-    // ---- the copy side of the ring: the lane's rows of tile s, their pages read one tile ahead
-    constexpr int RPL = G::TOK / 8;  // rows per lane
-    const int n_steps = (int)(stop - unit);
-    const int step0 = (int)(unit - item_unit);
-    int32_t page[RPL], slot[RPL];
-    auto lookup = [&](int s) {
+    // ---- scores of 16 rows x TOK tokens
+    float sc[G::TOK / 8][4];
 #pragma unroll
-      for (int i = 0; i < RPL; ++i) {
-        page[i] = -1;
-        const int32_t v = (step0 + s) * G::STEP + warp * G::TOK + lr + 8 * i;
-        if (s < n_steps && v < vis.count) {
-          const int32_t tok = v < vis.head ? v : v + vis.skip;
-          const int32_t col = a.c.page_size.div(tok);
-          slot[i] = tok - col * a.c.page_size.d;
-          const int32_t p = __ldg(a.c.table + b * a.c.table_stride + col);
-          page[i] = p >= 0 && p < a.c.pages ? p : -1;
+    for (int n = 0; n < G::TOK / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[n][i] = 0.f;
+    if constexpr (E4M3) {
+      constexpr int CPL = G::CHUNKS / 4;
+#pragma unroll
+      for (int n = 0; n < G::TOK / 8; ++n)
+#pragma unroll
+        for (int j = 0; j < CPL; ++j) {
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(kt + G::at(n * 8 + g, t4 * CPL + j)) : "memory");
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            mma16816<MT>(sc[n], qf[j * 4 + i], e4m3x2_to_f16x2(w[i]), e4m3x2_to_f16x2(w[i] >> 16));
         }
-      }
-    };
-    uint32_t seen[G::STAGES];  // bit r: row r of the stage's tile is a visible token
-    auto fill = [&](int stage, uint32_t& bits) {
-      const uint32_t kt = ring + stage * 2 * G::TILE, vt = kt + G::TILE;
-      const uint8_t* kb = static_cast<const uint8_t*>(a.c.k);
-      const uint8_t* vb = static_cast<const uint8_t*>(a.c.v);
-      bits = 0;
+    } else {
 #pragma unroll
-      for (int i = 0; i < RPL; ++i) {
-        const bool live = page[i] >= 0;
-        const int row = lr + 8 * i;
-        const uint32_t ball = __ballot_sync(0xffffffffu, live);
-        // one bit per row out of the four equal ones of its lanes
-        uint32_t x = ball & 0x11111111u;
-        x = (x | x >> 3) & 0x03030303u;
-        x = (x | x >> 6) & 0x000f000fu;
-        x = (x | x >> 12) & 0xffu;
-        bits |= x << (8 * i);
-        const uint8_t* ks = kb;
-        const uint8_t* vs = vb;
-        if (live) {
-          ks += (page[i] * a.c.k_page + slot[i] * a.c.k_slot + hk * a.c.k_head) * G::ES;
-          vs += (page[i] * a.c.v_page + slot[i] * a.c.v_slot + hk * a.c.v_head) * G::ES;
-        }
-#pragma unroll
-        for (int c = 0; c < G::CHUNKS; c += 4) {
-          const bool on = live && c + lc < chunks;
-          cp16(kt + G::at(row, c + lc), on ? ks + (c + lc) * 16 : kb, on);
-        }
-#pragma unroll
-        for (int c = 0; c < G::CHUNKS; c += 4) {
-          const bool on = live && c + lc < chunks;
-          cp16(vt + G::at(row, c + lc), on ? vs + (c + lc) * 16 : vb, on);
-        }
-      }
-    };
-
-    lookup(0);
-#pragma unroll
-    for (int s = 0; s < G::STAGES - 1; ++s) {
-      if (s < n_steps) fill(s, seen[s]);
-      lookup(s + 1);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-
-    for (int s0 = 0; s0 < n_steps; s0 += G::STAGES) {
-#pragma unroll
-      for (int sub = 0; sub < G::STAGES; ++sub) {
-        const int s = s0 + sub;
-        if (s >= n_steps) break;
-        asm volatile("cp.async.wait_group %0;" ::"n"(G::STAGES - 2) : "memory");
-        __syncwarp();
-        constexpr int kLast = G::STAGES - 1;
-        {  // refill the stage that the previous step has read
-          const int st = (sub + kLast) % G::STAGES;
-          if (s + kLast < n_steps) fill(st, seen[st]);
-          lookup(s + kLast + 1);
-          asm volatile("cp.async.commit_group;" ::: "memory");
-        }
-        const uint32_t kt = ring + sub * 2 * G::TILE, vt = kt + G::TILE;
-
-        // ---- scores of 16 rows x TOK tokens
-        float sc[G::TOK / 8][4];
-#pragma unroll
-        for (int n = 0; n < G::TOK / 8; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sc[n][i] = 0.f;
-        if constexpr (E4M3) {
-          constexpr int CPL = G::CHUNKS / 4;
-#pragma unroll
-          for (int n = 0; n < G::TOK / 8; ++n)
-#pragma unroll
-            for (int j = 0; j < CPL; ++j) {
-              uint32_t w[4];
-              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                           : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                           : "r"(kt + G::at(n * 8 + g, t4 * CPL + j)) : "memory");
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                mma16816<MT>(sc[n], qf[j * 4 + i], e4m3x2_to_f16x2(w[i]),
-                             e4m3x2_to_f16x2(w[i] >> 16));
-            }
-        } else {
-#pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks) {
-            uint32_t kf[4];  // tokens 0-7 (k 0-7, 8-15), tokens 8-15 (k 0-7, 8-15)
-            ldsm4(kf, kt + G::at((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
-            mma16816<MT>(sc[0], qf[ks], kf[0], kf[1]);
-            mma16816<MT>(sc[1], qf[ks], kf[2], kf[3]);
-          }
-        }
-
-        // ---- softmax in log2 units; a row that has seen nothing yet keeps m = -inf, l = 0
-        constexpr uint32_t kAll = G::TOK == 32 ? 0xffffffffu : (1u << G::TOK) - 1;
-        const uint32_t bits = seen[sub];
-        float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int n = 0; n < G::TOK / 8; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sc[n][i] *= rscale[i >> 1];
-            if (bits != kAll && !((bits >> (n * 8 + t4 * 2 + (i & 1))) & 1)) sc[n][i] = -INFINITY;
-            mx[i >> 1] = fmaxf(mx[i >> 1], sc[n][i]);
-          }
-        float mref[2];
-        bool grew = false;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-          mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-          grew |= mx[r] > m[r];
-          mx[r] = fmaxf(mx[r], m[r]);
-          mref[r] = mx[r] == -INFINITY ? 0.f : mx[r];
-        }
-        if (__any_sync(0xffffffffu, grew)) {
-          const float al[2] = {exp2_fast(m[0] - mref[0]), exp2_fast(m[1] - mref[1])};
-#pragma unroll
-          for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[n][i] *= al[i >> 1];
-          l[0] *= al[0], l[1] *= al[1];
-        }
-        m[0] = mx[0], m[1] = mx[1];
-#pragma unroll
-        for (int n = 0; n < G::TOK / 8; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sc[n][i] = exp2_fast(sc[n][i] - mref[i >> 1]);
-            l[i >> 1] += sc[n][i];
-          }
-
-        // ---- o += p v
-        if constexpr (E4M3) {
-#pragma unroll
-          for (int h = 0; h < G::TOK / 16; ++h) {
-            const uint32_t pf[4] = {pack2<MT>(sc[2 * h][0], sc[2 * h][1]),
-                                    pack2<MT>(sc[2 * h][2], sc[2 * h][3]),
-                                    pack2<MT>(sc[2 * h + 1][0], sc[2 * h + 1][1]),
-                                    pack2<MT>(sc[2 * h + 1][2], sc[2 * h + 1][3])};
-#pragma unroll
-            for (int blk = 0; blk < DP / 32; ++blk) {
-              // column g of n-tile (blk, j) stands for d = 32 blk + 4 g + j
-              uint32_t w[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int row = h * 16 + t4 * 2 + (i & 1) + (i >> 1) * 8;
-                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i])
-                             : "r"(vt + G::at(row, blk * 2 + (g >> 2)) + (g & 3) * 4) : "memory");
-              }
-              uint32_t f[4][2];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                f[i][0] = e4m3x2_to_f16x2(w[i]);
-                f[i][1] = e4m3x2_to_f16x2(w[i] >> 16);
-              }
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
-                mma16816<MT>(o[blk * 4 + j], pf, __byte_perm(f[0][j >> 1], f[1][j >> 1], sel),
-                             __byte_perm(f[2][j >> 1], f[3][j >> 1], sel));
-              }
-            }
-          }
-        } else {
-          // p rounded to T; for bf16 its rounding error goes through a second MMA, so p counts
-          // with 16 bits and the output is as near as its own type allows
-          uint32_t pf[4], pe[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x = sc[i >> 1][(i & 1) * 2], y = sc[i >> 1][(i & 1) * 2 + 1];
-            pf[i] = pack2<MT>(x, y);
-            if constexpr (!std::is_same_v<MT, __half>) {
-              const T* e = reinterpret_cast<const T*>(&pf[i]);
-              pe[i] = pack2<MT>(x - to_f32(e[0]), y - to_f32(e[1]));
-            }
-          }
-#pragma unroll
-          for (int n = 0; n < DP / 16; ++n) {
-            uint32_t vf[4];  // d 0-7 (tokens 0-7, 8-15), d 8-15 (tokens 0-7, 8-15)
-            ldsm4t(vf, vt + G::at(lane & 15, n * 2 + (lane >> 4)));
-            mma16816<MT>(o[2 * n], pf, vf[0], vf[1]);
-            mma16816<MT>(o[2 * n + 1], pf, vf[2], vf[3]);
-            if constexpr (!std::is_same_v<MT, __half>) {
-              mma16816<MT>(o[2 * n], pe, vf[0], vf[1]);
-              mma16816<MT>(o[2 * n + 1], pe, vf[2], vf[3]);
-            }
-          }
-        }
-        __syncwarp();  // the tile is read: its stage may be refilled
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        uint32_t kf[4];  // tokens 0-7 (k 0-7, 8-15), tokens 8-15 (k 0-7, 8-15)
+        ldsm4(kf, kt + G::at((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
+        mma16816<MT>(sc[0], qf[ks], kf[0], kf[1]);
+        mma16816<MT>(sc[1], qf[ks], kf[2], kf[3]);
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
 
-    // ---- the four warps' results meet in shared memory (the rings are idle now)
+    // ---- softmax in log2 units; a row that has seen nothing yet keeps m = -inf, l = 0
+    constexpr uint32_t kAll = G::TOK == 32 ? 0xffffffffu : (1u << G::TOK) - 1;
+#pragma unroll
+    for (int n = 0; n < G::TOK / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[n][i] *= rscale[i >> 1];
+    if (bits != kAll) {
+#pragma unroll
+      for (int n = 0; n < G::TOK / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!((bits >> (n * 8 + t4 * 2 + (i & 1))) & 1)) sc[n][i] = -INFINITY;
+    }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int n = 0; n < G::TOK / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], sc[n][i]);
+    float mref[2];
+    bool grew = false;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+      grew |= mx[r] > m[r];
+      mx[r] = fmaxf(mx[r], m[r]);
+      mref[r] = mx[r] == -INFINITY ? 0.f : mx[r];
+    }
+    if (__any_sync(0xffffffffu, grew)) {
+      const float al[2] = {exp2_fast(m[0] - mref[0]), exp2_fast(m[1] - mref[1])};
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][i] *= al[i >> 1];
+      l[0] *= al[0], l[1] *= al[1];
+    }
+    m[0] = mx[0], m[1] = mx[1];
+#pragma unroll
+    for (int n = 0; n < G::TOK / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[n][i] = exp2_fast(sc[n][i] - mref[i >> 1]);
+        l[i >> 1] += sc[n][i];
+      }
+
+    // ---- o += p v
+    if constexpr (E4M3) {
+#pragma unroll
+      for (int h = 0; h < G::TOK / 16; ++h) {
+        const uint32_t pf[4] = {pack2<MT>(sc[2 * h][0], sc[2 * h][1]),
+                                pack2<MT>(sc[2 * h][2], sc[2 * h][3]),
+                                pack2<MT>(sc[2 * h + 1][0], sc[2 * h + 1][1]),
+                                pack2<MT>(sc[2 * h + 1][2], sc[2 * h + 1][3])};
+#pragma unroll
+        for (int blk = 0; blk < DP / 32; ++blk) {
+          // column g of n-tile (blk, j) stands for d = 32 blk + 4 g + j
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = h * 16 + t4 * 2 + (i & 1) + (i >> 1) * 8;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i])
+                         : "r"(vt + G::at(row, blk * 2 + (g >> 2)) + (g & 3) * 4) : "memory");
+          }
+          uint32_t f[4][2];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f[i][0] = e4m3x2_to_f16x2(w[i]);
+            f[i][1] = e4m3x2_to_f16x2(w[i] >> 16);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
+            mma16816<MT>(o[blk * 4 + j], pf, __byte_perm(f[0][j >> 1], f[1][j >> 1], sel),
+                         __byte_perm(f[2][j >> 1], f[3][j >> 1], sel));
+          }
+        }
+      }
+    } else {
+      // p rounded to T; for bf16 its rounding error goes through a second MMA, so p counts
+      // with 16 bits and the output is as near as its own type allows
+      uint32_t pf[4], pe[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = sc[i >> 1][(i & 1) * 2], y = sc[i >> 1][(i & 1) * 2 + 1];
+        pf[i] = pack2<MT>(x, y);
+        if constexpr (!std::is_same_v<MT, __half>) {
+          const T* e = reinterpret_cast<const T*>(&pf[i]);
+          pe[i] = pack2<MT>(x - to_f32(e[0]), y - to_f32(e[1]));
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < DP / 16; ++n) {
+        uint32_t vf[4];  // d 0-7 (tokens 0-7, 8-15), d 8-15 (tokens 0-7, 8-15)
+        ldsm4t(vf, vt + G::at(lane & 15, n * 2 + (lane >> 4)));
+        mma16816<MT>(o[2 * n], pf, vf[0], vf[1]);
+        mma16816<MT>(o[2 * n + 1], pf, vf[2], vf[3]);
+        if constexpr (!std::is_same_v<MT, __half>) {
+          mma16816<MT>(o[2 * n], pe, vf[0], vf[1]);
+          mma16816<MT>(o[2 * n + 1], pe, vf[2], vf[3]);
+        }
+      }
+    }
+
+    // ---- the item's end, or the share's
+    const Cursor at = cc;
+    const bool item_end = advance(cc);
+    if (!item_end && s + 1 < n_steps) continue;
+    fresh = true;
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
-    __syncthreads();
-    float* wo = reinterpret_cast<float*>(smem) + warp * 16 * DP;
-#pragma unroll
-    for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = g + (i >> 1) * 8;
-        const int d = E4M3 ? (n >> 2) * 32 + (t4 * 2 + (i & 1)) * 4 + (n & 3)
-                           : n * 8 + t4 * 2 + (i & 1);
-        if (row < rows) wo[row * DP + d] = o[n][i];
-      }
     if (t4 == 0) {
       join_m[warp][g] = m[0], join_m[warp][g + 8] = m[1];
       join_l[warp][g] = l[0], join_l[warp][g + 8] = l[1];
     }
-    __syncthreads();
-
-    const int64_t c0 = block_of(item_unit), c1 = block_of(item_unit + steps - 1);
-    const float vscale = E4M3 ? a.c.v_scale[hk] : 1.f;
-    T* outp = static_cast<T*>(a.out) + ((int64_t)b * a.hq + head0) * a.D;
+    const int64_t c0 = block_of(item_unit), c1 = block_of(item_unit + at.steps - 1);
     const bool whole = c0 == c1;
+    const float vscale = E4M3 ? a.c.v_scale[at.hk] : 1.f;
+    T* outp = static_cast<T*>(a.out) + ((int64_t)at.b * a.hq + head0) * a.D;
     const int64_t part_floats = 16 * (int64_t)(a.D + 2);
-    float* part = a.parts + (2 * (int64_t)blockIdx.x + (unit == item_unit ? 1 : 0)) * part_floats;
+    // an item that starts in this share leaves its part in the block's second slot
+    float* part = a.parts + (2 * (int64_t)blockIdx.x + (item_unit >= unit0 ? 1 : 0)) * part_floats;
     const int vecs = a.D >> 2;
-    for (int i = tid; i < rows * vecs; i += kWarps * 32) {
-      const int row = i / vecs, d = (i % vecs) * 4;
-      float mm = -INFINITY;
+    float* jo = reinterpret_cast<float*>(smem + kWarps * G::RING);
+    // the four warps' outputs meet in shared memory, eight rows at a time
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, join_m[w][row]);
-      const float mr = mm == -INFINITY ? 0.f : mm;
-      float ll = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int half = 0; half < 2; ++half) {
+      if (half == 1 && rows <= 8) break;
+      if (half == 1) __syncthreads();  // the first eight are read
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = exp2_fast(join_m[w][row] - mr);
-        ll += f * join_l[w][row];
-        const float4 v = *reinterpret_cast<const float4*>(
-            reinterpret_cast<float*>(smem) + (w * 16 + row) * DP + d);
-        acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
-      }
-      if (whole) {
-        const float inv = ll == 0.f ? 0.f : vscale / ll;
-        uint2 pk = make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv),
-                              pack2<T>(acc[2] * inv, acc[3] * inv));
-        *reinterpret_cast<uint2*>(outp + row * a.D + d) = pk;
-      } else {
-        *reinterpret_cast<float4*>(part + 32 + row * a.D + d) =
-            make_float4(acc[0], acc[1], acc[2], acc[3]);
-        if (d == 0) part[row] = mm, part[16 + row] = ll;
+      for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int d = E4M3 ? (n >> 2) * 32 + (t4 * 2 + i) * 4 + (n & 3) : n * 8 + t4 * 2 + i;
+          jo[(warp * 8 + g) * DP + d] = o[n][half * 2 + i];
+        }
+      __syncthreads();
+      const int half_rows = min(8, rows - half * 8);
+      for (int i = tid; i < half_rows * vecs; i += kWarps * 32) {
+        const int r = i / vecs, d = (i - r * vecs) * 4, row = half * 8 + r;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, join_m[w][row]);
+        const float mr = mm == -INFINITY ? 0.f : mm;
+        float ll = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = exp2_fast(join_m[w][row] - mr);
+          ll += f * join_l[w][row];
+          const float4 v = *reinterpret_cast<const float4*>(jo + (w * 8 + r) * DP + d);
+          acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
+        }
+        if (whole) {
+          const float inv = ll == 0.f ? 0.f : vscale / ll;
+          *reinterpret_cast<uint2*>(outp + row * a.D + d) = make_uint2(
+              pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
+        } else {
+          __stcg(reinterpret_cast<float4*>(part + 32 + row * a.D + d),
+                 make_float4(acc[0], acc[1], acc[2], acc[3]));
+          if (d == 0) __stcg(part + row, mm), __stcg(part + 16 + row, ll);
+        }
       }
     }
+    __syncthreads();  // shared memory is free again; the part's stores are ordered before ...
     if (!whole) {
-      __threadfence();
-      __syncthreads();
-      const int item_id = b * items_per_seq + item;
-      if (tid == 0) {
+      const int item_id = at.b * items_per_seq + at.hk * a.row_blocks + at.rb;
+      if (tid == 0) {  // ... this release
         const int n_parts = (int)(c1 - c0 + 1);
-        const int before = atomicAdd(a.counters + item_id, 1);
+        int before;
+        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;"
+                     : "=r"(before) : "l"(a.counters + item_id) : "memory");
         last_flag = before == n_parts - 1;
         if (last_flag) a.counters[item_id] = 0;  // zero again for the next call
       }
       __syncthreads();
       if (last_flag) {
-        __threadfence();
+        // the item starts in c0's second slot and goes on in the others' first
+        const float* p0 = a.parts + (2 * c0 + 1) * part_floats;
+        const int n_parts = (int)(c1 - c0 + 1);
+        auto part_at = [&](int k) { return p0 + (k == 0 ? 0 : (2 * (int64_t)k - 1) * part_floats); };
         for (int i = tid; i < rows * vecs; i += kWarps * 32) {
-          const int row = i / vecs, d = (i % vecs) * 4;
-          float mm = -INFINITY, ll = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int64_t c = c0; c <= c1; ++c) {
-            // the item starts in c0's second slot and goes on in the others' first
-            const float* p = a.parts + (2 * c + (c == c0 ? 1 : 0)) * part_floats;
-            const float pm = __ldcg(p + row), pl = __ldcg(p + 16 + row);
+          const int row = i / vecs, d = (i - row * vecs) * 4;
+          float mm = -INFINITY;
+#pragma unroll 8
+          for (int k = 0; k < n_parts; ++k) mm = fmaxf(mm, __ldcg(part_at(k) + row));
+          const float mr = mm == -INFINITY ? 0.f : mm;
+          float ll = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+          for (int k = 0; k < n_parts; ++k) {
+            const float* p = part_at(k);
+            const float f = exp2_fast(__ldcg(p + row) - mr);
+            ll += f * __ldcg(p + 16 + row);
             const float4 v = __ldcg(reinterpret_cast<const float4*>(p + 32 + row * a.D + d));
-            const float nm = fmaxf(mm, pm);
-            const float nr = nm == -INFINITY ? 0.f : nm;
-            const float fa = exp2_fast(mm - nr), fb = exp2_fast(pm - nr);
-            ll = ll * fa + pl * fb;
-            acc[0] = acc[0] * fa + v.x * fb, acc[1] = acc[1] * fa + v.y * fb;
-            acc[2] = acc[2] * fa + v.z * fb, acc[3] = acc[3] * fa + v.w * fb;
-            mm = nm;
+            acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
           }
           const float inv = ll == 0.f ? 0.f : vscale / ll;
-          uint2 pk = make_uint2(pack2<T>(acc[0] * inv, acc[1] * inv),
-                                pack2<T>(acc[2] * inv, acc[3] * inv));
-          *reinterpret_cast<uint2*>(outp + row * a.D + d) = pk;
+          *reinterpret_cast<uint2*>(outp + row * a.D + d) = make_uint2(
+              pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
         }
       }
     }
-    __syncthreads();  // shared memory is free for the next part
-    unit = stop;
-    if (unit == seq_unit + steps * items_per_seq) {
-      seq_unit = unit;
-      ++b;
-    }
+    item_unit += at.steps;
   }
-}
-
-// Blocks of the launch: two per SM where their shared memory allows, else one.
-template <typename T, bool E4M3, int DP>
-int attn_blocks() {
-  return num_sms() * (Geo<T, E4M3, DP>::SMEM <= 100 * 1024 ? 2 : 1);
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 template <typename T, bool E4M3, int DP>
@@ -630,7 +658,7 @@ int launch_attn(const AttnArgs& a, cudaStream_t s) {
     return set_error(SP_ERR_LAUNCH, "paged attention: shared memory attribute: %s",
                      cudaGetErrorString(cudaGetLastError()));
   paged_attn_kernel<T, E4M3, DP>
-      <<<attn_blocks<T, E4M3, DP>(), kWarps * 32, G::SMEM, s>>>(a);
+      <<<num_sms() * G::PER_SM, kWarps * 32, G::SMEM, s>>>(a);
   return check_launch("paged attention");
 }
 
@@ -641,10 +669,11 @@ int launch_attn_d(const AttnArgs& a, cudaStream_t s) {
   return launch_attn<T, E4M3, 256>(a, s);
 }
 
-// The workspace: the parts of at most two blocks per SM at the largest head dim, then the
-// counters.  The place of the counters depends on the device alone, so that calls of different
+// The workspace: the parts of the blocks (two slots each) at the largest that blocks per SM and
+// head dim make them, then the counters.  The place of the counters depends on the device alone, so that calls of different
 // sizes can share a workspace without one's parts on another's counters.
-size_t parts_bytes() { return (size_t)num_sms() * 2 * 2 * 16 * (256 + 2) * sizeof(float); }
+size_t parts_bytes() { return (size_t)num_sms() * 2 * 16 * 2 * (128 + 2) * sizeof(float); }
+static_assert(3 * (64 + 2) <= 2 * (128 + 2) && 256 + 2 <= 2 * (128 + 2), "the parts fit");
 }  // namespace
 }  // namespace sp
 
@@ -690,6 +719,17 @@ extern "C" int sp_paged_attention(const void* cache, const void* q, int64_t q_se
     return set_error(SP_ERR_WORKSPACE, "paged attention: workspace missing or too small");
   if (!aligned(workspace, 16))
     return set_error(SP_ERR_ALIGN, "paged attention: workspace must be 16-byte aligned");
+  const int64_t es = h->dtype == SP_E4M3 ? 1 : 2;
+  const int64_t st[6] = {a.c.k_page, a.c.k_slot, a.c.k_head, a.c.v_page, a.c.v_slot, a.c.v_head};
+  uint32_t* to[6] = {&a.k_page, &a.k_slot, &a.k_head, &a.v_page, &a.v_slot, &a.v_head};
+  for (int i = 0; i < 6; ++i) {
+    if (st[i] * es / 16 > 0xffffffffLL)
+      return set_error(SP_ERR_SHAPE, "paged attention: a cache stride beyond 64 GB");
+    *to[i] = (uint32_t)(st[i] * es / 16);
+  }
+  for (int i = 0; i < 6; i += 3)  // a slot's and head's offset within the page
+    if ((h->page_size - 1) * (st[i + 1] * es / 16) + (hkv - 1) * (st[i + 2] * es / 16) > 0xffffffffLL)
+      return set_error(SP_ERR_SHAPE, "paged attention: a page spans more than 64 GB");
   a.q = q, a.out = out;
   a.lens = static_cast<const int32_t*>(seq_lens);
   a.q_seq = q_seq_stride, a.q_head = q_head_stride;
