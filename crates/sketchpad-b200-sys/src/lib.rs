@@ -264,7 +264,7 @@ extern "C" {
         rope_rows: i64, dtype: c_int, stream: *mut c_void
     ) -> c_int;
     pub fn sp_paged_attention_workspace_size(
-        B: i64, hq: i64, hkv: i64
+        hq: i64, hkv: i64, D: i64
     ) -> usize;
     pub fn sp_paged_attention(
         cache: *const c_void, q: *const c_void, q_seq_stride: i64, q_head_stride: i64,

@@ -524,9 +524,9 @@ int sp_paged_kv_append(const void* cache, const void* q, const void* k, const vo
  * or e4m3; block_table has B rows; query head h reads cache head h / (hq / hkv).  scale <= 0
  * selects 1/sqrt(D).
  * workspace: sp_paged_attention_workspace_size() bytes, 16-byte aligned, ZERO before its first
- * use (each call leaves its counters zero again) and not in use by another call in flight;
- * calls of any sizes that fit may share it. */
-size_t sp_paged_attention_workspace_size(int64_t B, int64_t hq, int64_t hkv);
+ * use (each call leaves its counters, the first MB, zero again) and not in use by another call
+ * in flight; calls of any sizes that fit may share it. */
+size_t sp_paged_attention_workspace_size(int64_t hq, int64_t hkv, int64_t D);
 int sp_paged_attention(const void* cache, const void* q, int64_t q_seq_stride,
                        int64_t q_head_stride, const void* block_table, int64_t table_cols,
                        int64_t table_stride, const void* seq_lens, void* out, int64_t B,

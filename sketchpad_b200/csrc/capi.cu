@@ -132,14 +132,14 @@ bool first_time_on_device(unsigned long long* flag_bits) {
 
 int encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, uint32_t rank, const void* base,
                  const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
-                 CUtensorMapSwizzle swizzle) {
+                 CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promotion) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return set_error(SP_ERR_LAUNCH, "cuTensorMapEncodeTiled unavailable from the driver");
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   CUresult r = fn(map, dt, rank, const_cast<void*>(base), reinterpret_cast<const cuuint64_t*>(dims),
                   reinterpret_cast<const cuuint64_t*>(strides_bytes),
                   reinterpret_cast<const cuuint32_t*>(box), estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle, promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return set_error(SP_ERR_ALIGN, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
   return SP_OK;

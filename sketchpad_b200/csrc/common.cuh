@@ -47,7 +47,33 @@ cudaMemPool_t scratch_pool();
 // cuTensorMapEncodeTiled obtained through cudaGetDriverEntryPoint (no libcuda link).
 int encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, uint32_t rank, const void* base,
                  const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
-                 CUtensorMapSwizzle swizzle);
+                 CUtensorMapSwizzle swizzle,
+                 CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+
+// A launch whose blocks may come up while the last blocks of the stream's kernel before it run,
+// where that kernel allows it (programmatic dependent launch).  The kernel has to execute
+// griddepcontrol.wait in every thread before it reads or writes anything that earlier work of
+// the stream touches.
+template <typename... P, typename... A>
+int launch_overlapped(const char* what, void (*kernel)(P...), unsigned blocks, unsigned threads,
+                      size_t smem, cudaStream_t s, A&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return set_error(SP_ERR_LAUNCH, "%s: launch failed: %s", what, cudaGetErrorString(e));
+  }
+  return SP_OK;
+}
 
 // Channels-last GroupNorm (groupnorm_nhwc.cu).
 bool gn_nhwc_applicable(int64_t B, int64_t C, int64_t H, int64_t W, const int64_t* x_strides, int es,

@@ -120,6 +120,31 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendA
   }
 }
 
+// One operand's tensor map.  Rows of 128 bytes are fetched as they are: the next 128 belong to
+// another head.
+bool cache_map(CUtensorMap* map, const void* base, const int64_t strides[4], int64_t pages,
+               int64_t page_size, int64_t hkv, int64_t D, int dtype) {
+  const int64_t es = dtype == SP_E4M3 ? 1 : 2;
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page_size, (uint64_t)hkv, (uint64_t)pages};
+  uint64_t st[3] = {(uint64_t)(strides[1] * es), (uint64_t)(strides[2] * es),
+                    (uint64_t)(strides[0] * es)};
+  const uint32_t box[4] = {(uint32_t)(128 / es), 8, 1, 1};
+  for (int i = 0; i < 3; ++i) {
+    if (st[i] >= 1ull << 40) return false;
+    if (st[i] == 0) {  // a dimension of one entry may have any stride; others must step
+      if (dims[i + 1] > 1) return false;
+      st[i] = 16;
+    }
+  }
+  return encode_tiled(map,
+                      dtype == SP_E4M3  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                      : dtype == SP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                      4, base, dims, st, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                      D * es <= 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B
+                                    : CU_TENSOR_MAP_L2_PROMOTION_L2_256B) == SP_OK;
+}
+
 }  // namespace
 }  // namespace sp
 
@@ -161,6 +186,9 @@ extern "C" int sp_paged_cache_create(void* k, void* v, const float* k_scale, con
   h->c.page_size = make_fast_div((int32_t)page_size);
   h->page_size = page_size;
   h->hkv = (int32_t)hkv, h->D = (int32_t)D, h->dtype = dtype;
+  h->tma = page_size % 8 == 0 && cache_map(&h->kmap, k, k_strides, pages, page_size, hkv, D, dtype) &&
+           cache_map(&h->vmap, v, v_strides, pages, page_size, hkv, D, dtype);
+  clear_error();  // without maps the attention takes its other path
   *cache = h;
   return SP_OK;
 }

@@ -4,30 +4,36 @@
 //   all of the sequence's, or its last `window` and its first `sinks`.
 //
 // Bound by HBM: every visible key and value is read once and meets only the hq / hkv query heads
-// that share it (at most 2 hq/hkv flop per byte of 16-bit cache).  The work is the list of
-// 4-tile steps of every (sequence, cache head) in order; the blocks take equal shares of that
-// list whatever the lengths are, so one long sequence uses the whole GPU and a ragged batch is
-// even.  Shares cut (sequence, head) items: a block leaves such a part's maximum, sum and
-// unnormalised output in the workspace, and the block that arrives last at an item (a counter
-// in the workspace) joins its parts in block order, so results do not depend on timing.
+// that share it (at most 2 hq/hkv flop per byte of 16-bit cache).  The work is the list of steps
+// (a tile per warp) of every (sequence, cache head) in order; the blocks, one per SM, take equal
+// shares of that list whatever the lengths are, so one long sequence uses the whole GPU and a
+// ragged batch is even.  Shares cut (sequence, head) items: a block leaves such a part's
+// maximum, sum and unnormalised output in the workspace, and the block that arrives last at an
+// item (a counter in the workspace) joins its parts in block order, so results do not depend on
+// timing.  (A second kernel for the joins cost 3 to 5 us more than it saved.)
 //
-// Inside a block the four warps work alone: each has its own ring of key / value tiles that it
-// fills with asynchronous 16-byte copies (the only loads of the kernel that wait on HBM), its
-// own running maximum, sum and output in registers, and no barrier until an item's end.  The
-// copies run ahead over the items' ends.  The query heads of a cache head are the 16 rows of
-// the warp's m16n8k16 MMAs (rows beyond hq / hkv are zeros: the MMAs are far from the bound).
-// Positions are counted over visible tokens only, so a window costs no masked work.
+// Inside a block the warps work alone: each has its own ring of key / value tiles in shared
+// memory, its own running maximum, sum and output in registers, and no barrier until an item's
+// end.  The copies run ahead over the items' ends.  A tile is made of granules of 8 tokens from a
+// multiple of 8 on, so where the page size is a multiple of 8 a granule lies in one page and
+// comes by TMA: one lookup and one box of 8 rows x 128 bytes per granule and operand.  (One bulk
+// copy per row measured a copy per 11.5 cycles and SM at best, half of the bandwidth for rows
+// of 128 bytes; 16-byte copies by the lanes cost a third of the warps' instructions.)  Other
+// page sizes take those 16-byte copies.  The query heads of a cache head are the 16 rows of the
+// warp's m16n8k16 MMAs (rows beyond hq / hkv are zeros: the MMAs are far from the bound).
 #include <type_traits>
 
 #include "common.cuh"
 #include "numeric.cuh"
 #include "paged_kv.cuh"
+#include "tc.cuh"
 
 namespace sp {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kMinSteps = 4;  // steps of a block's share at least: fewer parts to join
+constexpr int kMinSteps = 2;    // steps of a block's share at least: fewer parts to join
+constexpr int kLargeSteps = 8;  // wide steps per block from which a call counts as large
+constexpr int kMaxWide = 8;     // warps of a block on different vheads, at most
 
 struct AttnArgs {
   PagedCache c;
@@ -39,17 +45,30 @@ struct AttnArgs {
   int32_t B, hq, hkv, D;
   int32_t group;       // hq / hkv
   int32_t row_blocks;  // ceil(group / 16)
+  int32_t vheads;      // hkv * row_blocks: (cache head, up to 16 of its query heads)
+  int32_t part_rows;   // min(group, 16)
+  int32_t part_floats; // part_rows * (D + 2), rounded up to 16 bytes
+  int32_t heads_wide;  // warps of a block on different vheads at the same tokens, large calls
   int32_t window;      // 0: none
   int32_t sinks;
   float scale_log2;    // scale * log2(e)
-  int32_t* counters;   // [B * hkv * row_blocks], all zero between calls
-  float* parts;        // [2 * grid][16 * (D + 2)]: maxima, sums, rows of D
+  int32_t* counters;   // [items], all zero between calls
+  float* parts;        // [2 * grid, heads_wide][part_floats]: rows of D, then (maximum, sum) of each
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
   const int n = live ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
                : "memory");
+}
+// A box of 8 tokens x 128 bytes of the cache, counted on the mbarrier.
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x,
+                                        int slot, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(bar)
+      : "memory");
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -80,6 +99,15 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// pairs of f32 in one instruction: x * s, x + s
+__device__ __forceinline__ void mul2(float& x, float& y, float s) {
+  asm("{ .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %2};\n"
+      "mul.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a; }" : "+f"(x), "+f"(y) : "f"(s));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float s) {
+  asm("{ .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %2};\n"
+      "add.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a; }" : "+f"(x), "+f"(y) : "f"(s));
+}
 // (lo, hi) packed as two values of T, rounded to nearest
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -98,245 +126,312 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
   return r;
 }
 
-// The visible tokens of a sequence of length n: [0, head) and then [head + skip, n).
+// The visible tokens of a sequence: [0, head) and then [first, n), as granules of 8 tokens from
+// multiples of 8 on: `head_granules`, then those from granule `first / 8` on.  (A granule that
+// both parts reach into comes twice, with its own tokens visible each time.)
 struct Visible {
-  int32_t count, head, skip;
+  int32_t n, head, first, head_granules, granules;
 };
 __device__ __forceinline__ Visible visible_of(const AttnArgs& a, int b, int64_t capacity) {
   int32_t n = a.lens[b];
   if (n > capacity) n = (int32_t)capacity;
   if (n < 0) n = 0;
-  Visible s{n, n, 0};
+  Visible s{n, n, n, (n + 7) >> 3, (n + 7) >> 3};
   if (a.window > 0 && n > a.window) {
-    const int32_t first = n - a.window;
-    s.head = min(a.sinks, first);
-    s.skip = first - s.head;
-    s.count = a.window + s.head;
+    s.first = n - a.window;
+    s.head = min(a.sinks, s.first);
+    s.head_granules = (s.head + 7) >> 3;
+    s.granules = s.head_granules + ((n + 7) >> 3) - (s.first >> 3);
   }
   return s;
 }
+// Granule i: its first token, and a bit per visible token.
+__device__ __forceinline__ int32_t granule(const Visible& v, int32_t i, uint32_t& bits) {
+  const bool in_head = i < v.head_granules;
+  const int32_t base = 8 * (in_head ? i : (v.first >> 3) + i - v.head_granules);
+  const int32_t lo = in_head ? 0 : max(v.first - base, 0);
+  const int32_t hi = min((in_head ? v.head : v.n) - base, 8);
+  bits = (0xffu >> (8 - hi)) & (0xffu << lo);
+  return base;
+}
 
 // DP: head dim of the tiles (columns beyond D are zeros).  T: q, out.  E4M3: the cache's type
-// (else T).  A warp's tile holds TOK tokens of k and of v, rows of DP elements whose 16-byte
-// chunks are exchanged by XOR with the row, so that ldmatrix and the e4m3 reads are free of
-// bank conflicts.
+// (else T).  A warp's tile holds TOK tokens of k and of v as boxes of 8 tokens x 128 bytes, the
+// 16-byte chunks of a box's row r exchanged by XOR with r (TMA's 128-byte swizzle), so that
+// ldmatrix and the e4m3 reads are free of bank conflicts.
 template <typename T, bool E4M3, int DP>
 struct Geo {
-  static constexpr int TOK = E4M3 ? 32 : 16;
   static constexpr int ES = E4M3 ? 1 : 2;
-  static constexpr int ROW = DP * ES;          // bytes
-  static constexpr int CHUNKS = ROW / 16;
-  static constexpr int TILE = TOK * ROW;       // k or v
-  static constexpr int STAGES = DP > 64 ? 3 : 4;
-  static constexpr int RING = STAGES * 2 * TILE;  // per warp
-  static constexpr int STEP = kWarps * TOK;       // tokens per block step
-  static constexpr int JOIN = kWarps * 8 * DP * 4;  // the warps' outputs, eight rows at a time
-  static constexpr int SMEM = kWarps * RING + JOIN;
-  static constexpr int PER_SM = DP > 128 ? 1 : DP > 64 ? 2 : 3;  // blocks
-  static constexpr uint32_t KEY = CHUNKS >= 8 ? 7 : CHUNKS - 1;
+  static constexpr int CHUNKS = DP * ES / 16;      // of a row
+  static constexpr int BOXES = CHUNKS / 8;         // of a granule
+  static constexpr int TOK = DP * ES <= 128 ? 32 : 16;
+  static constexpr int TILE = TOK * DP * ES;       // k or v
+  // As many warps as their registers allow (12 of 168: 32 sequences up to 8192, D 128, 103 us
+  // against 110 with 8 of 255); an e4m3 tile's unpacking spills at 168 (112 against 130 us on
+  // four sequences up to 65536 with 8 warps and 12).
+  static constexpr int WARPS = DP > 128 ? (E4M3 ? 8 : 4) : E4M3 ? 8 : 12;
+  static constexpr int STAGES = DP > 128 && !E4M3 ? 3 : 2;
+  static constexpr int RING = STAGES * 2 * TILE;   // per warp
+  static constexpr int THREADS = WARPS * 32;
+  static constexpr int JROW = DP + (E4M3 ? 16 : 8); // row of the join, apart against bank conflicts
+  static constexpr int JOIN = WARPS * 4 * JROW * 4;  // the warps' outputs, four rows at a time
+  static constexpr int SMEM = 1024 + WARPS * RING + JOIN;  // 1024: the ring starts on a multiple
+  static_assert(SMEM <= 225 * 1024 && BOXES >= 1, "the rings and the join fit");
   __device__ static uint32_t at(int row, int chunk) {
-    return (uint32_t)(row * ROW + ((chunk ^ (row & KEY)) << 4));
+    return (uint32_t)((((row >> 3) * BOXES + (chunk >> 3)) << 10) + ((row & 7) << 7) +
+                      (((chunk ^ row) & 7) << 4));
   }
 };
 
-// A place in the list of steps: step `step` of `steps` of cache head hk, row block rb, of
-// sequence b.
+// A place in the list of steps: step `step` of `steps` of head block hb of sequence b.
 struct Cursor {
-  int b, hk, rb, step, steps;
+  int b, hb, step, steps;
   Visible vis;
 };
 
-template <typename T, bool E4M3, int DP>
-__global__ void __launch_bounds__(kWarps * 32, Geo<T, E4M3, DP>::PER_SM)
-    paged_attn_kernel(const AttnArgs a) {
+// TMA: the granules come through the tensor maps (else by 16-byte copies of the lanes).
+template <typename T, bool E4M3, int DP, bool TMA>
+__global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
+    paged_attn_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
+                      const __grid_constant__ CUtensorMap vmap) {
   using G = Geo<T, E4M3, DP>;
   using MT = std::conditional_t<E4M3, __half, T>;  // MMA type
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t scan_slots[kWarps];
-  __shared__ int32_t find_seq;
-  __shared__ int64_t find_unit;
+  extern __shared__ uint8_t smem_raw[];  // starts on 16 bytes
   __shared__ int last_flag;
-  __shared__ float join_m[kWarps][16], join_l[kWarps][16];
-  __shared__ uint32_t seen[kWarps][G::STAGES];  // bit r: row r of the stage's tile is visible
+  __shared__ float join_m[G::WARPS][16], join_l[G::WARPS][16];  // the warps', then weights
+  __shared__ float row_m[G::WARPS][16], row_l[G::WARPS][16];    // the vheads'
+  __shared__ uint32_t seen[G::WARPS][G::STAGES];  // bit r: row r of the stage's tile is visible
+  __shared__ alignas(8) uint64_t arrived[G::WARPS][G::STAGES];  // the stage's copies
+  __shared__ volatile int abort_flag;
+  uint8_t* const smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   const int nblk = gridDim.x;
-  const int items_per_seq = a.hkv * a.row_blocks;
   const int64_t capacity = (int64_t)a.c.table_cols * a.c.page_size.d;
-  auto steps_of = [&](const Visible& v) { return (v.count + G::STEP - 1) / G::STEP; };
+  constexpr int NG = G::TOK / 8;  // granules of a tile
 
-  // ---- the number of steps; sequences that show nothing come out as zeros
-  int64_t mine = 0;
-  for (int b = tid; b < a.B; b += kWarps * 32) mine += steps_of(visible_of(a, b, capacity));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) scan_slots[warp] = mine;
-  for (int b = blockIdx.x; b < a.B; b += nblk)
-    if (visible_of(a, b, capacity).count == 0) {
+  // The next kernel of the stream may come up as this one's blocks leave; this one has come up
+  // so itself, perhaps, and waits here for what it reads.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) abort_flag = 0;
+  if (TMA && lane == 0) {
+    for (int i = 0; i < G::STAGES; ++i) mbar_init(&arrived[warp][i], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- how the warps share the work: HB of them on as many vheads at the same tokens, TG times
+  // that at neighbouring tokens.  Large calls take HB = heads_wide, so that a block reads what
+  // lies together in memory (a token's heads; 256 bytes of a head at a time cost the HBM a
+  // fifth of its rate, 128 bytes a third); small ones HB = 1, which has fewer parts to join.
+  // Sequences that show nothing come out as zeros.
+  const int tg_wide = G::WARPS / a.heads_wide;
+  // (Every warp scans the lengths by itself: no barrier.)
+  int32_t wide = 0, narrow = 0;  // steps of an item, over the sequences
+  int first_granules = 0;        // of sequence `lane`
+#pragma unroll 1
+  for (int base = 0; base < a.B; base += 32) {
+    const int b = base + lane;
+    const int n = b < a.B ? visible_of(a, b, capacity).granules : 0;
+    if (base == 0) first_granules = n;
+    wide += (n + tg_wide * NG - 1) / (tg_wide * NG);
+    narrow += (n + G::WARPS * NG - 1) / (G::WARPS * NG);
+    if (n == 0 && warp == 0 && b < a.B && b % nblk == blockIdx.x) {
       T* o = static_cast<T*>(a.out) + (int64_t)b * a.hq * a.D;
-      for (int i = tid * 8; i < a.hq * a.D; i += kWarps * 32 * 8)
+#pragma unroll 1
+      for (int i = 0; i < a.hq * a.D; i += 8)
         *reinterpret_cast<uint4*>(o + i) = make_uint4(0, 0, 0, 0);
     }
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += scan_slots[w];
-  total *= items_per_seq;
-  if (total == 0) return;
+  }
+  wide = __reduce_add_sync(0xffffffffu, wide);
+  narrow = __reduce_add_sync(0xffffffffu, narrow);
+  const int items_wide = (a.vheads + a.heads_wide - 1) / a.heads_wide;
+  const bool large = wide * items_wide >= nblk * kLargeSteps;
+  const int HB = large ? a.heads_wide : 1, TG = large ? tg_wide : G::WARPS;
+  const int items_per_seq = large ? items_wide : a.vheads;
+  const int step_granules = TG * NG;
+  const int32_t total = large ? wide * items_wide : narrow * a.vheads;
+  auto steps_of = [&](int granules) { return (granules + step_granules - 1) / step_granules; };
+  const int my_h = warp % HB, my_t = warp / HB;  // my_t >= TG: a warp without work
+  // the vhead of this warp in head block hb, or -1
+  auto vhead = [&](int hb) {
+    const int v = hb * HB + my_h;
+    return my_t < TG && v < a.vheads ? v : -1;
+  };
 
-  // ---- this block's share [unit, unit_end) of the list
-  const int64_t users = min((int64_t)nblk, (total + kMinSteps - 1) / kMinSteps);
-  if (blockIdx.x >= users) return;
-  auto share_start = [&](int64_t c) { return total * c / users; };
-  auto block_of = [&](int64_t u) { return ((u + 1) * users - 1) / total; };
-  const int64_t unit0 = share_start(blockIdx.x);
-  const int n_steps = (int)(share_start(blockIdx.x + 1) - unit0);
+  // ---- this block's share of the list: `share` steps from unit0 on
+  const int32_t share = max((total + nblk - 1) / nblk, kMinSteps);
+  const int32_t unit0 = blockIdx.x * share;
+  if (unit0 >= total) return;
+  const int n_steps = min(share, total - unit0);
 
-  // ---- the sequence that holds unit0: scan the lengths a block's width at a time
-  int64_t seq_unit = 0;  // first unit of the sequence
-  Cursor cc{};           // where the computation is
+  // ---- the sequence that holds unit0
+  Cursor cc{};  // where the computation is
   {
-    int64_t before = 0;
-    for (int base = 0; base < a.B; base += kWarps * 32) {
-      const int64_t n =
-          base + tid < a.B ? (int64_t)steps_of(visible_of(a, base + tid, capacity)) * items_per_seq
-                           : 0;
-      int64_t inc = n;
+    int32_t before = 0, seq_unit = 0;
+#pragma unroll 1
+    for (int base = 0; base < a.B; base += 32) {
+      int32_t n = first_granules;
+      if (base > 0) n = base + lane < a.B ? visible_of(a, base + lane, capacity).granules : 0;
+      n = steps_of(n) * items_per_seq;
+      int32_t inc = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+        const int32_t u = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += u;
       }
-      __syncthreads();
-      if (lane == 31) scan_slots[warp] = inc;
-      if (tid == 0) find_seq = -1;
-      __syncthreads();
-      int64_t off = before, chunk = 0;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) off += scan_slots[w];
-        chunk += scan_slots[w];
-      }
-      const int64_t lo = off + inc - n;
-      if (unit0 >= lo && unit0 < lo + n) {
-        find_seq = base + tid;
-        find_unit = lo;
-      }
-      __syncthreads();
-      if (find_seq >= 0) {
-        cc.b = find_seq;
-        seq_unit = find_unit;
+      const int32_t lo = before + inc - n;
+      const uint32_t here = __ballot_sync(0xffffffffu, unit0 >= lo && unit0 < lo + n);
+      if (here) {
+        cc.b = base + __ffs(here) - 1;
+        seq_unit = __shfl_sync(0xffffffffu, lo, __ffs(here) - 1);
         break;
       }
-      before += chunk;
+      before += __shfl_sync(0xffffffffu, inc, 31);
     }
     cc.vis = visible_of(a, cc.b, capacity);
-    cc.steps = steps_of(cc.vis);
-    const int rel = (int)((unit0 - seq_unit) / cc.steps);  // head-major within the sequence
-    cc.step = (int)(unit0 - seq_unit - (int64_t)rel * cc.steps);
-    cc.hk = rel / a.row_blocks;
-    cc.rb = rel - cc.hk * a.row_blocks;
+    cc.steps = steps_of(cc.vis.granules);
+    cc.hb = (unit0 - seq_unit) / cc.steps;  // head blocks in order within the sequence
+    cc.step = unit0 - seq_unit - cc.hb * cc.steps;
   }
   // To the next step of the list (only while one is left).  True at an item's end.
   auto advance = [&](Cursor& c) {
     if (++c.step < c.steps) return false;
     c.step = 0;
-    if (++c.rb == a.row_blocks) {
-      c.rb = 0;
-      if (++c.hk == a.hkv) {
-        c.hk = 0;
-        do {
-          ++c.b;
-          if (c.b >= a.B) break;
-          c.vis = visible_of(a, c.b, capacity);
-          c.steps = steps_of(c.vis);
-        } while (c.steps == 0);
-      }
+    if (++c.hb == items_per_seq) {
+      c.hb = 0;
+      do {
+        ++c.b;
+        if (c.b >= a.B) break;
+        c.vis = visible_of(a, c.b, capacity);
+        c.steps = steps_of(c.vis.granules);
+      } while (c.steps == 0);
     }
     return true;
   };
 
-  // ---- the copy side of the ring: the lane's rows of a tile, their pages read one step ahead
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * G::RING;
-  const int lr = lane >> 2, lc = lane & 3;  // copy: row lr + 8 i, chunks lc + 4 i
-  const int chunks = a.D * G::ES / 16;      // live chunks of a row
-  constexpr int RPL = G::TOK / 8;           // rows per lane
+  // ---- the copy side of the ring.  A step's pages are looked up one step before its copies:
+  // with TMA by lane i for granule i of the tile, else by lane r for row r.
+  uint8_t* const ring_p = smem + warp * G::RING;
+  const uint32_t ring = smem_u32(ring_p);
   const uint8_t* kb = static_cast<const uint8_t*>(a.c.k);
   const uint8_t* vb = static_cast<const uint8_t*>(a.c.v);
+  struct Place {
+    int32_t page, slot, head;
+    uint32_t bits;  // TMA: the granule's visible tokens; else bit 0
+  };
   Cursor lk = cc;
-  int looked = 0, lk_head = 0;
-  int32_t page[RPL], slot[RPL];
-  auto lookup = [&]() {
+  int looked = 0;
+  auto lookup = [&](Place& r) {
+    r.page = -1;
+    r.bits = 0;
     if (looked < n_steps) {
-      lk_head = lk.hk;
-      const int32_t* row = a.c.table + lk.b * a.c.table_stride;
-#pragma unroll
-      for (int i = 0; i < RPL; ++i) {
-        page[i] = -1;
-        const int32_t v = lk.step * G::STEP + warp * G::TOK + lr + 8 * i;
-        if (v < lk.vis.count) {
-          const int32_t tok = v < lk.vis.head ? v : v + lk.vis.skip;
+      const int v = vhead(lk.hb);
+      r.head = v / a.row_blocks;
+      const int in_tile = TMA ? lane : lane >> 3;
+      const int32_t i = lk.step * step_granules + my_t * NG + in_tile;
+      if (v >= 0 && in_tile < NG && i < lk.vis.granules) {
+        uint32_t bits;
+        int32_t tok = granule(lk.vis, i, bits);
+        if constexpr (!TMA) {
+          tok += lane & 7;
+          bits = bits >> (lane & 7) & 1;
+        }
+        if (bits != 0) {
           const int32_t col = a.c.page_size.div(tok);
-          slot[i] = tok - col * a.c.page_size.d;
-          page[i] = __ldg(row + col);
+          r.slot = tok - col * a.c.page_size.d;
+          r.bits = bits;
+          r.page = __ldg(a.c.table + lk.b * a.c.table_stride + col);
         }
       }
       advance(lk);
     }
     ++looked;
   };
-  auto fill = [&](int stage) {
+  auto fill = [&](const Place& r, int stage) {
     const uint32_t kt = ring + stage * (2 * G::TILE), vt = kt + G::TILE;
-    uint32_t bits = 0;
-#pragma unroll
-    for (int i = 0; i < RPL; ++i) {
-      const bool live = (uint32_t)page[i] < (uint32_t)a.c.pages;
-      const int row = lr + 8 * i;
-      // one bit per row out of the four equal ones of its lanes
-      uint32_t x = __ballot_sync(0xffffffffu, live) & 0x11111111u;
-      x = (x | x >> 3) & 0x03030303u;
-      x = (x | x >> 6) & 0x000f000fu;
-      x = (x | x >> 12) & 0xffu;
-      bits |= x << (8 * i);
-      const uint8_t* ks = kb;
-      const uint8_t* vs = vb;
+    const bool live = (uint32_t)r.page < (uint32_t)a.c.pages;
+    if constexpr (TMA) {
+      uint32_t bits = live ? r.bits << (8 * lane) : 0;
+      const int boxes = __popc(__ballot_sync(0xffffffffu, live)) * (2 * G::BOXES);
+      bits = __reduce_or_sync(0xffffffffu, bits);
+      if (lane == 0) {
+        seen[warp][stage] = bits;
+        mbar_arrive_expect_tx(&arrived[warp][stage], boxes * 1024);
+      }
+      __syncwarp();
       if (live) {
-        ks += ((uint64_t)(uint32_t)page[i] * a.k_page +
-               (uint32_t)(slot[i] * a.k_slot + lk_head * a.k_head)) << 4;
-        vs += ((uint64_t)(uint32_t)page[i] * a.v_page +
-               (uint32_t)(slot[i] * a.v_slot + lk_head * a.v_head)) << 4;
-      }
+        const uint32_t bar = smem_u32(&arrived[warp][stage]);
 #pragma unroll
-      for (int c = 0; c < G::CHUNKS; c += 4) {
-        const bool on = live && c + lc < chunks;
-        cp16(kt + G::at(row, c + lc), ks + (on ? (c + lc) * 16 : 0), on);
+        for (int i = 0; i < G::BOXES; ++i) {
+          const int x = i * (128 / G::ES);
+          tma_box(kt + (lane * G::BOXES + i) * 1024, &kmap, bar, x, r.slot, r.head, r.page);
+          tma_box(vt + (lane * G::BOXES + i) * 1024, &vmap, bar, x, r.slot, r.head, r.page);
+        }
       }
+    } else {
+      const uint32_t bits = __ballot_sync(0xffffffffu, live);
+      if (lane == 0) seen[warp][stage] = bits;
+      uint64_t ko = 0, vo = 0;
+      if (live) {
+        ko = (uint64_t)(uint32_t)r.page * a.k_page + (uint32_t)(r.slot * a.k_slot + r.head * a.k_head);
+        vo = (uint64_t)(uint32_t)r.page * a.v_page + (uint32_t)(r.slot * a.v_slot + r.head * a.v_head);
+      }
+      const int chunks = a.D * G::ES / 16;  // live chunks of a row
 #pragma unroll
-      for (int c = 0; c < G::CHUNKS; c += 4) {
-        const bool on = live && c + lc < chunks;
-        cp16(vt + G::at(row, c + lc), vs + (on ? (c + lc) * 16 : 0), on);
+      for (int i = 0; i < NG; ++i) {
+        const int row = i * 8 + g;
+        const uint8_t* ks = kb + (__shfl_sync(0xffffffffu, ko, row) << 4);
+        const uint8_t* vs = vb + (__shfl_sync(0xffffffffu, vo, row) << 4);
+#pragma unroll
+        for (int c = 0; c < G::CHUNKS; c += 4) {
+          const bool on = (bits >> row & 1) && c + t4 < chunks;
+          cp16(kt + G::at(row, c + t4), ks + (on ? (c + t4) * 16 : 0), on);
+          cp16(vt + G::at(row, c + t4), vs + (on ? (c + t4) * 16 : 0), on);
+        }
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    if (lane == 0) seen[warp][stage] = bits;
   };
 
-  lookup();
-#pragma unroll
-  for (int s = 0; s < G::STAGES - 1; ++s) {
-    if (s < n_steps) fill(s);
-    lookup();
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
+  Place next;
+  lookup(next);
 
+  // Where the lane reads in a tile: chunk c of the row is 16 c bytes on, XORed (tiles start on
+  // multiples of 1 KB).  kofs: k rows for ldmatrix (tokens (lane & 7) + 8 (lane >> 4), chunk
+  // lane >> 3 & 1), or for e4m3 token g, the lane's quarter of the row.  vofs: v rows for
+  // transposing ldmatrix (token lane & 15, chunk lane >> 4).
+  const uint32_t vofs = (((lane & 15) >> 3) * G::BOXES << 10) + ((lane & 7) << 7) +
+                        (((lane >> 4) ^ (lane & 7)) << 4);
+  uint32_t kofs;
+  if constexpr (E4M3) {
+    const int c = t4 * (G::CHUNKS / 4);
+    kofs = ((c >> 3) << 10) + (g << 7) + (((c & 7) ^ g) << 4);
+  } else {
+    kofs = ((lane >> 4) * G::BOXES << 10) + ((lane & 7) << 7) +
+           ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+  }
   uint32_t qf[DP / 16][4];
   float rscale[2], m[2], l[2], o[DP / 8][4];
-  int64_t item_unit = unit0 - cc.step;  // the item's first unit
-  bool fresh = true;
-  int stage = 0, refill = G::STAGES - 1;
-  for (int s = 0; s < n_steps; ++s) {
-    const int rows = min(16, a.group - cc.rb * 16);
-    const int head0 = cc.hk * a.group + cc.rb * 16;
+  int32_t item_unit = unit0 - cc.step;  // the item's first unit
+  bool fresh = true, failed = false;
+  int stage = 0, refill = 0;
+  uint32_t parity = 0;
+#pragma unroll 1
+  for (int s = 1 - G::STAGES; s < n_steps; ++s) {
+    // copies go out STAGES - 1 steps ahead, into the stage that the step before has read
+    __syncwarp();
+    if (s + G::STAGES - 1 < n_steps && !failed) fill(next, refill);
+    else if (!TMA) asm volatile("cp.async.commit_group;" ::: "memory");
+    lookup(next);
+    if (++refill == G::STAGES) refill = 0;
+    if (s < 0) continue;
+    const int vh = max(vhead(cc.hb), 0), hk = vh / a.row_blocks;
+    const int first_row = (vh - hk * a.row_blocks) * 16;
+    const int rows = min(16, a.group - first_row), head0 = hk * a.group + first_row;
     if (fresh) {
       // ---- a new item: q, the 16 rows of the A operand, from global memory into fragments
       fresh = false;
@@ -381,7 +476,7 @@ __global__ void __launch_bounds__(kWarps * 32, Geo<T, E4M3, DP>::PER_SM)
           const uint32_t e = (__float_as_uint(qmax[r]) >> 23) & 0xff;
           const bool plain = e >= 1 && e <= 252;
           mul[r] = plain ? __uint_as_float((254 - e) << 23) : 1.f;
-          rscale[r] *= a.c.k_scale[cc.hk] * (plain ? __uint_as_float(e << 23) : 1.f);
+          rscale[r] *= a.c.k_scale[hk] * (plain ? __uint_as_float(e << 23) : 1.f);
         }
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks)
@@ -399,17 +494,28 @@ __global__ void __launch_bounds__(kWarps * 32, Geo<T, E4M3, DP>::PER_SM)
         for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
     }
 
-    asm volatile("cp.async.wait_group %0;" ::"n"(G::STAGES - 2) : "memory");
-    __syncwarp();
-    // refill the stage that the previous step has read
-    if (s + G::STAGES - 1 < n_steps) fill(refill);
-    lookup();
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    if constexpr (TMA) {
+      if (!mbar_wait_warp(&arrived[warp][stage], parity, &abort_flag, WD_TMA_WAIT)) failed = true;
+    } else {
+      asm volatile("cp.async.wait_group %0;" ::"n"(G::STAGES - 1) : "memory");
+      __syncwarp();
+    }
     const uint32_t kt = ring + stage * (2 * G::TILE), vt = kt + G::TILE;
-    const uint32_t bits = seen[warp][stage];
-    refill = stage;
-    stage = stage + 1 == G::STAGES ? 0 : stage + 1;
+    const uint32_t bits = failed ? 0 : seen[warp][stage];
+    constexpr uint32_t kAll = G::TOK == 32 ? 0xffffffffu : (1u << G::TOK) - 1;
+    if (TMA && bits != kAll && bits != 0) {
+      // v of tokens that are not seen has weight zero but may be NaN: zeros instead, ordered
+      // before the copies that come here later
+      uint8_t* vp = ring_p + stage * (2 * G::TILE) + G::TILE;
+      if (lane < G::TOK && !(bits >> lane & 1))
+        for (int i = 0; i < G::CHUNKS; ++i)
+          *reinterpret_cast<uint4*>(vp + G::at(lane, i)) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+    }
+    if (++stage == G::STAGES) stage = 0, parity ^= 1;
 
+    if (bits != 0) {
     // ---- scores of 16 rows x TOK tokens
     float sc[G::TOK / 8][4];
 #pragma unroll
@@ -425,27 +531,29 @@ __global__ void __launch_bounds__(kWarps * 32, Geo<T, E4M3, DP>::PER_SM)
           uint32_t w[4];
           asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
                        : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(kt + G::at(n * 8 + g, t4 * CPL + j)) : "memory");
+                       : "r"(((kt + kofs) ^ (j << 4)) + (n * G::BOXES << 10)) : "memory");
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             mma16816<MT>(sc[n], qf[j * 4 + i], e4m3x2_to_f16x2(w[i]), e4m3x2_to_f16x2(w[i] >> 16));
         }
     } else {
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
-        uint32_t kf[4];  // tokens 0-7 (k 0-7, 8-15), tokens 8-15 (k 0-7, 8-15)
-        ldsm4(kf, kt + G::at((lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
-        mma16816<MT>(sc[0], qf[ks], kf[0], kf[1]);
-        mma16816<MT>(sc[1], qf[ks], kf[2], kf[3]);
-      }
+      for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+        for (int h = 0; h < G::TOK / 16; ++h) {
+          uint32_t kf[4];  // tokens 0-7 (k 0-7, 8-15), tokens 8-15 (k 0-7, 8-15)
+          ldsm4(kf, ((kt + kofs) ^ ((ks * 2 & 7) << 4)) +
+                        ((h * 2 * G::BOXES + (ks * 2 >> 3)) << 10));
+          mma16816<MT>(sc[2 * h], qf[ks], kf[0], kf[1]);
+          mma16816<MT>(sc[2 * h + 1], qf[ks], kf[2], kf[3]);
+        }
     }
 
     // ---- softmax in log2 units; a row that has seen nothing yet keeps m = -inf, l = 0
-    constexpr uint32_t kAll = G::TOK == 32 ? 0xffffffffu : (1u << G::TOK) - 1;
 #pragma unroll
     for (int n = 0; n < G::TOK / 8; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sc[n][i] *= rscale[i >> 1];
+      for (int r = 0; r < 2; ++r) mul2(sc[n][2 * r], sc[n][2 * r + 1], rscale[r]);
     if (bits != kAll) {
 #pragma unroll
       for (int n = 0; n < G::TOK / 8; ++n)
@@ -473,16 +581,18 @@ __global__ void __launch_bounds__(kWarps * 32, Geo<T, E4M3, DP>::PER_SM)
 #pragma unroll
       for (int n = 0; n < DP / 8; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] *= al[i >> 1];
+        for (int r = 0; r < 2; ++r) mul2(o[n][2 * r], o[n][2 * r + 1], al[r]);
       l[0] *= al[0], l[1] *= al[1];
     }
     m[0] = mx[0], m[1] = mx[1];
 #pragma unroll
     for (int n = 0; n < G::TOK / 8; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sc[n][i] = exp2_fast(sc[n][i] - mref[i >> 1]);
-        l[i >> 1] += sc[n][i];
+      for (int r = 0; r < 2; ++r) {
+        add2(sc[n][2 * r], sc[n][2 * r + 1], -mref[r]);
+        sc[n][2 * r] = exp2_fast(sc[n][2 * r]);
+        sc[n][2 * r + 1] = exp2_fast(sc[n][2 * r + 1]);
+        l[r] += sc[n][2 * r] + sc[n][2 * r + 1];
       }
 
     // ---- o += p v
@@ -494,53 +604,54 @@ __global__ void __launch_bounds__(kWarps * 32, Geo<T, E4M3, DP>::PER_SM)
                                 pack2<MT>(sc[2 * h + 1][0], sc[2 * h + 1][1]),
                                 pack2<MT>(sc[2 * h + 1][2], sc[2 * h + 1][3])};
 #pragma unroll
-        for (int blk = 0; blk < DP / 32; ++blk) {
-          // column g of n-tile (blk, j) stands for d = 32 blk + 4 g + j
-          uint32_t w[4];
+        for (int n = 0; n < DP / 32; ++n) {
+          // two chunks of 16 values of d: a register of the transposed 16-bit read has values
+          // d = 16 c + 2 g and the next of two tokens, so column g of n-tile (c, e) stands for
+          // d = 16 c + 2 g + e
+          uint32_t vf[4];
+          ldsm4t(vf, ((vt + vofs) ^ ((n * 2 & 7) << 4)) +
+                         ((h * 2 * G::BOXES + (n * 2 >> 3)) << 10));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = h * 16 + t4 * 2 + (i & 1) + (i >> 1) * 8;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i])
-                         : "r"(vt + G::at(row, blk * 2 + (g >> 2)) + (g & 3) * 4) : "memory");
-          }
-          uint32_t f[4][2];
+          for (int i = 0; i < 4; ++i) vf[i] = __byte_perm(vf[i], 0, 0x3120);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f[i][0] = e4m3x2_to_f16x2(w[i]);
-            f[i][1] = e4m3x2_to_f16x2(w[i] >> 16);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
-            mma16816<MT>(o[blk * 4 + j], pf, __byte_perm(f[0][j >> 1], f[1][j >> 1], sel),
-                         __byte_perm(f[2][j >> 1], f[3][j >> 1], sel));
+          for (int c = 0; c < 2; ++c) {
+            mma16816<MT>(o[n * 4 + c * 2], pf, e4m3x2_to_f16x2(vf[c * 2]),
+                         e4m3x2_to_f16x2(vf[c * 2 + 1]));
+            mma16816<MT>(o[n * 4 + c * 2 + 1], pf, e4m3x2_to_f16x2(vf[c * 2] >> 16),
+                         e4m3x2_to_f16x2(vf[c * 2 + 1] >> 16));
           }
         }
       }
     } else {
       // p rounded to T; for bf16 its rounding error goes through a second MMA, so p counts
       // with 16 bits and the output is as near as its own type allows
-      uint32_t pf[4], pe[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = sc[i >> 1][(i & 1) * 2], y = sc[i >> 1][(i & 1) * 2 + 1];
-        pf[i] = pack2<MT>(x, y);
-        if constexpr (!std::is_same_v<MT, __half>) {
-          const T* e = reinterpret_cast<const T*>(&pf[i]);
-          pe[i] = pack2<MT>(x - to_f32(e[0]), y - to_f32(e[1]));
+      for (int h = 0; h < G::TOK / 16; ++h) {
+        uint32_t pf[4], pe[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = sc[2 * h + (i >> 1)][(i & 1) * 2];
+          const float y = sc[2 * h + (i >> 1)][(i & 1) * 2 + 1];
+          pf[i] = pack2<MT>(x, y);
+          if constexpr (!std::is_same_v<MT, __half>) {
+            const T* e = reinterpret_cast<const T*>(&pf[i]);
+            pe[i] = pack2<MT>(x - to_f32(e[0]), y - to_f32(e[1]));
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n) {
+          uint32_t vf[4];  // d 0-7 (tokens 0-7, 8-15), d 8-15 (tokens 0-7, 8-15)
+          ldsm4t(vf, ((vt + vofs) ^ ((n * 2 & 7) << 4)) +
+                         ((h * 2 * G::BOXES + (n * 2 >> 3)) << 10));
+          mma16816<MT>(o[2 * n], pf, vf[0], vf[1]);
+          mma16816<MT>(o[2 * n + 1], pf, vf[2], vf[3]);
+          if constexpr (!std::is_same_v<MT, __half>) {
+            mma16816<MT>(o[2 * n], pe, vf[0], vf[1]);
+            mma16816<MT>(o[2 * n + 1], pe, vf[2], vf[3]);
+          }
         }
       }
-#pragma unroll
-      for (int n = 0; n < DP / 16; ++n) {
-        uint32_t vf[4];  // d 0-7 (tokens 0-7, 8-15), d 8-15 (tokens 0-7, 8-15)
-        ldsm4t(vf, vt + G::at(lane & 15, n * 2 + (lane >> 4)));
-        mma16816<MT>(o[2 * n], pf, vf[0], vf[1]);
-        mma16816<MT>(o[2 * n + 1], pf, vf[2], vf[3]);
-        if constexpr (!std::is_same_v<MT, __half>) {
-          mma16816<MT>(o[2 * n], pe, vf[0], vf[1]);
-          mma16816<MT>(o[2 * n + 1], pe, vf[2], vf[3]);
-        }
-      }
+    }
     }
 
     // ---- the item's end, or the share's
@@ -553,133 +664,290 @@ __global__ void __launch_bounds__(kWarps * 32, Geo<T, E4M3, DP>::PER_SM)
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
     }
+    const int c0 = item_unit / share;
+    const int n_parts = (item_unit + at.steps - 1) / share - c0 + 1;
+    const int v0 = at.hb * HB, heads = min(HB, a.vheads - v0);
+    const int part_floats = a.part_floats;
+    const int64_t slot_floats = (int64_t)a.heads_wide * part_floats;
+    // an item that starts in this share leaves its parts in the block's second slot
+    float* part = a.parts + (2 * (int64_t)blockIdx.x + (item_unit >= unit0 ? 1 : 0)) * slot_floats;
+    const int vecs = a.D >> 2;
+    float* jo = reinterpret_cast<float*>(smem + G::WARPS * G::RING);
+    // rows of vhead v, its cache head, its first output row
+    auto place = [&](int v, int& k, int& n) {
+      k = v / a.row_blocks;
+      const int r0 = (v - k * a.row_blocks) * 16;
+      n = min(16, a.group - r0);
+      return static_cast<T*>(a.out) + ((int64_t)at.b * a.hq + k * a.group + r0) * a.D;
+    };
+    if (TG == 1) {
+      // a warp has its vhead alone: its rows go out as they are
+      if (my_h < heads && my_t == 0) {
+        int k, n;
+        T* outp = place(v0 + my_h, k, n);
+        float* p = part + my_h * part_floats;
+#pragma unroll 1
+        for (int r = 0; r < 2; ++r) {
+          const int row = g + 8 * r;
+          const float lr = r ? l[1] : l[0];
+          const float inv = lr == 0.f ? 0.f : (E4M3 ? a.c.v_scale[k] : 1.f) / lr;
+          if (row >= n) break;
+          if (n_parts > 1 && t4 == 0)
+            __stcg(reinterpret_cast<float2*>(p + a.part_rows * a.D + 2 * row),
+                   make_float2(r ? m[1] : m[0], lr));
+          auto val = [&](int e, int i) { return r ? o[e][2 + i] : o[e][i]; };
+          if constexpr (E4M3) {
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) {
+              const int d = c * 16 + t4 * 4;
+              if (d >= a.D) continue;
+              const float4 v = make_float4(val(2 * c, 0), val(2 * c + 1, 0), val(2 * c, 1),
+                                           val(2 * c + 1, 1));
+              if (n_parts > 1)
+                __stcg(reinterpret_cast<float4*>(p + row * a.D + d), v);
+              else
+                *reinterpret_cast<uint2*>(outp + row * a.D + d) =
+                    make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < DP / 8; ++e) {
+              const int d = e * 8 + t4 * 2;
+              if (d >= a.D) continue;
+              const float x = val(e, 0), y = val(e, 1);
+              if (n_parts > 1)
+                __stcg(reinterpret_cast<float2*>(p + row * a.D + d), make_float2(x, y));
+              else
+                *reinterpret_cast<uint32_t*>(outp + row * a.D + d) = pack2<T>(x * inv, y * inv);
+            }
+          }
+        }
+      }
+    } else {
     if (t4 == 0) {
       join_m[warp][g] = m[0], join_m[warp][g + 8] = m[1];
       join_l[warp][g] = l[0], join_l[warp][g + 8] = l[1];
     }
-    const int64_t c0 = block_of(item_unit), c1 = block_of(item_unit + at.steps - 1);
-    const bool whole = c0 == c1;
-    const float vscale = E4M3 ? a.c.v_scale[at.hk] : 1.f;
-    T* outp = static_cast<T*>(a.out) + ((int64_t)at.b * a.hq + head0) * a.D;
-    const int64_t part_floats = 16 * (int64_t)(a.D + 2);
-    // an item that starts in this share leaves its part in the block's second slot
-    float* part = a.parts + (2 * (int64_t)blockIdx.x + (item_unit >= unit0 ? 1 : 0)) * part_floats;
-    const int vecs = a.D >> 2;
-    float* jo = reinterpret_cast<float*>(smem + kWarps * G::RING);
-    // the four warps' outputs meet in shared memory, eight rows at a time
+    __syncthreads();
+    // each row's maximum and sum over the warps on its vhead, and the warps' weights
+    if (tid < HB * 16) {
+      const int h = tid >> 4, row = tid & 15;
+      float mm = -INFINITY, ll = 0.f;
+#pragma unroll 2
+      for (int w = h; w < HB * TG; w += HB) mm = fmaxf(mm, join_m[w][row]);
+      const float mr = mm == -INFINITY ? 0.f : mm;
+#pragma unroll 2
+      for (int w = h; w < HB * TG; w += HB) {
+        const float f = exp2_fast(join_m[w][row] - mr);
+        ll += f * join_l[w][row];
+        join_m[w][row] = f;
+      }
+      row_m[h][row] = mm, row_l[h][row] = ll;
+    }
+    // the warps' outputs meet in shared memory, four rows at a time
+#pragma unroll 1
+    for (int piece = 0; piece * 4 < a.part_rows; ++piece) {
+      auto val = [&](int e, int i) { return piece >> 1 ? o[e][2 + i] : o[e][i]; };
+      if (g >> 2 == (piece & 1)) {
+        float* dst = jo + (warp * 4 + (g & 3)) * G::JROW;
+        if constexpr (E4M3) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (half == 1 && rows <= 8) break;
-      if (half == 1) __syncthreads();  // the first eight are read
+          for (int c = 0; c < DP / 16; ++c)
+            *reinterpret_cast<float4*>(dst + c * 16 + t4 * 4) = make_float4(
+                val(2 * c, 0), val(2 * c + 1, 0), val(2 * c, 1), val(2 * c + 1, 1));
+        } else {
 #pragma unroll
-      for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int d = E4M3 ? (n >> 2) * 32 + (t4 * 2 + i) * 4 + (n & 3) : n * 8 + t4 * 2 + i;
-          jo[(warp * 8 + g) * DP + d] = o[n][half * 2 + i];
+          for (int n = 0; n < DP / 8; ++n)
+            *reinterpret_cast<float2*>(dst + n * 8 + t4 * 2) =
+                make_float2(val(n, 0), val(n, 1));
         }
+      }
       __syncthreads();
-      const int half_rows = min(8, rows - half * 8);
-      for (int i = tid; i < half_rows * vecs; i += kWarps * 32) {
-        const int r = i / vecs, d = (i - r * vecs) * 4, row = half * 8 + r;
-        float mm = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, join_m[w][row]);
-        const float mr = mm == -INFINITY ? 0.f : mm;
-        float ll = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float f = exp2_fast(join_m[w][row] - mr);
-          ll += f * join_l[w][row];
-          const float4 v = *reinterpret_cast<const float4*>(jo + (w * 8 + r) * DP + d);
+#pragma unroll 1
+      for (int i = tid; i < heads * 4 * vecs; i += G::THREADS) {
+        const int hr = i / vecs, d = (i - hr * vecs) * 4, h = hr >> 2, row = piece * 4 + (hr & 3);
+        int k, n;
+        T* outp = place(v0 + h, k, n);
+        if (row >= n) continue;
+        const float mm = row_m[h][row], ll = row_l[h][row];
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int w = h; w < HB * TG; w += HB) {
+          const float f = join_m[w][row];
+          const float4 v = *reinterpret_cast<const float4*>(jo + (w * 4 + (hr & 3)) * G::JROW + d);
           acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
         }
-        if (whole) {
-          const float inv = ll == 0.f ? 0.f : vscale / ll;
+        if (n_parts == 1) {
+          const float inv = ll == 0.f ? 0.f : (E4M3 ? a.c.v_scale[k] : 1.f) / ll;
           *reinterpret_cast<uint2*>(outp + row * a.D + d) = make_uint2(
               pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
         } else {
-          __stcg(reinterpret_cast<float4*>(part + 32 + row * a.D + d),
+          float* p = part + h * part_floats;
+          __stcg(reinterpret_cast<float4*>(p + row * a.D + d),
                  make_float4(acc[0], acc[1], acc[2], acc[3]));
-          if (d == 0) __stcg(part + row, mm), __stcg(part + 16 + row, ll);
+          float* ml = p + a.part_rows * a.D + 2 * row;
+          if (d == 0) __stcg(ml, mm), __stcg(ml + 1, ll);
         }
       }
+      __syncthreads();  // shared memory is free again
     }
-    __syncthreads();  // shared memory is free again; the part's stores are ordered before ...
-    if (!whole) {
-      const int item_id = at.b * items_per_seq + at.hk * a.row_blocks + at.rb;
-      if (tid == 0) {  // ... this release
-        const int n_parts = (int)(c1 - c0 + 1);
-        int before;
-        asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;"
-                     : "=r"(before) : "l"(a.counters + item_id) : "memory");
-        last_flag = before == n_parts - 1;
-        if (last_flag) a.counters[item_id] = 0;  // zero again for the next call
-      }
-      __syncthreads();
-      if (last_flag) {
-        // the item starts in c0's second slot and goes on in the others' first
-        const float* p0 = a.parts + (2 * c0 + 1) * part_floats;
-        const int n_parts = (int)(c1 - c0 + 1);
-        auto part_at = [&](int k) { return p0 + (k == 0 ? 0 : (2 * (int64_t)k - 1) * part_floats); };
-        for (int i = tid; i < rows * vecs; i += kWarps * 32) {
-          const int row = i / vecs, d = (i - row * vecs) * 4;
-          float mm = -INFINITY;
-#pragma unroll 8
-          for (int k = 0; k < n_parts; ++k) mm = fmaxf(mm, __ldcg(part_at(k) + row));
-          const float mr = mm == -INFINITY ? 0.f : mm;
-          float ll = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-          for (int k = 0; k < n_parts; ++k) {
-            const float* p = part_at(k);
-            const float f = exp2_fast(__ldcg(p + row) - mr);
-            ll += f * __ldcg(p + 16 + row);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p + 32 + row * a.D + d));
-            acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
-          }
-          const float inv = ll == 0.f ? 0.f : vscale / ll;
-          *reinterpret_cast<uint2*>(outp + row * a.D + d) = make_uint2(
-              pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
-        }
-      }
     }
     item_unit += at.steps;
+    if (n_parts == 1) continue;
+    __syncthreads();  // the part's stores are ordered before ...
+    if (tid == 0) {   // ... this release
+      int32_t* counter = a.counters + at.b * items_per_seq + at.hb;
+      int before;
+      asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;"
+                   : "=r"(before) : "l"(counter) : "memory");
+      last_flag = before == n_parts - 1;
+      if (last_flag) *counter = 0;  // zero again for the next call
+    }
+    __syncthreads();
+    if (last_flag) {
+      // the item starts in c0's second slot and goes on in the others' first
+      const float* p0 = a.parts + (2 * (int64_t)c0 + 1) * slot_floats;
+      const int64_t stride = 2 * slot_floats;
+      // a warp per row: the parts' maximum, and what their weighted sums are divided by
+#pragma unroll 1
+      for (int i = warp; i < heads * a.part_rows; i += G::WARPS) {
+        const int h = i / a.part_rows, row = i - h * a.part_rows;
+        int kh, n;
+        place(v0 + h, kh, n);
+        if (row >= n) continue;
+        const float* p = p0 + h * part_floats + a.part_rows * a.D + 2 * row;
+        float mm = -INFINITY, ll = 0.f;
+        auto add = [&](float pm, float pl) {
+          const float nm = fmaxf(mm, pm), nr = nm == -INFINITY ? 0.f : nm;
+          ll = ll * exp2_fast(mm - nr) + pl * exp2_fast(pm - nr);
+          mm = nm;
+        };
+#pragma unroll 1
+        for (int k = lane; k < n_parts; k += 32) {
+          const float2 x = __ldcg(
+              reinterpret_cast<const float2*>(p + (k == 0 ? 0 : k * stride - slot_floats)));
+          add(x.x, x.y);
+        }
+#pragma unroll 1
+        for (int x = 16; x > 0; x >>= 1) {
+          const float pm = __shfl_xor_sync(0xffffffffu, mm, x);
+          add(pm, __shfl_xor_sync(0xffffffffu, ll, x));
+        }
+        if (lane == 0) {
+          row_m[h][row] = mm == -INFINITY ? 0.f : mm;
+          row_l[h][row] = ll == 0.f ? 0.f : (E4M3 ? a.c.v_scale[kh] : 1.f) / ll;
+        }
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int i = tid; i < heads * a.part_rows * vecs; i += G::THREADS) {
+        const int hr = i / vecs, d = (i - hr * vecs) * 4;
+        const int h = hr / a.part_rows, row = hr - h * a.part_rows;
+        int kh, n;
+        T* outp = place(v0 + h, kh, n);
+        if (row >= n) continue;
+        const float* p = p0 + h * part_floats;
+        const int ml = a.part_rows * a.D + 2 * row, at_d = row * a.D + d;
+        const float mr = row_m[h][row], inv = row_l[h][row];
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int k = 0; k < n_parts; k += 8) {
+          float f[8];
+          float4 v[8];
+          const float* q = p;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const bool on = k + u < n_parts;
+            f[u] = on ? __ldcg(q + ml) : -INFINITY;
+            v[u] = on ? __ldcg(reinterpret_cast<const float4*>(q + at_d)) : float4{};
+            q += k + u == 0 ? slot_floats : stride;
+          }
+          p = q;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            f[u] = exp2_fast(f[u] - mr);
+            acc[0] += f[u] * v[u].x, acc[1] += f[u] * v[u].y;
+            acc[2] += f[u] * v[u].z, acc[3] += f[u] * v[u].w;
+          }
+        }
+        *reinterpret_cast<uint2*>(outp + row * a.D + d) = make_uint2(
+            pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
+      }
+      __syncthreads();  // row_m and row_l are read
+    }
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  if constexpr (TMA) {
+    // Every copy has been waited for, unless a wait ran out (the watchdog word says so and the
+    // output is not valid): then give those in flight the time to land before the block ends.
+    if (failed) {
+      const long long t0 = clock64();
+      while (clock64() - t0 < 20000000ll) {
+      }
+    }
+  } else {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+}
+
+// Warps of a block on different vheads: as many as keep all warps busy, or nearly, and at most
+// `most_wide`: 8 for 16-bit caches (32 sequences up to 8192, 8 heads of 128: 103 us, 122 with 1;
+// 64 windows of 1024, 12 heads of 64: 41 against 53); 1 for e4m3, whose unpacking keeps it
+// below the HBM's rate either way, so the joins of many heads count (112 us, 124 with 4).
+int heads_wide(int vheads, int warps, int most_wide) {
+  int best = 1;
+  double most = 0;
+  for (int h = 1; h <= warps && h <= vheads && h <= most_wide; ++h) {
+    const double busy = (double)vheads / ((vheads + h - 1) / h * h) * (warps / h * h) / warps;
+    if (busy * (h >= 4 ? 1.0 : h >= 2 ? 0.9 : 0.8) >= most)
+      most = busy * (h >= 4 ? 1.0 : h >= 2 ? 0.9 : 0.8), best = h;
+  }
+  return best;
+}
+
+template <typename T, bool E4M3, int DP, bool TMA>
+int launch_attn_tma(AttnArgs a, const CacheHandle* h, cudaStream_t s) {
+  using G = Geo<T, E4M3, DP>;
+  a.heads_wide = heads_wide(a.vheads, G::WARPS, E4M3 ? 1 : kMaxWide);
+  auto kernel = paged_attn_kernel<T, E4M3, DP, TMA>;
+  static unsigned long long flags = 0;
+  if (first_time_on_device(&flags) &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM) !=
+          cudaSuccess)
+    return set_error(SP_ERR_LAUNCH, "paged attention: shared memory attribute: %s",
+                     cudaGetErrorString(cudaGetLastError()));
+  const int blocks = num_sms();
+  return launch_overlapped("paged attention", kernel, blocks, G::THREADS, G::SMEM, s, a, h->kmap,
+                           h->vmap);
 }
 
 template <typename T, bool E4M3, int DP>
-int launch_attn(const AttnArgs& a, cudaStream_t s) {
-  using G = Geo<T, E4M3, DP>;
-  static unsigned long long flags = 0;
-  if (first_time_on_device(&flags) &&
-      cudaFuncSetAttribute(paged_attn_kernel<T, E4M3, DP>,
-                           cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM) != cudaSuccess)
-    return set_error(SP_ERR_LAUNCH, "paged attention: shared memory attribute: %s",
-                     cudaGetErrorString(cudaGetLastError()));
-  paged_attn_kernel<T, E4M3, DP>
-      <<<num_sms() * G::PER_SM, kWarps * 32, G::SMEM, s>>>(a);
-  return check_launch("paged attention");
+int launch_attn(const AttnArgs& a, const CacheHandle* h, cudaStream_t s) {
+  return h->tma ? launch_attn_tma<T, E4M3, DP, true>(a, h, s)
+                : launch_attn_tma<T, E4M3, DP, false>(a, h, s);
 }
 
 template <typename T, bool E4M3>
-int launch_attn_d(const AttnArgs& a, cudaStream_t s) {
-  if (a.D <= 64) return launch_attn<T, E4M3, 64>(a, s);
-  if (a.D <= 128) return launch_attn<T, E4M3, 128>(a, s);
-  return launch_attn<T, E4M3, 256>(a, s);
+int launch_attn_d(const AttnArgs& a, const CacheHandle* h, cudaStream_t s) {
+  if constexpr (!E4M3)
+    if (a.D <= 64) return launch_attn<T, E4M3, 64>(a, h, s);
+  if (a.D <= 128) return launch_attn<T, E4M3, 128>(a, h, s);
+  return launch_attn<T, E4M3, 256>(a, h, s);
 }
 
-// The workspace: the parts of the blocks (two slots each) at the largest that blocks per SM and
-// head dim make them, then the counters.  The place of the counters depends on the device alone, so that calls of different
-// sizes can share a workspace without one's parts on another's counters.
-size_t parts_bytes() { return (size_t)num_sms() * 2 * 16 * 2 * (128 + 2) * sizeof(float); }
-static_assert(3 * (64 + 2) <= 2 * (128 + 2) && 256 + 2 <= 2 * (128 + 2), "the parts fit");
+// The workspace: the counters, then the blocks' parts (two slots each).
+constexpr int kItems = 1 << 18;  // of a launch, at most
+int64_t part_floats_of(int64_t rows, int64_t D) { return (rows * (D + 2) + 3) / 4 * 4; }
+size_t workspace_bytes_of(int64_t rows, int64_t D) {
+  return kItems * sizeof(int32_t) +
+         (size_t)num_sms() * 2 * kMaxWide * (size_t)part_floats_of(rows, D) * sizeof(float);
+}
 }  // namespace
 }  // namespace sp
 
-extern "C" size_t sp_paged_attention_workspace_size(int64_t B, int64_t hq, int64_t hkv) {
-  if (B <= 0 || hkv <= 0 || hq <= 0 || hq % hkv) return 0;
-  return sp::parts_bytes() + (size_t)B * hkv * ((hq / hkv + 15) / 16) * sizeof(int32_t);
+extern "C" size_t sp_paged_attention_workspace_size(int64_t hq, int64_t hkv, int64_t D) {
+  if (hkv <= 0 || hq <= 0 || hq % hkv || D <= 0) return 0;
+  const int64_t group = hq / hkv;
+  return sp::workspace_bytes_of(group < 16 ? group : 16, D);
 }
 
 extern "C" int sp_paged_attention(const void* cache, const void* q, int64_t q_seq_stride,
@@ -712,10 +980,11 @@ extern "C" int sp_paged_attention(const void* cache, const void* q, int64_t q_se
       !aligned(seq_lens, 4))
     return set_error(SP_ERR_ALIGN, "paged attention: q heads must be 4-byte aligned, out 16-byte");
   if (B == 0) return SP_OK;
-  if (B * hkv * ((hq / hkv + 15) / 16) > (1LL << 30))
-    return set_error(SP_ERR_SHAPE, "paged attention: too many sequences x heads");
+  const int64_t group = hq / hkv, vheads = hkv * ((group + 15) / 16);
+  if (vheads > kItems)
+    return set_error(SP_ERR_SHAPE, "paged attention: more than %d heads", kItems);
   if (int rc = require_sm100()) return rc;
-  if (!workspace || workspace_bytes < sp_paged_attention_workspace_size(B, hq, hkv))
+  if (!workspace || workspace_bytes < sp_paged_attention_workspace_size(hq, hkv, h->D))
     return set_error(SP_ERR_WORKSPACE, "paged attention: workspace missing or too small");
   if (!aligned(workspace, 16))
     return set_error(SP_ERR_ALIGN, "paged attention: workspace must be 16-byte aligned");
@@ -730,19 +999,37 @@ extern "C" int sp_paged_attention(const void* cache, const void* q, int64_t q_se
   for (int i = 0; i < 6; i += 3)  // a slot's and head's offset within the page
     if ((h->page_size - 1) * (st[i + 1] * es / 16) + (hkv - 1) * (st[i + 2] * es / 16) > 0xffffffffLL)
       return set_error(SP_ERR_SHAPE, "paged attention: a page spans more than 64 GB");
-  a.q = q, a.out = out;
-  a.lens = static_cast<const int32_t*>(seq_lens);
   a.q_seq = q_seq_stride, a.q_head = q_head_stride;
-  a.B = (int32_t)B, a.hq = (int32_t)hq, a.hkv = (int32_t)hkv, a.D = h->D;
-  a.group = (int32_t)(hq / hkv), a.row_blocks = (a.group + 15) / 16;
+  a.hq = (int32_t)hq, a.hkv = (int32_t)hkv, a.D = h->D;
+  a.group = (int32_t)group, a.row_blocks = (int32_t)((group + 15) / 16);
+  a.vheads = (int32_t)vheads, a.part_rows = (int32_t)(group < 16 ? group : 16);
+  a.part_floats = (int32_t)part_floats_of(a.part_rows, h->D);
   a.window = (int32_t)window, a.sinks = (int32_t)sinks;
   a.scale_log2 = (scale > 0.f ? scale : 1.f / sqrtf((float)h->D)) * 1.4426950408889634f;
-  a.parts = static_cast<float*>(workspace);
-  a.counters = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + parts_bytes());
+  a.counters = static_cast<int32_t*>(workspace);
+  a.parts = reinterpret_cast<float*>(a.counters + kItems);
+  const int32_t* table = a.c.table;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (h->dtype == SP_E4M3)
-    return dtype == SP_F16 ? launch_attn_d<__half, true>(a, s)
-                           : launch_attn_d<__nv_bfloat16, true>(a, s);
-  return dtype == SP_F16 ? launch_attn_d<__half, false>(a, s)
-                         : launch_attn_d<__nv_bfloat16, false>(a, s);
+  // sequences of a launch: the item table holds theirs, and steps count in 31 bits
+  const int64_t granules = (table_cols * h->page_size + 7) / 8;
+  if (granules * vheads > 2147483647LL - 65536)
+    return set_error(SP_ERR_SHAPE, "paged attention: a sequence of too many tokens x heads");
+  const int64_t most = kItems / vheads < (2147483647LL - 65536) / (granules * vheads)
+                           ? kItems / vheads : (2147483647LL - 65536) / (granules * vheads);
+  for (int64_t b = 0; b < B; b += most) {
+    a.B = (int32_t)(B - b < most ? B - b : most);
+    a.q = static_cast<const uint8_t*>(q) + b * q_seq_stride * 2;
+    a.out = static_cast<uint8_t*>(out) + b * hq * h->D * 2;
+    a.lens = static_cast<const int32_t*>(seq_lens) + b;
+    a.c.table = table + b * table_stride;
+    int rc;
+    if (h->dtype == SP_E4M3)
+      rc = dtype == SP_F16 ? launch_attn_d<__half, true>(a, h, s)
+                           : launch_attn_d<__nv_bfloat16, true>(a, h, s);
+    else
+      rc = dtype == SP_F16 ? launch_attn_d<__half, false>(a, h, s)
+                           : launch_attn_d<__nv_bfloat16, false>(a, h, s);
+    if (rc) return rc;
+  }
+  return SP_OK;
 }

@@ -28,6 +28,10 @@ struct CacheHandle {
   int64_t page_size;
   int32_t hkv, D;
   int dtype;
+  // [pages, heads, slots, D], boxes of 8 slots x 128 bytes, 128-byte swizzle; `tma`: they exist
+  // and the page size is a multiple of 8
+  CUtensorMap kmap, vmap;
+  bool tma;
 };
 
 // The block table of one call joins the handle's cache; fills c.

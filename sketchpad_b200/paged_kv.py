@@ -15,7 +15,7 @@ The cache holds bf16 or f16, or e4m3 values times a scale per head.
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, Optional, Tuple
+from typing import Dict, Optional
 
 import torch
 
@@ -53,7 +53,7 @@ class PagedKVCache:
             raise TypeError("the cache holds bf16, f16 or float8_e4m3fn")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.page_size, self.kv_heads, self.head_dim = k.shape
-        self._work_bytes: Dict[Tuple[int, int], int] = {}
+        self._work_bytes: Dict[int, int] = {}
         self._handle = ctypes.c_void_p()
         _lib.call("sp_paged_cache_create", ptr(k), ptr(v), ptr(k_scale), ptr(v_scale),
                   _lib.i64_array(k.stride()), _lib.i64_array(v.stride()), *k.shape, self._code,
@@ -139,13 +139,13 @@ class PagedKVCache:
                 raw_stream(index))
         return q_out
 
-    def workspace_size(self, batch: int, heads: int) -> int:
-        """Bytes of the workspace of an `attend` call."""
-        return _lib.load().sp_paged_attention_workspace_size(batch, heads, self.kv_heads)
+    def workspace_size(self, heads: int) -> int:
+        """Bytes of the workspace of an `attend` call of `heads` query heads."""
+        return _lib.load().sp_paged_attention_workspace_size(heads, self.kv_heads, self.head_dim)
 
-    def new_workspace(self, batch: int, heads: int) -> torch.Tensor:
-        """A workspace for `attend` calls of up to `batch` sequences and `heads` query heads."""
-        return torch.zeros((self.workspace_size(batch, heads) + 3) // 4, dtype=torch.int32,
+    def new_workspace(self, heads: int) -> torch.Tensor:
+        """A workspace for `attend` calls of `heads` query heads, of any batch."""
+        return torch.zeros((self.workspace_size(heads) + 3) // 4, dtype=torch.int32,
                            device=self.device)
 
     def attend(self, q: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, *,
@@ -186,9 +186,9 @@ class PagedKVCache:
         q, q_ptr, q_seq, q_head = _heads(q)
         stream = raw_stream(index)
         if workspace is None:
-            need = self._work_bytes.get((B, hq))
+            need = self._work_bytes.get(hq)
             if need is None:
-                need = self._work_bytes[B, hq] = self.workspace_size(B, hq)
+                need = self._work_bytes[hq] = self.workspace_size(hq)
             work = _workspaces.get(index, stream, need)
         else:
             work = (workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size())
