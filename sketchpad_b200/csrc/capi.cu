@@ -55,14 +55,17 @@ int check_launch(const char* what) {
 }
 
 int require_sm100() {
+  static signed char known[64] = {};  // 1: sm_100
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return set_error(SP_ERR_DEVICE, "no CUDA device");
+  if (dev >= 0 && dev < 64 && __atomic_load_n(&known[dev], __ATOMIC_RELAXED) == 1) return SP_OK;
   int major = 0, minor = 0;
   cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
   cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
   if (major != 10 || minor != 0)
     return set_error(SP_ERR_DEVICE, "device %d is sm_%d%d; this library is built for sm_100a",
                      dev, major, minor);
+  if (dev >= 0 && dev < 64) __atomic_store_n(&known[dev], (signed char)1, __ATOMIC_RELAXED);
   return SP_OK;
 }
 

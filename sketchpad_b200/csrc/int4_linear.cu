@@ -303,6 +303,8 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int
   float* xsum = reinterpret_cast<float*>(smem + R::BLOCK);
   uint8_t* xsm = smem + R::BLOCK + cs * GPC * TM * 8;
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
   // ---- the copy side: the next chunk to copy
   int ft = tile0, fc = gw;
   if (gw >= cs) ft = n_tiles;  // nothing for this warp
@@ -327,8 +329,11 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // The weights do not come from the kernel before (a repack is not launched so as to overlap),
+  // so they are on their way while it ends; everything else waits for it.
 #pragma unroll
   for (int u = 0; u < kI4Deep - 1; ++u) fetch(ring + u * R::STAGE);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- the slab of x: row m at m * (256 cs + 64) bytes (64 so that two rows' 64-byte pieces
   // fall into different halves of the banks)
@@ -679,8 +684,7 @@ int launch_int4(Int4Args a, cudaStream_t s) {
                      cudaGetErrorString(cudaGetLastError()));
   const Int4Plan p = int4_plan(a.M, a.N, a.C, GPC, Ring<GPC, ZP>::BLOCK);
   a.S = p.S, a.cs = p.cs, a.U = p.U;
-  kernel<<<p.blocks, kI4Warps * 32, p.smem, s>>>(a);
-  return check_launch("int4 linear");
+  return launch_overlapped("int4 linear", kernel, p.blocks, kI4Warps * 32, p.smem, s, a);
 }
 
 template <int NT, int GPC>

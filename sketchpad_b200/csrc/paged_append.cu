@@ -7,8 +7,8 @@
 //
 // Bound by HBM for prompts (q read and written, k and v read and written once) and by latency
 // for single tokens.  One block per token: a thread owns eight values at one place of a head
-// and walks the heads, so the token's position, page and (cos, sin) pairs are loaded once for
-// all of its heads.
+// and walks the heads, four at a time, so the token's position, page and (cos, sin) pairs are
+// loaded once for all of its heads, and the first heads' values while those are looked up.
 #include <new>
 
 #include "common.cuh"
@@ -19,6 +19,7 @@ namespace sp {
 namespace {
 
 constexpr int kAppThreads = 256;
+constexpr int kAppHeads = 4;  // heads of a thread whose loads are under way together
 
 struct AppendArgs {
   PagedCache c;
@@ -43,15 +44,41 @@ struct V8 {
 // padding: nothing of it enters the cache, and its q comes out as zeros.
 template <typename T, bool E4M3>
 __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t t = blockIdx.x;
   const int lanes = a.D >> 3;                   // threads per head
   const int slots = kAppThreads / lanes;        // heads in flight
-  const int lane = threadIdx.x % lanes, slot = threadIdx.x / lanes;
+  const int slot = threadIdx.x / lanes, lane = threadIdx.x - slot * lanes;
   if (slot >= slots) return;
-  const int heads = a.hq + 2 * a.hkv;
+  const int heads = a.hq + 2 * a.hkv, d0 = lane * 8;
+  const T* q = static_cast<const T*>(a.q) + t * a.q_tok + d0;
+  const T* k = static_cast<const T*>(a.k) + t * a.k_tok + d0;
+  const T* v = static_cast<const T*>(a.v) + t * a.v_tok + d0;
+  V8<T> x[kAppHeads];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < kAppHeads; ++u) {
+      const int h = h0 + u * slots, hk = h - a.hq;
+      if (h < heads) {
+        const T* src = hk < 0        ? q + h * a.q_head
+                       : hk < a.hkv ? k + hk * a.k_head
+                                    : v + (hk - a.hkv) * a.v_head;
+        *reinterpret_cast<uint4*>(&x[u]) = *reinterpret_cast<const uint4*>(src);
+      }
+    }
+  };
+  load(slot);
   const int32_t seq = a.seq_ids[t], pos = a.positions[t];
   bool live = pos >= 0 && seq >= 0 && seq < a.c.table_rows;
   if (a.rope) live = live && pos < a.rope_rows;
+  float cs[8] = {1.f, 0.f, 1.f, 0.f, 1.f, 0.f, 1.f, 0.f};
+  if (a.rope && live) {
+    const float4* r = reinterpret_cast<const float4*>(a.rope + (int64_t)pos * (a.D >> 1)) + 2 * lane;
+    const float4 r0 = __ldg(r), r1 = __ldg(r + 1);
+    cs[0] = r0.x, cs[1] = r0.y, cs[2] = r0.z, cs[3] = r0.w;
+    cs[4] = r1.x, cs[5] = r1.y, cs[6] = r1.z, cs[7] = r1.w;
+  }
   int32_t page = -1, in_page = 0;
   if (live) {
     const int32_t col = a.c.page_size.div(pos);
@@ -60,62 +87,50 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendA
     if (live) page = a.c.table[seq * a.c.table_stride + col];
     live = live && page >= 0 && page < a.c.pages;
   }
-  float cs[8];
-  if (a.rope && live) {
-    const float4* r = reinterpret_cast<const float4*>(a.rope + (int64_t)pos * (a.D >> 1)) + 2 * lane;
-    const float4 r0 = __ldg(r), r1 = __ldg(r + 1);
-    cs[0] = r0.x, cs[1] = r0.y, cs[2] = r0.z, cs[3] = r0.w;
-    cs[4] = r1.x, cs[5] = r1.y, cs[6] = r1.z, cs[7] = r1.w;
-  }
-  const int d0 = lane * 8;
-  for (int h = slot; h < heads; h += slots) {
-    const bool is_q = h < a.hq;
-    const bool is_k = !is_q && h < a.hq + a.hkv;
-    const int hk = h - a.hq - (is_k ? 0 : a.hkv);
-    if (!live) {
-      if (is_q)
-        reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (t * a.hq + h) * a.D + d0)[0] =
-            make_uint4(0, 0, 0, 0);
-      continue;
-    }
-    const T* src = is_q   ? static_cast<const T*>(a.q) + t * a.q_tok + h * a.q_head
-                   : is_k ? static_cast<const T*>(a.k) + t * a.k_tok + hk * a.k_head
-                          : static_cast<const T*>(a.v) + t * a.v_tok + hk * a.v_head;
-    V8<T> x;
-    *reinterpret_cast<uint4*>(&x) = *reinterpret_cast<const uint4*>(src + d0);
-    float f[8];
+  const int64_t k_at = page * a.c.k_page + in_page * a.c.k_slot + d0;
+  const int64_t v_at = page * a.c.v_page + in_page * a.c.v_slot + d0;
+  for (int h0 = slot; h0 < heads; h0 += kAppHeads * slots) {
+    if (h0 != slot) load(h0);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f32(x.e[i]);
-    if (a.rope && (is_q || is_k)) {
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        const float x0 = f[i], x1 = f[i + 1];
-        f[i] = x0 * cs[i] - x1 * cs[i + 1];
-        f[i + 1] = x1 * cs[i] + x0 * cs[i + 1];
+    for (int u = 0; u < kAppHeads; ++u) {
+      const int h = h0 + u * slots;
+      if (h >= heads) break;
+      const bool is_q = h < a.hq, is_v = h >= a.hq + a.hkv;
+      const int hk = h - a.hq - (is_v ? a.hkv : 0);
+      if (!live) {
+        if (is_q)
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (t * a.hq + h) * a.D + d0) =
+              make_uint4(0, 0, 0, 0);
+        continue;
       }
-    }
-    if (E4M3 && !is_q) {
-      const float s = is_k ? a.c.k_scale[hk] : a.c.v_scale[hk];
-      uint16_t o[4];
+      float f[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = e4m3x2_from_f32(f[2 * i] / s, f[2 * i + 1] / s);
-      const int64_t at = is_k ? page * a.c.k_page + in_page * a.c.k_slot + hk * a.c.k_head
-                              : page * a.c.v_page + in_page * a.c.v_slot + hk * a.c.v_head;
-      uint8_t* dst = static_cast<uint8_t*>(is_k ? a.c.k : a.c.v) + at + d0;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(o[0] | (uint32_t)o[1] << 16,
-                                                  o[2] | (uint32_t)o[3] << 16);
-    } else {
+      for (int i = 0; i < 8; ++i) f[i] = to_f32(x[u].e[i]);
+      if (a.rope && !is_v) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x.e[i] = from_f32<T>(f[i]);
-      T* dst;
-      if (is_q) {
-        dst = static_cast<T*>(a.q_out) + (t * a.hq + h) * a.D;
+        for (int i = 0; i < 8; i += 2) {
+          const float x0 = f[i], x1 = f[i + 1];
+          f[i] = x0 * cs[i] - x1 * cs[i + 1];
+          f[i + 1] = x1 * cs[i] + x0 * cs[i + 1];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[u].e[i] = from_f32<T>(f[i]);
+      }
+      if (E4M3 && !is_q) {
+        const float inv = 1.f / (is_v ? a.c.v_scale[hk] : a.c.k_scale[hk]);
+        uint16_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = e4m3x2_from_f32(f[2 * i] * inv, f[2 * i + 1] * inv);
+        uint8_t* dst = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) +
+                       (is_v ? v_at + hk * a.c.v_head : k_at + hk * a.c.k_head);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(o[0] | (uint32_t)o[1] << 16,
+                                                    o[2] | (uint32_t)o[3] << 16);
       } else {
-        const int64_t at = is_k ? page * a.c.k_page + in_page * a.c.k_slot + hk * a.c.k_head
-                                : page * a.c.v_page + in_page * a.c.v_slot + hk * a.c.v_head;
-        dst = static_cast<T*>(is_k ? a.c.k : a.c.v) + at;
+        T* dst = is_q   ? static_cast<T*>(a.q_out) + (t * a.hq + h) * a.D + d0
+                 : is_v ? static_cast<T*>(a.c.v) + v_at + hk * a.c.v_head
+                        : static_cast<T*>(a.c.k) + k_at + hk * a.c.k_head;
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(&x[u]);
       }
-      *reinterpret_cast<uint4*>(dst + d0) = *reinterpret_cast<uint4*>(&x);
     }
   }
 }
@@ -246,12 +261,11 @@ extern "C" int sp_paged_kv_append(const void* cache, const void* q, const void* 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned grid = (unsigned)tokens;
   const bool f8 = h->dtype == SP_E4M3;
-  if (dtype == SP_F16) {
-    if (f8) paged_append_kernel<__half, true><<<grid, kAppThreads, 0, s>>>(a);
-    else paged_append_kernel<__half, false><<<grid, kAppThreads, 0, s>>>(a);
-  } else {
-    if (f8) paged_append_kernel<__nv_bfloat16, true><<<grid, kAppThreads, 0, s>>>(a);
-    else paged_append_kernel<__nv_bfloat16, false><<<grid, kAppThreads, 0, s>>>(a);
-  }
-  return check_launch("paged append");
+  auto run = [&](auto kernel) {
+    return launch_overlapped("paged append", kernel, grid, kAppThreads, 0, s, a);
+  };
+  if (dtype == SP_F16)
+    return f8 ? run(paged_append_kernel<__half, true>) : run(paged_append_kernel<__half, false>);
+  return f8 ? run(paged_append_kernel<__nv_bfloat16, true>)
+            : run(paged_append_kernel<__nv_bfloat16, false>);
 }

@@ -6,9 +6,10 @@
 //   e4m3: s = max|y| / 448 (1 when the row is all zero), q = e4m3(y / s)
 //
 // Bound by HBM: a row is read once, held in registers across the two block reductions (sum of
-// squares, then max|y|), and written once.  One block per row: with 16-byte vectors a thread
-// holds one to eight of them, so a block has just the threads that its row needs and several
-// rows share an SM, one loading while another reduces.  All arithmetic is f32.
+// squares, then max|y|), and written once.  A block has just the threads that a row needs, a
+// few 16-byte vectors each, and several blocks share an SM.  The blocks walk the rows: the
+// weights stay in registers, and the next row's loads are under way while this one is reduced.
+// All arithmetic is f32.
 #include "common.cuh"
 #include "numeric.cuh"
 
@@ -23,7 +24,7 @@ struct RmsArgs {
   void* res_out;     // or null
   float* scale;      // e4m3 only
   int64_t x_stride, res_stride;  // elements
-  int n;
+  int rows, n;
   float eps;
 };
 
@@ -84,94 +85,97 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, VE>& v) {
 }
 
 // The row in registers: VPT vectors of VE elements per thread, n <= VPT * VE * blockDim.x and
-// n a multiple of VE.  A thread reads its elements before it writes them, so y may be x and
+// n a multiple of VE.  A row is read whole before any of it is written, so y may be x and
 // res_out may be x or residual.
-template <typename T, int VE, int VPT, bool FP8>
-__global__ void __launch_bounds__(1024) rms_reg_kernel(const RmsArgs a) {
-  __shared__ float sum_slots[33], max_slots[33];
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-  const T* res = a.res ? static_cast<const T*>(a.res) + row * a.res_stride : nullptr;
+template <typename T, int VE, int VPT, bool FP8, int THREADS>
+__global__ void __launch_bounds__(THREADS) rms_reg_kernel(const RmsArgs a) {
+  __shared__ float sum_slots[2][33], max_slots[2][33];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const bool has_res = a.res != nullptr, has_w = a.w != nullptr;
   const T* w = static_cast<const T*>(a.w);
   const int step = blockDim.x * VE;
   Vec<T, VE> v[VPT], rv[VPT], wv[VPT];
+  auto load = [&](int row) {
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* res = static_cast<const T*>(a.res) + (has_res ? row * a.res_stride : 0);
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int i = threadIdx.x * VE + j * step;
-    if (i < a.n) {
-      load_vec(v[j], x + i);
-      if (res) load_vec(rv[j], res + i);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int i = threadIdx.x * VE + j * step;
-    if (i < a.n && w) load_vec(wv[j], w + i);
-  }
-  float ss = 0.f;
-#pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int i = threadIdx.x * VE + j * step;
-    if (i < a.n) {
-#pragma unroll
-      for (int t = 0; t < VE; ++t) {
-        if (res) v[j].e[t] = from_f32<T>(to_f32(v[j].e[t]) + to_f32(rv[j].e[t]));
-        const float f = to_f32(v[j].e[t]);
-        ss += f * f;
+    for (int j = 0; j < VPT; ++j) {
+      const int i = threadIdx.x * VE + j * step;
+      if (i < a.n) {
+        load_vec(v[j], x + i);
+        if (has_res) load_vec(rv[j], res + i);
       }
-      if (a.res_out)
-        store_vec(static_cast<T*>(a.res_out) + row * a.n + i, v[j]);
     }
+  };
+  load(blockIdx.x);
+#pragma unroll
+  for (int j = 0; j < VPT; ++j) {
+    const int i = threadIdx.x * VE + j * step;
+    if (i < a.n && has_w) load_vec(wv[j], w + i);
   }
-  const float rstd = rsqrtf(block_reduce<false>(ss, sum_slots) / (float)a.n + a.eps);
-  if constexpr (!FP8) {
-    T* y = static_cast<T*>(a.y) + row * a.n;
+  // two sets of slots in turn: a row's reductions do not wait for the last row's readers
+  for (int row = blockIdx.x, turn = 0; row < a.rows; row += gridDim.x, turn ^= 1) {
+    Vec<T, VE> r[VPT];
+    float ss = 0.f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int i = threadIdx.x * VE + j * step;
       if (i < a.n) {
 #pragma unroll
-        for (int t = 0; t < VE; ++t)
-          v[j].e[t] = from_f32<T>(to_f32(v[j].e[t]) * rstd * (w ? to_f32(wv[j].e[t]) : 1.f));
-        store_vec(y + i, v[j]);
+        for (int t = 0; t < VE; ++t) {
+          r[j].e[t] = has_res ? from_f32<T>(to_f32(v[j].e[t]) + to_f32(rv[j].e[t])) : v[j].e[t];
+          const float f = to_f32(r[j].e[t]);
+          ss += f * f;
+        }
+        if (a.res_out) store_vec(static_cast<T*>(a.res_out) + (int64_t)row * a.n + i, r[j]);
       }
     }
-  } else {
-    float amax = 0.f;
+    if (row + gridDim.x < a.rows) load(row + gridDim.x);
+    const float rstd = rsqrtf(block_reduce<false>(ss, sum_slots[turn]) / (float)a.n + a.eps);
+    auto y_at = [&](int j, int t) {
+      return to_f32(r[j].e[t]) * rstd * (has_w ? to_f32(wv[j].e[t]) : 1.f);
+    };
+    if constexpr (!FP8) {
+      T* y = static_cast<T*>(a.y) + (int64_t)row * a.n;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int i = threadIdx.x * VE + j * step;
-      if (i < a.n) {
+      for (int j = 0; j < VPT; ++j) {
+        const int i = threadIdx.x * VE + j * step;
+        if (i < a.n) {
 #pragma unroll
-        for (int t = 0; t < VE; ++t)
-          amax = max_nan(amax, fabsf(to_f32(v[j].e[t]) * rstd * (w ? to_f32(wv[j].e[t]) : 1.f)));
+          for (int t = 0; t < VE; ++t) r[j].e[t] = from_f32<T>(y_at(j, t));
+          store_vec(y + i, r[j]);
+        }
       }
-    }
-    amax = block_reduce<true>(amax, max_slots);
-    const float s = row_scale(amax);
-    const float inv = 1.f / s;
-    if (threadIdx.x == 0) a.scale[row] = s;
-    uint8_t* q = static_cast<uint8_t*>(a.y) + row * a.n;
+    } else {
+      float amax = 0.f;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int i = threadIdx.x * VE + j * step;
-      if (i < a.n) {
-        if constexpr (VE == 8) {
-          uint16_t o[4];
+      for (int j = 0; j < VPT; ++j) {
+        const int i = threadIdx.x * VE + j * step;
+        if (i < a.n) {
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            const float f0 = to_f32(v[j].e[2 * t]) * rstd * (w ? to_f32(wv[j].e[2 * t]) : 1.f);
-            const float f1 =
-                to_f32(v[j].e[2 * t + 1]) * rstd * (w ? to_f32(wv[j].e[2 * t + 1]) : 1.f);
-            o[t] = e4m3x2_from_f32(f0 * inv, f1 * inv);
-          }
-          *reinterpret_cast<uint2*>(q + i) = make_uint2(o[0] | (uint32_t)o[1] << 16,
-                                                        o[2] | (uint32_t)o[3] << 16);
-        } else {
+          for (int t = 0; t < VE; ++t) amax = max_nan(amax, fabsf(y_at(j, t)));
+        }
+      }
+      amax = block_reduce<true>(amax, max_slots[turn]);
+      const float s = row_scale(amax);
+      const float inv = 1.f / s;
+      if (threadIdx.x == 0) a.scale[row] = s;
+      uint8_t* q = static_cast<uint8_t*>(a.y) + (int64_t)row * a.n;
 #pragma unroll
-          for (int t = 0; t < VE; ++t) {
-            const float f = to_f32(v[j].e[t]) * rstd * (w ? to_f32(wv[j].e[t]) : 1.f);
-            q[i + t] = (uint8_t)e4m3x2_from_f32(f * inv, 0.f);
+      for (int j = 0; j < VPT; ++j) {
+        const int i = threadIdx.x * VE + j * step;
+        if (i < a.n) {
+          if constexpr (VE == 8) {
+            uint16_t o[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              o[t] = e4m3x2_from_f32(y_at(j, 2 * t) * inv, y_at(j, 2 * t + 1) * inv);
+            *reinterpret_cast<uint2*>(q + i) = make_uint2(o[0] | (uint32_t)o[1] << 16,
+                                                          o[2] | (uint32_t)o[3] << 16);
+          } else {
+#pragma unroll
+            for (int t = 0; t < VE; ++t) q[i + t] = (uint8_t)e4m3x2_from_f32(y_at(j, t) * inv, 0.f);
           }
         }
       }
@@ -186,6 +190,8 @@ __global__ void __launch_bounds__(1024) rms_reg_kernel(const RmsArgs a) {
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(1024) rms_long_kernel(const RmsArgs a) {
   __shared__ float sum_slots[33], max_slots[33];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
   const T* res = a.res ? static_cast<const T*>(a.res) + row * a.res_stride : nullptr;
@@ -227,20 +233,24 @@ int launch_rms(const RmsArgs& a, int64_t rows, cudaStream_t s) {
                    aligned(a.res_out, 16) && aligned(a.y, FP8 ? 8 : 16) &&
                    (a.x_stride * es) % 16 == 0 &&
                    (!a.res || (aligned(a.res, 16) && (a.res_stride * es) % 16 == 0));
-  const unsigned grid = (unsigned)rows;
-  auto threads = [](int items) { return (unsigned)((items + 31) / 32 * 32); };
+  // blocks that share an SM: by threads, three quarters of the most it can hold
+  auto run = [&](auto kernel, int items) {
+    const unsigned threads = (unsigned)((items + 31) / 32 * 32);
+    const int64_t most = (int64_t)num_sms() * (threads >= 1536 ? 1 : 1536 / threads);
+    return launch_overlapped("rms norm", kernel, (unsigned)(rows < most ? rows : most), threads, 0,
+                             s, a);
+  };
   if (vec) {
     const int nv = a.n / 8;
-    if (nv <= 512) rms_reg_kernel<T, 8, 1, FP8><<<grid, threads(nv), 0, s>>>(a);
-    else if (nv <= 1024) rms_reg_kernel<T, 8, 2, FP8><<<grid, threads((nv + 1) / 2), 0, s>>>(a);
-    else if (nv <= 4096) rms_reg_kernel<T, 8, 4, FP8><<<grid, threads((nv + 3) / 4), 0, s>>>(a);
-    else rms_long_kernel<T, FP8><<<grid, 1024, 0, s>>>(a);
+    if (nv <= 512) return run(rms_reg_kernel<T, 8, 1, FP8, 512>, nv);
+    if (nv <= 1024) return run(rms_reg_kernel<T, 8, 2, FP8, 512>, (nv + 1) / 2);
+    if (nv <= 2048) return run(rms_reg_kernel<T, 8, 2, FP8, 1024>, (nv + 1) / 2);
   } else {
-    if (a.n <= 1024) rms_reg_kernel<T, 1, 4, FP8><<<grid, threads((a.n + 3) / 4), 0, s>>>(a);
-    else if (a.n <= 8192) rms_reg_kernel<T, 1, 8, FP8><<<grid, threads((a.n + 7) / 8), 0, s>>>(a);
-    else rms_long_kernel<T, FP8><<<grid, 1024, 0, s>>>(a);
+    if (a.n <= 1024) return run(rms_reg_kernel<T, 1, 4, FP8, 256>, (a.n + 3) / 4);
+    if (a.n <= 4096) return run(rms_reg_kernel<T, 1, 8, FP8, 512>, (a.n + 7) / 8);
+    if (a.n <= 8192) return run(rms_reg_kernel<T, 1, 8, FP8, 1024>, (a.n + 7) / 8);
   }
-  return check_launch("rms norm");
+  return launch_overlapped("rms norm", rms_long_kernel<T, FP8>, (unsigned)rows, 1024u, 0, s, a);
 }
 
 template <bool FP8>
@@ -275,7 +285,7 @@ extern "C" int sp_rms_norm(const void* x, int64_t x_row_stride, const void* resi
                            void* residual_out, int64_t rows, int64_t n, float eps, int dtype,
                            void* stream) {
   const sp::RmsArgs a{x, residual, weight, y, residual_out, nullptr, x_row_stride,
-                      residual_row_stride, (int)n, eps};
+                      residual_row_stride, (int)rows, (int)n, eps};
   return sp::rms_entry<false>(a, rows, n, dtype, stream);
 }
 
@@ -284,6 +294,6 @@ extern "C" int sp_rms_norm_fp8(const void* x, int64_t x_row_stride, const void* 
                                float* scale, void* residual_out, int64_t rows, int64_t n,
                                float eps, int dtype, void* stream) {
   const sp::RmsArgs a{x, residual, weight, q, residual_out, scale, x_row_stride,
-                      residual_row_stride, (int)n, eps};
+                      residual_row_stride, (int)rows, (int)n, eps};
   return sp::rms_entry<true>(a, rows, n, dtype, stream);
 }

@@ -180,7 +180,7 @@ class PagedKVCache:
         if sinks < 0:
             raise ValueError("sinks must not be negative")
         if out is None:
-            out = q.new_empty((B, hq, D))
+            out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, hq, D))
         elif out.shape != (B, hq, D) or out.dtype != q.dtype or not out.is_contiguous():
             raise ValueError(f"out must be contiguous {q.dtype} [{B}, {hq}, {D}]")
         q, q_ptr, q_seq, q_head = _heads(q)

@@ -18,6 +18,11 @@ _norm = _lib.Entry("sp_rms_norm")
 _norm_fp8 = _lib.Entry("sp_rms_norm_fp8")
 
 
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of x's shape and dtype (empty_like keeps x's strides, and is quicker)."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def _rows(t: torch.Tensor, n: int):
     """(t, pointer, row stride) of t as rows of n values (a copy only where t has no such view)."""
     if not t.is_contiguous():
@@ -50,7 +55,7 @@ def _operands(x, weight, residual, residual_out):
             raise ValueError("residual must have x's shape and dtype")
         rr = _rows(residual, n)
         if residual_out is None:
-            residual_out = x.new_empty(shape)
+            residual_out = _like(x)
     if residual_out is not None:
         if residual_out.shape != shape or residual_out.dtype != dtype or \
                 not residual_out.is_contiguous():
@@ -70,7 +75,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6,
     index, rows, n, xr, rr, w_ptr, ro_ptr, residual_out = _operands(x, weight, residual,
                                                                     residual_out)
     if out is None:
-        out = x.new_empty(x.shape)
+        out = _like(x)
     elif out.shape != x.shape or out.dtype != x.dtype or not out.is_contiguous():
         raise ValueError("out must be contiguous and have x's shape and dtype")
     else:
@@ -90,7 +95,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1
     code = dtype_code(x.dtype)
     index, rows, n, xr, rr, w_ptr, ro_ptr, residual_out = _operands(x, weight, residual,
                                                                     residual_out)
-    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    q = (torch.empty_like(x, dtype=torch.float8_e4m3fn) if x.is_contiguous()
+         else x.new_empty(x.shape, dtype=torch.float8_e4m3fn))
     scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     _norm_fp8(xr[1], xr[2], rr[1], rr[2], w_ptr, q.data_ptr(), scale.data_ptr(), ro_ptr, rows, n,
               eps, code, raw_stream(index))
