@@ -7,8 +7,8 @@
 //
 // Bound by HBM for prompts (q read and written, k and v read and written once) and by latency
 // for single tokens.  One block per token: a thread owns eight values at one place of a head
-// and walks the heads, four at a time, so the token's position, page and (cos, sin) pairs are
-// loaded once for all of its heads, and the first heads' values while those are looked up.
+// and walks the heads, so the token's position, page and (cos, sin) pairs are loaded once for
+// all of its heads, and the first heads' values while those are looked up.
 #include <new>
 
 #include "common.cuh"
@@ -19,7 +19,7 @@ namespace sp {
 namespace {
 
 constexpr int kAppThreads = 256;
-constexpr int kAppHeads = 4;  // heads of a thread whose loads are under way together
+constexpr int kAppHeads = 2;  // heads of q of a thread whose loads are under way together
 
 struct AppendArgs {
   PagedCache c;
@@ -35,15 +35,10 @@ struct AppendArgs {
   int32_t hq, hkv, D;
 };
 
-template <typename T>
-struct V8 {
-  T e[8];
-};
-
 // A token outside its sequence (seq id, position, page or rope row that does not exist) is
 // padding: nothing of it enters the cache, and its q comes out as zeros.
 template <typename T, bool E4M3>
-__global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppThreads, 5) paged_append_kernel(const AppendArgs a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t t = blockIdx.x;
@@ -51,24 +46,24 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendA
   const int slots = kAppThreads / lanes;        // heads in flight
   const int slot = threadIdx.x / lanes, lane = threadIdx.x - slot * lanes;
   if (slot >= slots) return;
-  const int heads = a.hq + 2 * a.hkv, d0 = lane * 8;
+  const int d0 = lane * 8;
   const T* q = static_cast<const T*>(a.q) + t * a.q_tok + d0;
   const T* k = static_cast<const T*>(a.k) + t * a.k_tok + d0;
   const T* v = static_cast<const T*>(a.v) + t * a.v_tok + d0;
-  V8<T> x[kAppHeads];
-  auto load = [&](int h0) {
-#pragma unroll
-    for (int u = 0; u < kAppHeads; ++u) {
-      const int h = h0 + u * slots, hk = h - a.hq;
-      if (h < heads) {
-        const T* src = hk < 0        ? q + h * a.q_head
-                       : hk < a.hkv ? k + hk * a.k_head
-                                    : v + (hk - a.hkv) * a.v_head;
-        *reinterpret_cast<uint4*>(&x[u]) = *reinterpret_cast<const uint4*>(src);
-      }
-    }
+  // head h of k and then v; kAppHeads heads of q
+  auto load_kv = [&](int h) {
+    const T* src = h < a.hkv ? k + h * a.k_head : v + (h - a.hkv) * a.v_head;
+    return *reinterpret_cast<const uint4*>(src);
   };
-  load(slot);
+  uint4 kv, qx[kAppHeads];
+  auto load_q = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < kAppHeads; ++u)
+      if (h0 + u * slots < a.hq)
+        qx[u] = *reinterpret_cast<const uint4*>(q + (h0 + u * slots) * a.q_head);
+  };
+  load_q(slot);
+  if (slot < 2 * a.hkv) kv = load_kv(slot);
   const int32_t seq = a.seq_ids[t], pos = a.positions[t];
   bool live = pos >= 0 && seq >= 0 && seq < a.c.table_rows;
   if (a.rope) live = live && pos < a.rope_rows;
@@ -87,50 +82,67 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendA
     if (live) page = a.c.table[seq * a.c.table_stride + col];
     live = live && page >= 0 && page < a.c.pages;
   }
-  const int64_t k_at = page * a.c.k_page + in_page * a.c.k_slot + d0;
-  const int64_t v_at = page * a.c.v_page + in_page * a.c.v_slot + d0;
-  for (int h0 = slot; h0 < heads; h0 += kAppHeads * slots) {
-    if (h0 != slot) load(h0);
+  auto rotate = [&](float (&f)[8], const uint4& x) {
+    const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float x0 = to_f32(e[i]), x1 = to_f32(e[i + 1]);
+      f[i] = x0 * cs[i] - x1 * cs[i + 1];
+      f[i + 1] = x1 * cs[i] + x0 * cs[i + 1];
+    }
+  };
+  auto pack = [&](const float (&f)[8]) {
+    uint4 x;
+    T* e = reinterpret_cast<T*>(&x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(f[i]);
+    return x;
+  };
+
+  T* qo = static_cast<T*>(a.q_out) + t * a.hq * a.D + d0;
+  for (int h0 = slot; h0 < a.hq; h0 += kAppHeads * slots) {
+    if (h0 != slot) load_q(h0);
 #pragma unroll
     for (int u = 0; u < kAppHeads; ++u) {
       const int h = h0 + u * slots;
-      if (h >= heads) break;
-      const bool is_q = h < a.hq, is_v = h >= a.hq + a.hkv;
-      const int hk = h - a.hq - (is_v ? a.hkv : 0);
-      if (!live) {
-        if (is_q)
-          *reinterpret_cast<uint4*>(static_cast<T*>(a.q_out) + (t * a.hq + h) * a.D + d0) =
-              make_uint4(0, 0, 0, 0);
-        continue;
-      }
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = to_f32(x[u].e[i]);
-      if (a.rope && !is_v) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const float x0 = f[i], x1 = f[i + 1];
-          f[i] = x0 * cs[i] - x1 * cs[i + 1];
-          f[i + 1] = x1 * cs[i] + x0 * cs[i + 1];
+      if (h < a.hq) {
+        if (!live) {
+          qx[u] = make_uint4(0, 0, 0, 0);
+        } else if (a.rope) {
+          float f[8];
+          rotate(f, qx[u]);
+          qx[u] = pack(f);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[u].e[i] = from_f32<T>(f[i]);
+        *reinterpret_cast<uint4*>(qo + h * a.D) = qx[u];
       }
-      if (E4M3 && !is_q) {
-        const float inv = 1.f / (is_v ? a.c.v_scale[hk] : a.c.k_scale[hk]);
-        uint16_t o[4];
+    }
+  }
+  if (!live) return;
+  const int64_t k_at = page * a.c.k_page + in_page * a.c.k_slot + d0;
+  const int64_t v_at = page * a.c.v_page + in_page * a.c.v_slot + d0;
+  for (int h = slot; h < 2 * a.hkv; h += slots) {
+    if (h != slot) kv = load_kv(h);
+    const bool is_k = h < a.hkv;
+    const int hk = is_k ? h : h - a.hkv;
+    const int64_t at = is_k ? k_at + hk * a.c.k_head : v_at + hk * a.c.v_head;
+    float f[8];
+    if (is_k && a.rope) {
+      rotate(f, kv);
+      if (!E4M3) kv = pack(f);
+    } else if (E4M3) {
+      const T* e = reinterpret_cast<const T*>(&kv);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = e4m3x2_from_f32(f[2 * i] * inv, f[2 * i + 1] * inv);
-        uint8_t* dst = static_cast<uint8_t*>(is_v ? a.c.v : a.c.k) +
-                       (is_v ? v_at + hk * a.c.v_head : k_at + hk * a.c.k_head);
-        *reinterpret_cast<uint2*>(dst) = make_uint2(o[0] | (uint32_t)o[1] << 16,
-                                                    o[2] | (uint32_t)o[3] << 16);
-      } else {
-        T* dst = is_q   ? static_cast<T*>(a.q_out) + (t * a.hq + h) * a.D + d0
-                 : is_v ? static_cast<T*>(a.c.v) + v_at + hk * a.c.v_head
-                        : static_cast<T*>(a.c.k) + k_at + hk * a.c.k_head;
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(&x[u]);
-      }
+      for (int i = 0; i < 8; ++i) f[i] = to_f32(e[i]);
+    }
+    if constexpr (E4M3) {
+      const float inv = 1.f / (is_k ? a.c.k_scale[hk] : a.c.v_scale[hk]);
+      uint16_t o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = e4m3x2_from_f32(f[2 * i] * inv, f[2 * i + 1] * inv);
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(is_k ? a.c.k : a.c.v) + at) =
+          make_uint2(o[0] | (uint32_t)o[1] << 16, o[2] | (uint32_t)o[3] << 16);
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<T*>(is_k ? a.c.k : a.c.v) + at) = kv;
     }
   }
 }

@@ -5,11 +5,13 @@
 //   y = r / sqrt(mean(r^2) + eps) * w
 //   e4m3: s = max|y| / 448 (1 when the row is all zero), q = e4m3(y / s)
 //
-// Bound by HBM: a row is read once, held in registers across the two block reductions (sum of
-// squares, then max|y|), and written once.  A block has just the threads that a row needs, a
-// few 16-byte vectors each, and several blocks share an SM.  The blocks walk the rows: the
-// weights stay in registers, and the next row's loads are under way while this one is reduced.
-// All arithmetic is f32.
+// Bound by HBM, and close behind by the instructions per element.  A row is read once, held in
+// registers as t = r w in f32 across one block reduction (of the sum of r^2 and of max|t|
+// together: max|y| is max|t| / sqrt(...)), and written once as t / sqrt(...).  A block has just
+// the threads that a row needs, a few 16-byte vectors each, and several blocks share an SM.  The
+// blocks walk the rows: the weights stay in registers, and the next row's loads are under way
+// while this one is reduced.  (Forming y for the maximum and again for the output, with two
+// reductions, took 33 instructions an element and 58 us at 8192 x 5120 bf16.)
 #include "common.cuh"
 #include "numeric.cuh"
 
@@ -28,25 +30,29 @@ struct RmsArgs {
   float eps;
 };
 
-// Sum (or NaN-keeping maximum) over the block; every thread gets it.  `slots`: 33 floats.
+// Sum of `v` and, if MAX, NaN-keeping maximum of `m` over the block; every thread gets them.
+// `slots`: 32 of each.
 template <bool MAX>
-__device__ __forceinline__ float block_reduce(float v, float* slots) {
+__device__ __forceinline__ void block_reduce(float& v, float& m, float (*slots)[32]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? max_nan(v, u) : v + u;
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (MAX) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   }
-  if (nw == 1) return v;
-  if (lane == 0) slots[warp] = v;
+  if (nw == 1) return;
+  if (lane == 0) {
+    slots[0][warp] = v;
+    if (MAX) slots[1][warp] = m;
+  }
   __syncthreads();
-  v = lane < nw ? slots[lane] : 0.f;
+  v = lane < nw ? slots[0][lane] : 0.f;
+  if (MAX) m = lane < nw ? slots[1][lane] : 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? max_nan(v, u) : v + u;
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (MAX) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   }
-  return v;
 }
 
 // The row's e4m3 scale.  Kept a normal number, so that 1 / scale is finite.
@@ -89,7 +95,7 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T, VE>& v) {
 // res_out may be x or residual.
 template <typename T, int VE, int VPT, bool FP8, int THREADS>
 __global__ void __launch_bounds__(THREADS) rms_reg_kernel(const RmsArgs a) {
-  __shared__ float sum_slots[2][33], max_slots[2][33];
+  __shared__ float slots[2][2][32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const bool has_res = a.res != nullptr, has_w = a.w != nullptr;
@@ -114,51 +120,41 @@ __global__ void __launch_bounds__(THREADS) rms_reg_kernel(const RmsArgs a) {
     const int i = threadIdx.x * VE + j * step;
     if (i < a.n && has_w) load_vec(wv[j], w + i);
   }
-  // two sets of slots in turn: a row's reductions do not wait for the last row's readers
+  // two sets of slots in turn: a row's reduction does not wait for the last row's readers
   for (int row = blockIdx.x, turn = 0; row < a.rows; row += gridDim.x, turn ^= 1) {
-    Vec<T, VE> r[VPT];
-    float ss = 0.f;
+    float t[VPT][VE], ss = 0.f, amax = 0.f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int i = threadIdx.x * VE + j * step;
       if (i < a.n) {
 #pragma unroll
-        for (int t = 0; t < VE; ++t) {
-          r[j].e[t] = has_res ? from_f32<T>(to_f32(v[j].e[t]) + to_f32(rv[j].e[t])) : v[j].e[t];
-          const float f = to_f32(r[j].e[t]);
+        for (int e = 0; e < VE; ++e) {
+          if (has_res) v[j].e[e] = from_f32<T>(to_f32(v[j].e[e]) + to_f32(rv[j].e[e]));
+          const float f = to_f32(v[j].e[e]);
           ss += f * f;
+          t[j][e] = has_w ? f * to_f32(wv[j].e[e]) : f;
+          if (FP8) amax = max_nan(amax, fabsf(t[j][e]));
         }
-        if (a.res_out) store_vec(static_cast<T*>(a.res_out) + (int64_t)row * a.n + i, r[j]);
+        if (a.res_out) store_vec(static_cast<T*>(a.res_out) + (int64_t)row * a.n + i, v[j]);
       }
     }
     if (row + gridDim.x < a.rows) load(row + gridDim.x);
-    const float rstd = rsqrtf(block_reduce<false>(ss, sum_slots[turn]) / (float)a.n + a.eps);
-    auto y_at = [&](int j, int t) {
-      return to_f32(r[j].e[t]) * rstd * (has_w ? to_f32(wv[j].e[t]) : 1.f);
-    };
+    block_reduce<FP8>(ss, amax, slots[turn]);
+    const float rstd = rsqrtf(ss / (float)a.n + a.eps);
     if constexpr (!FP8) {
       T* y = static_cast<T*>(a.y) + (int64_t)row * a.n;
 #pragma unroll
       for (int j = 0; j < VPT; ++j) {
         const int i = threadIdx.x * VE + j * step;
         if (i < a.n) {
+          Vec<T, VE> o;
 #pragma unroll
-          for (int t = 0; t < VE; ++t) r[j].e[t] = from_f32<T>(y_at(j, t));
-          store_vec(y + i, r[j]);
+          for (int e = 0; e < VE; ++e) o.e[e] = from_f32<T>(t[j][e] * rstd);
+          store_vec(y + i, o);
         }
       }
     } else {
-      float amax = 0.f;
-#pragma unroll
-      for (int j = 0; j < VPT; ++j) {
-        const int i = threadIdx.x * VE + j * step;
-        if (i < a.n) {
-#pragma unroll
-          for (int t = 0; t < VE; ++t) amax = max_nan(amax, fabsf(y_at(j, t)));
-        }
-      }
-      amax = block_reduce<true>(amax, max_slots[turn]);
-      const float s = row_scale(amax);
+      const float s = row_scale(amax * rstd);
       const float inv = 1.f / s;
       if (threadIdx.x == 0) a.scale[row] = s;
       uint8_t* q = static_cast<uint8_t*>(a.y) + (int64_t)row * a.n;
@@ -169,13 +165,14 @@ __global__ void __launch_bounds__(THREADS) rms_reg_kernel(const RmsArgs a) {
           if constexpr (VE == 8) {
             uint16_t o[4];
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-              o[t] = e4m3x2_from_f32(y_at(j, 2 * t) * inv, y_at(j, 2 * t + 1) * inv);
+            for (int e = 0; e < 4; ++e)
+              o[e] = e4m3x2_from_f32(t[j][2 * e] * rstd * inv, t[j][2 * e + 1] * rstd * inv);
             *reinterpret_cast<uint2*>(q + i) = make_uint2(o[0] | (uint32_t)o[1] << 16,
                                                           o[2] | (uint32_t)o[3] << 16);
           } else {
 #pragma unroll
-            for (int t = 0; t < VE; ++t) q[i + t] = (uint8_t)e4m3x2_from_f32(y_at(j, t) * inv, 0.f);
+            for (int e = 0; e < VE; ++e)
+              q[i + e] = (uint8_t)e4m3x2_from_f32(t[j][e] * rstd * inv, 0.f);
           }
         }
       }
@@ -189,7 +186,7 @@ __global__ void __launch_bounds__(THREADS) rms_reg_kernel(const RmsArgs a) {
 // thread reads and writes only its own elements).
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(1024) rms_long_kernel(const RmsArgs a) {
-  __shared__ float sum_slots[33], max_slots[33];
+  __shared__ float slots[2][32];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t row = blockIdx.x;
@@ -197,27 +194,27 @@ __global__ void __launch_bounds__(1024) rms_long_kernel(const RmsArgs a) {
   const T* res = a.res ? static_cast<const T*>(a.res) + row * a.res_stride : nullptr;
   const T* w = static_cast<const T*>(a.w);
   T* ro = a.res_out ? static_cast<T*>(a.res_out) + row * a.n : nullptr;
-  float ss = 0.f;
+  float ss = 0.f, amax = 0.f;
   for (int i = threadIdx.x; i < a.n; i += blockDim.x) {
     T v = x[i];
     if (res) v = from_f32<T>(to_f32(v) + to_f32(res[i]));
     if (ro) ro[i] = v;
-    ss += to_f32(v) * to_f32(v);
+    const float f = to_f32(v);
+    ss += f * f;
+    if (FP8) amax = max_nan(amax, fabsf(w ? f * to_f32(w[i]) : f));
   }
-  const float rstd = rsqrtf(block_reduce<false>(ss, sum_slots) / (float)a.n + a.eps);
+  block_reduce<FP8>(ss, amax, slots);
+  const float rstd = rsqrtf(ss / (float)a.n + a.eps);
   auto y_at = [&](int i) {
     T v = ro ? ro[i] : x[i];
     if (!ro && res) v = from_f32<T>(to_f32(v) + to_f32(res[i]));
-    return to_f32(v) * rstd * (w ? to_f32(w[i]) : 1.f);
+    return (w ? to_f32(v) * to_f32(w[i]) : to_f32(v)) * rstd;
   };
   if constexpr (!FP8) {
     T* y = static_cast<T*>(a.y) + row * a.n;
     for (int i = threadIdx.x; i < a.n; i += blockDim.x) y[i] = from_f32<T>(y_at(i));
   } else {
-    float amax = 0.f;
-    for (int i = threadIdx.x; i < a.n; i += blockDim.x) amax = max_nan(amax, fabsf(y_at(i)));
-    amax = block_reduce<true>(amax, max_slots);
-    const float s = row_scale(amax);
+    const float s = row_scale(amax * rstd);
     const float inv = 1.f / s;
     if (threadIdx.x == 0) a.scale[row] = s;
     uint8_t* q = static_cast<uint8_t*>(a.y) + row * a.n;
