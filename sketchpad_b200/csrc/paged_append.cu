@@ -19,6 +19,7 @@ namespace sp {
 namespace {
 
 constexpr int kAppThreads = 256;
+constexpr int64_t kAppMany = 1024;
 constexpr int kAppHeads = 2;  // heads of q of a thread whose loads are under way together
 
 struct AppendArgs {
@@ -38,12 +39,12 @@ struct AppendArgs {
 // A token outside its sequence (seq id, position, page or rope row that does not exist) is
 // padding: nothing of it enters the cache, and its q comes out as zeros.
 template <typename T, bool E4M3>
-__global__ void __launch_bounds__(kAppThreads, 5) paged_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppThreads, 4) paged_append_kernel(const AppendArgs a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t t = blockIdx.x;
   const int lanes = a.D >> 3;                   // threads per head
-  const int slots = kAppThreads / lanes;        // heads in flight
+  const int slots = (int)blockDim.x / lanes;    // heads in flight
   const int slot = threadIdx.x / lanes, lane = threadIdx.x - slot * lanes;
   if (slot >= slots) return;
   const int d0 = lane * 8;
@@ -274,7 +275,9 @@ extern "C" int sp_paged_kv_append(const void* cache, const void* q, const void* 
   const unsigned grid = (unsigned)tokens;
   const bool f8 = h->dtype == SP_E4M3;
   auto run = [&](auto kernel) {
-    return launch_overlapped("paged append", kernel, grid, kAppThreads, 0, s, a);
+    // many tokens: fewer threads with more heads each, which share the lookups
+    return launch_overlapped("paged append", kernel, grid,
+                             tokens >= kAppMany ? kAppThreads / 2 : kAppThreads, 0, s, a);
   };
   if (dtype == SP_F16)
     return f8 ? run(paged_append_kernel<__half, true>) : run(paged_append_kernel<__half, false>);
