@@ -43,7 +43,7 @@ constexpr int kI4Warps = 16;
 constexpr int kI4Deep = 3;          // stages of a warp's ring, of a chunk (2 KB) each
 constexpr int kI4Tiles = 1 << 16;   // counters of the workspace: row tiles of a launch
 constexpr int kI4Smem = 226 * 1024; // shared memory of a block (the SM's, but for 1 KB)
-constexpr double kTileCost = 0.5, kSlabCost = 1.0, kWarpTime = 13;  // see int4_plan
+constexpr double kTileCost = 0.5, kSlabCost = 1.0, kWarpTime = 11;  // see int4_plan
 constexpr int kRedRow = 36;         // row of the join: 32 values, 36 apart against bank conflicts
 constexpr int kRedBytes = kI4Warps * 8 * kRedRow * 4;
 
@@ -79,6 +79,9 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
 }
 // t[0..1] += s a[0..1], one instruction
 __device__ __forceinline__ void fma2(float* t, const float* a, float s) {
@@ -261,25 +264,59 @@ __device__ __forceinline__ void store_y(const Int4Args& a, int m, int n, float v
   }
 }
 
-// An accumulator fragment: rows m and m + 1 of x, outputs n and n + 8.
-__device__ __forceinline__ void store_frag(const Int4Args& a, const float (&v)[4], int m, int n,
-                                           int mrows) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (m + (e & 1) < mrows && n + (e >> 1) * 8 < a.N)
-      store_y(a, m + (e & 1), n + (e >> 1) * 8, v[e]);
-}
-
 // Waits for the U warps of group `id` (a warp alone: for its lanes).
 __device__ __forceinline__ void group_sync(int id, int U) {
   if (U == 1) __syncwarp();
   else asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(U * 32) : "memory");
 }
 
+// The end of a tile for eight rows of x: thread gt of the group's 32 U adds up the warps' sums in
+// `gred` for values gt, gt + 32 U, ... (output o & 31 of the tile, row o >> 5 of the eight).
+__device__ __forceinline__ void join_rows(const Int4Args& a, const float* gred, const float* back,
+                                       float* part, int n, int gt, int tile) {
+#pragma unroll 1
+  for (int o = gt; o < 256; o += a.U * 32) {
+    const int m = n * 8 + (o >> 5), row = tile * 32 + (o & 31);
+    const float* p = gred + (o >> 5) * kRedRow + (o & 31);
+    float v = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < a.U; ++k) v += p[k * 8 * kRedRow];
+    v *= back[m];
+    if (a.S > 1) __stcg(part + n * 256 + o, v);
+    else if (m < a.M && row < a.N) store_y(a, m, row, v);
+  }
+}
+
+// The slabs' sums of a tile, in order: float4 o holds four outputs of a row of x.
+__device__ __forceinline__ void join_slabs(const Int4Args& a, const float* parts, int tile_floats,
+                                        int gt, int tile) {
+#pragma unroll 1
+  for (int o = gt; o < tile_floats / 4; o += a.U * 32) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int k0 = 0; k0 < a.S; k0 += 8) {
+      float4 p[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        p[k] = k0 + k < a.S
+                   ? __ldcg(reinterpret_cast<const float4*>(parts + (k0 + k) * tile_floats) + o)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        v[0] += p[k].x, v[1] += p[k].y, v[2] += p[k].z, v[3] += p[k].w;
+    }
+    const int m = o >> 3, row = tile * 32 + (o & 7) * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (m < a.M && row + e < a.N) store_y(a, m, row + e, v[e]);
+  }
+}
+
 // NT: n-tiles of 8 rows of x.  GPC: groups per chunk of 128 inputs (4: groups of 32, 2: of 64,
 // 1: of 128 and more).  ZP: zero points (else 8).  SBF: bf16 scales (else f16).
 template <int NT, int GPC, bool ZP, bool SBF>
-__global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int4Args a) {
+__global__ void __launch_bounds__(kI4Warps * 32, 1)
+    int4_linear_kernel(const __grid_constant__ Int4Args a) {
   using R = Ring<GPC, ZP>;
   constexpr int TM = 8 * NT;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -329,11 +366,20 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  // The weights do not come from the kernel before (a repack is not launched so as to overlap),
-  // so they are on their way while it ends; everything else waits for it.
+  // While the kernel before ends, the first chunks move into the L2 (which that kernel's own
+  // stores would meet there as well); everything is read after the wait.
+  {
+    const int c = gw + (lane >> 4) * U;
+    if (tile0 < n_tiles && c < cs) {
+      const int64_t at = (int64_t)tile0 * a.C + cb + c;
+      prefetch_l2(a.q + at * 2048 + (lane & 15) * 128);
+      if ((lane & 15) * 128 < R::SB) prefetch_l2(a.s + at * R::SB + (lane & 15) * 128);
+      if (ZP && (lane & 15) * 128 < R::ZB) prefetch_l2(a.z + at * R::ZB + (lane & 15) * 128);
+    }
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 #pragma unroll
   for (int u = 0; u < kI4Deep - 1; ++u) fetch(ring + u * R::STAGE);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- the slab of x: row m at m * (256 cs + 64) bytes (64 so that two rows' 64-byte pieces
   // fall into different halves of the banks)
@@ -475,46 +521,20 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int
       xo += U * 256;
     }
 
-    // ---- the tile's end.  A warp alone keeps its values where the MMA left them; a group's
-    // warps join eight rows of x at a time, thread gt owning values gt, gt + 32 U, ... (row
-    // o & 31 of the tile, row o >> 5 of those of x).
-    const int gt = gw * 32 + lane, own = U * 32;
+    // ---- the tile's end: the group's warps join eight rows of x at a time
+    const int gt = gw * 32 + lane;
     float* gred = red + group * U * 8 * kRedRow;
     float* parts = a.parts + (int64_t)tile * a.S * (NT * 256);
-    float* part = parts + slab * (NT * 256);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      if (U == 1) {
+      group_sync(group, U);  // the sums of before are read
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) {
-          const float b0 = back[n * 8 + t4 * 2], b1 = back[n * 8 + t4 * 2 + 1];
-          const float v[4] = {tot[rt][n][0] * b0, tot[rt][n][1] * b1, tot[rt][n][2] * b0,
-                              tot[rt][n][3] * b1};
-          if (a.S > 1)
-            __stcg(reinterpret_cast<float4*>(part) + (n * 2 + rt) * 32 + lane,
-                   make_float4(v[0], v[1], v[2], v[3]));
-          else
-            store_frag(a, v, n * 8 + t4 * 2, tile * 32 + rt * 16 + g, mrows);
-        }
-      } else {
-        group_sync(group, U);  // the sums of before are read
+      for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            gred[(gw * 8 + t4 * 2 + (e & 1)) * kRedRow + rt * 16 + (e >> 1) * 8 + g] =
-                tot[rt][n][e];
-        group_sync(group, U);
-        for (int o = gt; o < 256; o += own) {
-          const int m = n * 8 + (o >> 5), row = tile * 32 + (o & 31);
-          float v = 0.f;
-#pragma unroll 2
-          for (int k = 0; k < U; ++k) v += gred[(k * 8 + (o >> 5)) * kRedRow + (o & 31)];
-          v *= back[m];
-          if (a.S > 1) __stcg(part + n * 256 + o, v);
-          else if (m < mrows && row < a.N) store_y(a, m, row, v);
-        }
-      }
+        for (int e = 0; e < 4; ++e)
+          gred[(gw * 8 + t4 * 2 + (e & 1)) * kRedRow + rt * 16 + (e >> 1) * 8 + g] = tot[rt][n][e];
+      group_sync(group, U);
+      join_rows(a, gred, back, parts + slab * (NT * 256), n, gt, tile);
     }
     if (a.S > 1) {
       // one thread's release covers the group's stores, which the barrier orders before it
@@ -528,31 +548,7 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1) int4_linear_kernel(const Int
         last_flag[group] = last;
       }
       group_sync(group, U);
-      if (last_flag[group]) {
-        // float4 o of the tile: in the MMA's layout, or four outputs of a row of x
-        for (int o = gt; o < NT * 64; o += own) {
-          float v[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int k0 = 0; k0 < a.S; k0 += 8) {
-            float4 p[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              p[k] = k0 + k < a.S
-                         ? __ldcg(reinterpret_cast<const float4*>(parts + (k0 + k) * (NT * 256)) + o)
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              v[0] += p[k].x, v[1] += p[k].y, v[2] += p[k].z, v[3] += p[k].w;
-          }
-          if (U == 1) {
-            store_frag(a, v, (o >> 6) * 8 + t4 * 2, tile * 32 + (o >> 5 & 1) * 16 + g, mrows);
-          } else {
-            const int m = o >> 3, row = tile * 32 + (o & 7) * 4;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (m < mrows && row + e < a.N) store_y(a, m, row + e, v[e]);
-          }
-        }
-      }
+      if (last_flag[group]) join_slabs(a, parts, NT * 256, gt, tile);
     }
   }
 }
