@@ -43,7 +43,7 @@ constexpr int kI4Warps = 16;
 constexpr int kI4Deep = 3;          // stages of a warp's ring, of a chunk (2 KB) each
 constexpr int kI4Tiles = 1 << 16;   // counters of the workspace: row tiles of a launch
 constexpr int kI4Smem = 226 * 1024; // shared memory of a block (the SM's, but for 1 KB)
-constexpr double kTileCost = 0.5, kSlabCost = 1.0, kWarpTime = 11;  // see int4_plan
+constexpr double kTileCost = 1.0, kSlabCost = 2.0, kWarpTime = 13;  // see int4_plan
 constexpr int kRedRow = 36;         // row of the join: 32 values, 36 apart against bank conflicts
 constexpr int kRedBytes = kI4Warps * 8 * kRedRow * 4;
 

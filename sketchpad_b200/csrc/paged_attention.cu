@@ -31,8 +31,9 @@
 namespace sp {
 namespace {
 
-constexpr int kMinSteps = 2;    // steps of a block's share at least: fewer parts to join
-constexpr int kLargeSteps = 8;  // wide steps per block from which a call counts as large
+// Wide steps per block from which a call counts as large.  From 2 to 8 nothing changes that was
+// measured; at 24, 38 sequences of 442 tokens (12 heads of 256) take 155 us instead of 109.
+constexpr int kLargeSteps = 8;
 constexpr int kMaxWide = 8;     // warps of a block on different vheads, at most
 
 struct AttnArgs {
@@ -198,8 +199,7 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
   using MT = std::conditional_t<E4M3, __half, T>;  // MMA type
   extern __shared__ uint8_t smem_raw[];  // starts on 16 bytes
   __shared__ int last_flag;
-  __shared__ float join_m[G::WARPS][16], join_l[G::WARPS][16];  // the warps', then weights
-  __shared__ float row_m[G::WARPS][16], row_l[G::WARPS][16];    // the vheads'
+  __shared__ float2 join_ml[G::WARPS][16];  // the warps' maxima and sums
   __shared__ uint32_t seen[G::WARPS][G::STAGES];  // bit r: row r of the stage's tile is visible
   __shared__ alignas(8) uint64_t arrived[G::WARPS][G::STAGES];  // the stage's copies
   __shared__ volatile int abort_flag;
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
   };
 
   // ---- this block's share of the list: `share` steps from unit0 on
-  const int32_t share = max((total + nblk - 1) / nblk, kMinSteps);
+  const int32_t share = (total + nblk - 1) / nblk;
   const int32_t unit0 = blockIdx.x * share;
   if (unit0 >= total) return;
   const int n_steps = min(share, total - unit0);
@@ -516,142 +516,142 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
     if (++stage == G::STAGES) stage = 0, parity ^= 1;
 
     if (bits != 0) {
-    // ---- scores of 16 rows x TOK tokens
-    float sc[G::TOK / 8][4];
-#pragma unroll
-    for (int n = 0; n < G::TOK / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sc[n][i] = 0.f;
-    if constexpr (E4M3) {
-      constexpr int CPL = G::CHUNKS / 4;
+      // ---- scores of 16 rows x TOK tokens
+      float sc[G::TOK / 8][4];
 #pragma unroll
       for (int n = 0; n < G::TOK / 8; ++n)
 #pragma unroll
-        for (int j = 0; j < CPL; ++j) {
-          uint32_t w[4];
-          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                       : "r"(((kt + kofs) ^ (j << 4)) + (n * G::BOXES << 10)) : "memory");
+        for (int i = 0; i < 4; ++i) sc[n][i] = 0.f;
+      if constexpr (E4M3) {
+        constexpr int CPL = G::CHUNKS / 4;
+#pragma unroll
+        for (int n = 0; n < G::TOK / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < CPL; ++j) {
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(((kt + kofs) ^ (j << 4)) + (n * G::BOXES << 10)) : "memory");
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              mma16816<MT>(sc[n], qf[j * 4 + i], e4m3x2_to_f16x2(w[i]), e4m3x2_to_f16x2(w[i] >> 16));
+          }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+          for (int h = 0; h < G::TOK / 16; ++h) {
+            uint32_t kf[4];  // tokens 0-7 (k 0-7, 8-15), tokens 8-15 (k 0-7, 8-15)
+            ldsm4(kf, ((kt + kofs) ^ ((ks * 2 & 7) << 4)) +
+                          ((h * 2 * G::BOXES + (ks * 2 >> 3)) << 10));
+            mma16816<MT>(sc[2 * h], qf[ks], kf[0], kf[1]);
+            mma16816<MT>(sc[2 * h + 1], qf[ks], kf[2], kf[3]);
+          }
+      }
+
+      // ---- softmax in log2 units; a row that has seen nothing yet keeps m = -inf, l = 0
+#pragma unroll
+      for (int n = 0; n < G::TOK / 8; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) mul2(sc[n][2 * r], sc[n][2 * r + 1], rscale[r]);
+      if (bits != kAll) {
+#pragma unroll
+        for (int n = 0; n < G::TOK / 8; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            mma16816<MT>(sc[n], qf[j * 4 + i], e4m3x2_to_f16x2(w[i]), e4m3x2_to_f16x2(w[i] >> 16));
-        }
-    } else {
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks)
-#pragma unroll
-        for (int h = 0; h < G::TOK / 16; ++h) {
-          uint32_t kf[4];  // tokens 0-7 (k 0-7, 8-15), tokens 8-15 (k 0-7, 8-15)
-          ldsm4(kf, ((kt + kofs) ^ ((ks * 2 & 7) << 4)) +
-                        ((h * 2 * G::BOXES + (ks * 2 >> 3)) << 10));
-          mma16816<MT>(sc[2 * h], qf[ks], kf[0], kf[1]);
-          mma16816<MT>(sc[2 * h + 1], qf[ks], kf[2], kf[3]);
-        }
-    }
-
-    // ---- softmax in log2 units; a row that has seen nothing yet keeps m = -inf, l = 0
-#pragma unroll
-    for (int n = 0; n < G::TOK / 8; ++n)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) mul2(sc[n][2 * r], sc[n][2 * r + 1], rscale[r]);
-    if (bits != kAll) {
+            if (!((bits >> (n * 8 + t4 * 2 + (i & 1))) & 1)) sc[n][i] = -INFINITY;
+      }
+      float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int n = 0; n < G::TOK / 8; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!((bits >> (n * 8 + t4 * 2 + (i & 1))) & 1)) sc[n][i] = -INFINITY;
-    }
-    float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int n = 0; n < G::TOK / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], sc[n][i]);
-    float mref[2];
-    bool grew = false;
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      grew |= mx[r] > m[r];
-      mx[r] = fmaxf(mx[r], m[r]);
-      mref[r] = mx[r] == -INFINITY ? 0.f : mx[r];
-    }
-    if (__any_sync(0xffffffffu, grew)) {
-      const float al[2] = {exp2_fast(m[0] - mref[0]), exp2_fast(m[1] - mref[1])};
-#pragma unroll
-      for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) mul2(o[n][2 * r], o[n][2 * r + 1], al[r]);
-      l[0] *= al[0], l[1] *= al[1];
-    }
-    m[0] = mx[0], m[1] = mx[1];
-#pragma unroll
-    for (int n = 0; n < G::TOK / 8; ++n)
+        for (int i = 0; i < 4; ++i) mx[i >> 1] = fmaxf(mx[i >> 1], sc[n][i]);
+      float mref[2];
+      bool grew = false;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        add2(sc[n][2 * r], sc[n][2 * r + 1], -mref[r]);
-        sc[n][2 * r] = exp2_fast(sc[n][2 * r]);
-        sc[n][2 * r + 1] = exp2_fast(sc[n][2 * r + 1]);
-        l[r] += sc[n][2 * r] + sc[n][2 * r + 1];
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+        grew |= mx[r] > m[r];
+        mx[r] = fmaxf(mx[r], m[r]);
+        mref[r] = mx[r] == -INFINITY ? 0.f : mx[r];
       }
+      if (__any_sync(0xffffffffu, grew)) {
+        const float al[2] = {exp2_fast(m[0] - mref[0]), exp2_fast(m[1] - mref[1])};
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) mul2(o[n][2 * r], o[n][2 * r + 1], al[r]);
+        l[0] *= al[0], l[1] *= al[1];
+      }
+      m[0] = mx[0], m[1] = mx[1];
+#pragma unroll
+      for (int n = 0; n < G::TOK / 8; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          add2(sc[n][2 * r], sc[n][2 * r + 1], -mref[r]);
+          sc[n][2 * r] = exp2_fast(sc[n][2 * r]);
+          sc[n][2 * r + 1] = exp2_fast(sc[n][2 * r + 1]);
+          l[r] += sc[n][2 * r] + sc[n][2 * r + 1];
+        }
 
-    // ---- o += p v
-    if constexpr (E4M3) {
+      // ---- o += p v
+      if constexpr (E4M3) {
 #pragma unroll
-      for (int h = 0; h < G::TOK / 16; ++h) {
-        const uint32_t pf[4] = {pack2<MT>(sc[2 * h][0], sc[2 * h][1]),
-                                pack2<MT>(sc[2 * h][2], sc[2 * h][3]),
-                                pack2<MT>(sc[2 * h + 1][0], sc[2 * h + 1][1]),
-                                pack2<MT>(sc[2 * h + 1][2], sc[2 * h + 1][3])};
+        for (int h = 0; h < G::TOK / 16; ++h) {
+          const uint32_t pf[4] = {pack2<MT>(sc[2 * h][0], sc[2 * h][1]),
+                                  pack2<MT>(sc[2 * h][2], sc[2 * h][3]),
+                                  pack2<MT>(sc[2 * h + 1][0], sc[2 * h + 1][1]),
+                                  pack2<MT>(sc[2 * h + 1][2], sc[2 * h + 1][3])};
 #pragma unroll
-        for (int n = 0; n < DP / 32; ++n) {
-          // two chunks of 16 values of d: a register of the transposed 16-bit read has values
-          // d = 16 c + 2 g and the next of two tokens, so column g of n-tile (c, e) stands for
-          // d = 16 c + 2 g + e
-          uint32_t vf[4];
-          ldsm4t(vf, ((vt + vofs) ^ ((n * 2 & 7) << 4)) +
-                         ((h * 2 * G::BOXES + (n * 2 >> 3)) << 10));
+          for (int n = 0; n < DP / 32; ++n) {
+            // two chunks of 16 values of d: a register of the transposed 16-bit read has values
+            // d = 16 c + 2 g and the next of two tokens, so column g of n-tile (c, e) stands for
+            // d = 16 c + 2 g + e
+            uint32_t vf[4];
+            ldsm4t(vf, ((vt + vofs) ^ ((n * 2 & 7) << 4)) +
+                           ((h * 2 * G::BOXES + (n * 2 >> 3)) << 10));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) vf[i] = __byte_perm(vf[i], 0, 0x3120);
+            for (int i = 0; i < 4; ++i) vf[i] = __byte_perm(vf[i], 0, 0x3120);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            mma16816<MT>(o[n * 4 + c * 2], pf, e4m3x2_to_f16x2(vf[c * 2]),
-                         e4m3x2_to_f16x2(vf[c * 2 + 1]));
-            mma16816<MT>(o[n * 4 + c * 2 + 1], pf, e4m3x2_to_f16x2(vf[c * 2] >> 16),
-                         e4m3x2_to_f16x2(vf[c * 2 + 1] >> 16));
+            for (int c = 0; c < 2; ++c) {
+              mma16816<MT>(o[n * 4 + c * 2], pf, e4m3x2_to_f16x2(vf[c * 2]),
+                           e4m3x2_to_f16x2(vf[c * 2 + 1]));
+              mma16816<MT>(o[n * 4 + c * 2 + 1], pf, e4m3x2_to_f16x2(vf[c * 2] >> 16),
+                           e4m3x2_to_f16x2(vf[c * 2 + 1] >> 16));
+            }
+          }
+        }
+      } else {
+        // p rounded to T; for bf16 its rounding error goes through a second MMA, so p counts
+        // with 16 bits and the output is as near as its own type allows
+#pragma unroll
+        for (int h = 0; h < G::TOK / 16; ++h) {
+          uint32_t pf[4], pe[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float x = sc[2 * h + (i >> 1)][(i & 1) * 2];
+            const float y = sc[2 * h + (i >> 1)][(i & 1) * 2 + 1];
+            pf[i] = pack2<MT>(x, y);
+            if constexpr (!std::is_same_v<MT, __half>) {
+              const T* e = reinterpret_cast<const T*>(&pf[i]);
+              pe[i] = pack2<MT>(x - to_f32(e[0]), y - to_f32(e[1]));
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < DP / 16; ++n) {
+            uint32_t vf[4];  // d 0-7 (tokens 0-7, 8-15), d 8-15 (tokens 0-7, 8-15)
+            ldsm4t(vf, ((vt + vofs) ^ ((n * 2 & 7) << 4)) +
+                           ((h * 2 * G::BOXES + (n * 2 >> 3)) << 10));
+            mma16816<MT>(o[2 * n], pf, vf[0], vf[1]);
+            mma16816<MT>(o[2 * n + 1], pf, vf[2], vf[3]);
+            if constexpr (!std::is_same_v<MT, __half>) {
+              mma16816<MT>(o[2 * n], pe, vf[0], vf[1]);
+              mma16816<MT>(o[2 * n + 1], pe, vf[2], vf[3]);
+            }
           }
         }
       }
-    } else {
-      // p rounded to T; for bf16 its rounding error goes through a second MMA, so p counts
-      // with 16 bits and the output is as near as its own type allows
-#pragma unroll
-      for (int h = 0; h < G::TOK / 16; ++h) {
-        uint32_t pf[4], pe[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = sc[2 * h + (i >> 1)][(i & 1) * 2];
-          const float y = sc[2 * h + (i >> 1)][(i & 1) * 2 + 1];
-          pf[i] = pack2<MT>(x, y);
-          if constexpr (!std::is_same_v<MT, __half>) {
-            const T* e = reinterpret_cast<const T*>(&pf[i]);
-            pe[i] = pack2<MT>(x - to_f32(e[0]), y - to_f32(e[1]));
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < DP / 16; ++n) {
-          uint32_t vf[4];  // d 0-7 (tokens 0-7, 8-15), d 8-15 (tokens 0-7, 8-15)
-          ldsm4t(vf, ((vt + vofs) ^ ((n * 2 & 7) << 4)) +
-                         ((h * 2 * G::BOXES + (n * 2 >> 3)) << 10));
-          mma16816<MT>(o[2 * n], pf, vf[0], vf[1]);
-          mma16816<MT>(o[2 * n + 1], pf, vf[2], vf[3]);
-          if constexpr (!std::is_same_v<MT, __half>) {
-            mma16816<MT>(o[2 * n], pe, vf[0], vf[1]);
-            mma16816<MT>(o[2 * n + 1], pe, vf[2], vf[3]);
-          }
-        }
-      }
-    }
     }
 
     // ---- the item's end, or the share's
@@ -723,79 +723,69 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
           }
         }
       }
+      if (n_parts > 1) __syncthreads();  // the part's stores come before the release below
     } else {
-    if (t4 == 0) {
-      join_m[warp][g] = m[0], join_m[warp][g + 8] = m[1];
-      join_l[warp][g] = l[0], join_l[warp][g + 8] = l[1];
-    }
-    __syncthreads();
-    // each row's maximum and sum over the warps on its vhead, and the warps' weights
-    if (tid < HB * 16) {
-      const int h = tid >> 4, row = tid & 15;
-      float mm = -INFINITY, ll = 0.f;
-#pragma unroll 2
-      for (int w = h; w < HB * TG; w += HB) mm = fmaxf(mm, join_m[w][row]);
-      const float mr = mm == -INFINITY ? 0.f : mm;
-#pragma unroll 2
-      for (int w = h; w < HB * TG; w += HB) {
-        const float f = exp2_fast(join_m[w][row] - mr);
-        ll += f * join_l[w][row];
-        join_m[w][row] = f;
+      // the warps' maxima, sums and outputs meet in shared memory, four rows at a time
+      if (t4 == 0) {
+        join_ml[warp][g] = make_float2(m[0], l[0]);
+        join_ml[warp][g + 8] = make_float2(m[1], l[1]);
       }
-      row_m[h][row] = mm, row_l[h][row] = ll;
-    }
-    // the warps' outputs meet in shared memory, four rows at a time
 #pragma unroll 1
-    for (int piece = 0; piece * 4 < a.part_rows; ++piece) {
-      auto val = [&](int e, int i) { return piece >> 1 ? o[e][2 + i] : o[e][i]; };
-      if (g >> 2 == (piece & 1)) {
-        float* dst = jo + (warp * 4 + (g & 3)) * G::JROW;
-        if constexpr (E4M3) {
+      for (int piece = 0; piece * 4 < a.part_rows; ++piece) {
+        auto val = [&](int e, int i) { return piece >> 1 ? o[e][2 + i] : o[e][i]; };
+        if (g >> 2 == (piece & 1)) {
+          float* dst = jo + (warp * 4 + (g & 3)) * G::JROW;
+          if constexpr (E4M3) {
 #pragma unroll
-          for (int c = 0; c < DP / 16; ++c)
-            *reinterpret_cast<float4*>(dst + c * 16 + t4 * 4) = make_float4(
-                val(2 * c, 0), val(2 * c + 1, 0), val(2 * c, 1), val(2 * c + 1, 1));
-        } else {
+            for (int c = 0; c < DP / 16; ++c)
+              *reinterpret_cast<float4*>(dst + c * 16 + t4 * 4) = make_float4(
+                  val(2 * c, 0), val(2 * c + 1, 0), val(2 * c, 1), val(2 * c + 1, 1));
+          } else {
 #pragma unroll
-          for (int n = 0; n < DP / 8; ++n)
-            *reinterpret_cast<float2*>(dst + n * 8 + t4 * 2) =
-                make_float2(val(n, 0), val(n, 1));
+            for (int n = 0; n < DP / 8; ++n)
+              *reinterpret_cast<float2*>(dst + n * 8 + t4 * 2) =
+                  make_float2(val(n, 0), val(n, 1));
+          }
         }
-      }
-      __syncthreads();
+        __syncthreads();
 #pragma unroll 1
-      for (int i = tid; i < heads * 4 * vecs; i += G::THREADS) {
-        const int hr = i / vecs, d = (i - hr * vecs) * 4, h = hr >> 2, row = piece * 4 + (hr & 3);
-        int k, n;
-        T* outp = place(v0 + h, k, n);
-        if (row >= n) continue;
-        const float mm = row_m[h][row], ll = row_l[h][row];
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = tid; i < heads * 4 * vecs; i += G::THREADS) {
+          const int hr = i / vecs, d = (i - hr * vecs) * 4, h = hr >> 2, row = piece * 4 + (hr & 3);
+          int k, n;
+          T* outp = place(v0 + h, k, n);
+          if (row >= n) continue;
+          float mm = -INFINITY, ll = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-        for (int w = h; w < HB * TG; w += HB) {
-          const float f = join_m[w][row];
-          const float4 v = *reinterpret_cast<const float4*>(jo + (w * 4 + (hr & 3)) * G::JROW + d);
-          acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
+          for (int w = h; w < HB * TG; w += HB) mm = fmaxf(mm, join_ml[w][row].x);
+          const float mr = mm == -INFINITY ? 0.f : mm;
+#pragma unroll 1
+          for (int w = h; w < HB * TG; w += HB) {
+            const float2 x = join_ml[w][row];
+            const float4 v = *reinterpret_cast<const float4*>(jo + (w * 4 + (hr & 3)) * G::JROW + d);
+            const float f = exp2_fast(x.x - mr);
+            ll += f * x.y;
+            acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
+          }
+          if (n_parts == 1) {
+            const float inv = ll == 0.f ? 0.f : (E4M3 ? a.c.v_scale[k] : 1.f) / ll;
+            *reinterpret_cast<uint2*>(outp + row * a.D + d) = make_uint2(
+                pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
+          } else {
+            float* p = part + h * part_floats;
+            __stcg(reinterpret_cast<float4*>(p + row * a.D + d),
+                   make_float4(acc[0], acc[1], acc[2], acc[3]));
+            if (d == 0)
+              __stcg(reinterpret_cast<float2*>(p + a.part_rows * a.D + 2 * row),
+                     make_float2(mm, ll));
+          }
         }
-        if (n_parts == 1) {
-          const float inv = ll == 0.f ? 0.f : (E4M3 ? a.c.v_scale[k] : 1.f) / ll;
-          *reinterpret_cast<uint2*>(outp + row * a.D + d) = make_uint2(
-              pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
-        } else {
-          float* p = part + h * part_floats;
-          __stcg(reinterpret_cast<float4*>(p + row * a.D + d),
-                 make_float4(acc[0], acc[1], acc[2], acc[3]));
-          float* ml = p + a.part_rows * a.D + 2 * row;
-          if (d == 0) __stcg(ml, mm), __stcg(ml + 1, ll);
-        }
+        // shared memory is free again, and the part's stores come before the release below
+        __syncthreads();
       }
-      __syncthreads();  // shared memory is free again
-    }
     }
     item_unit += at.steps;
     if (n_parts == 1) continue;
-    __syncthreads();  // the part's stores are ordered before ...
-    if (tid == 0) {   // ... this release
+    if (tid == 0) {
       int32_t* counter = a.counters + at.b * items_per_seq + at.hb;
       int before;
       asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;"
@@ -808,37 +798,6 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
       // the item starts in c0's second slot and goes on in the others' first
       const float* p0 = a.parts + (2 * (int64_t)c0 + 1) * slot_floats;
       const int64_t stride = 2 * slot_floats;
-      // a warp per row: the parts' maximum, and what their weighted sums are divided by
-#pragma unroll 1
-      for (int i = warp; i < heads * a.part_rows; i += G::WARPS) {
-        const int h = i / a.part_rows, row = i - h * a.part_rows;
-        int kh, n;
-        place(v0 + h, kh, n);
-        if (row >= n) continue;
-        const float* p = p0 + h * part_floats + a.part_rows * a.D + 2 * row;
-        float mm = -INFINITY, ll = 0.f;
-        auto add = [&](float pm, float pl) {
-          const float nm = fmaxf(mm, pm), nr = nm == -INFINITY ? 0.f : nm;
-          ll = ll * exp2_fast(mm - nr) + pl * exp2_fast(pm - nr);
-          mm = nm;
-        };
-#pragma unroll 1
-        for (int k = lane; k < n_parts; k += 32) {
-          const float2 x = __ldcg(
-              reinterpret_cast<const float2*>(p + (k == 0 ? 0 : k * stride - slot_floats)));
-          add(x.x, x.y);
-        }
-#pragma unroll 1
-        for (int x = 16; x > 0; x >>= 1) {
-          const float pm = __shfl_xor_sync(0xffffffffu, mm, x);
-          add(pm, __shfl_xor_sync(0xffffffffu, ll, x));
-        }
-        if (lane == 0) {
-          row_m[h][row] = mm == -INFINITY ? 0.f : mm;
-          row_l[h][row] = ll == 0.f ? 0.f : (E4M3 ? a.c.v_scale[kh] : 1.f) / ll;
-        }
-      }
-      __syncthreads();
 #pragma unroll 1
       for (int i = tid; i < heads * a.part_rows * vecs; i += G::THREADS) {
         const int hr = i / vecs, d = (i - hr * vecs) * 4;
@@ -848,32 +807,39 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
         if (row >= n) continue;
         const float* p = p0 + h * part_floats;
         const int ml = a.part_rows * a.D + 2 * row, at_d = row * a.D + d;
-        const float mr = row_m[h][row], inv = row_l[h][row];
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        float mm = -INFINITY, ll = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
-        for (int k = 0; k < n_parts; k += 8) {
-          float f[8];
-          float4 v[8];
-          const float* q = p;
+        for (int k = 0; k < n_parts; k += 4) {
+          float2 x[4];
+          float4 v[4];
+          float nm = mm;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
+          for (int u = 0; u < 4; ++u) {
             const bool on = k + u < n_parts;
-            f[u] = on ? __ldcg(q + ml) : -INFINITY;
-            v[u] = on ? __ldcg(reinterpret_cast<const float4*>(q + at_d)) : float4{};
-            q += k + u == 0 ? slot_floats : stride;
+            x[u] = on ? __ldcg(reinterpret_cast<const float2*>(p + ml))
+                      : make_float2(-INFINITY, 0.f);
+            v[u] = on ? __ldcg(reinterpret_cast<const float4*>(p + at_d)) : float4{};
+            p += k + u == 0 ? slot_floats : stride;
           }
-          p = q;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            f[u] = exp2_fast(f[u] - mr);
-            acc[0] += f[u] * v[u].x, acc[1] += f[u] * v[u].y;
-            acc[2] += f[u] * v[u].z, acc[3] += f[u] * v[u].w;
+          for (int u = 0; u < 4; ++u) nm = fmaxf(nm, x[u].x);
+          const float nr = nm == -INFINITY ? 0.f : nm, old = exp2_fast(mm - nr);
+          mm = nm;
+          ll *= old;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] *= old;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float f = exp2_fast(x[u].x - nr);
+            ll += f * x[u].y;
+            acc[0] += f * v[u].x, acc[1] += f * v[u].y;
+            acc[2] += f * v[u].z, acc[3] += f * v[u].w;
           }
         }
+        const float inv = ll == 0.f ? 0.f : (E4M3 ? a.c.v_scale[kh] : 1.f) / ll;
         *reinterpret_cast<uint2*>(outp + row * a.D + d) = make_uint2(
             pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv));
       }
-      __syncthreads();  // row_m and row_l are read
     }
   }
   if constexpr (TMA) {
