@@ -669,8 +669,31 @@ int ring_bytes(int gpc, bool zp) {
   return kI4Warps * kI4Deep * (2048 + 64 * gpc + (zp ? 32 * gpc : 0));
 }
 
+size_t workspace_of(const Int4Plan& p) { return (size_t)kI4Tiles * sizeof(int32_t) + p.part_bytes; }
+
+// The plan of a call's sizes, looked up where this thread has made it before (a search of some
+// microseconds).
+const Int4Plan& planned(int64_t M, int64_t N, int64_t C, int gpc, bool zp) {
+  struct Entry {
+    int64_t key[5];
+    Int4Plan plan;
+  };
+  static thread_local Entry table[64] = {};
+  const int64_t key[5] = {M, N, C, gpc * 2 + zp, num_sms()};
+  uint64_t h = 0;
+  for (int64_t k : key) h = (h ^ (uint64_t)k) * 0x9e3779b97f4a7c15ull;
+  Entry& e = table[h >> 58];
+  for (int i = 0; i < 5; ++i)
+    if (e.key[i] != key[i]) {
+      e.plan = int4_plan(M, N, C, gpc, ring_bytes(gpc, zp));
+      for (int k = 0; k < 5; ++k) e.key[k] = key[k];
+      break;
+    }
+  return e.plan;
+}
+
 template <int NT, int GPC, bool ZP, bool SBF>
-int launch_int4(Int4Args a, cudaStream_t s) {
+int launch_int4(Int4Args a, const Int4Plan& p, cudaStream_t s) {
   auto kernel = int4_linear_kernel<NT, GPC, ZP, SBF>;
   static unsigned long long flags = 0;
   if (first_time_on_device(&flags) &&
@@ -678,24 +701,23 @@ int launch_int4(Int4Args a, cudaStream_t s) {
                            kI4Smem - 1024 - kRedBytes) != cudaSuccess)
     return set_error(SP_ERR_LAUNCH, "int4 linear: shared memory attribute: %s",
                      cudaGetErrorString(cudaGetLastError()));
-  const Int4Plan p = int4_plan(a.M, a.N, a.C, GPC, Ring<GPC, ZP>::BLOCK);
   a.S = p.S, a.cs = p.cs, a.U = p.U;
   return launch_overlapped("int4 linear", kernel, p.blocks, kI4Warps * 32, p.smem, s, a);
 }
 
 template <int NT, int GPC>
-int launch_int4_zs(const Int4Args& a, bool sbf, cudaStream_t s) {
-  if (a.z) return sbf ? launch_int4<NT, GPC, true, true>(a, s)
-                      : launch_int4<NT, GPC, true, false>(a, s);
-  return sbf ? launch_int4<NT, GPC, false, true>(a, s) : launch_int4<NT, GPC, false, false>(a, s);
+int launch_int4_zs(const Int4Args& a, const Int4Plan& p, bool sbf, cudaStream_t s) {
+  if (a.z) return sbf ? launch_int4<NT, GPC, true, true>(a, p, s)
+                      : launch_int4<NT, GPC, true, false>(a, p, s);
+  return sbf ? launch_int4<NT, GPC, false, true>(a, p, s) : launch_int4<NT, GPC, false, false>(a, p, s);
 }
 
 template <int NT>
-int launch_int4_g(const Int4Args& a, int gpc, bool sbf, cudaStream_t s) {
+int launch_int4_g(const Int4Args& a, const Int4Plan& p, int gpc, bool sbf, cudaStream_t s) {
   switch (gpc) {
-    case 1: return launch_int4_zs<NT, 1>(a, sbf, s);
-    case 2: return launch_int4_zs<NT, 2>(a, sbf, s);
-    default: return launch_int4_zs<NT, 4>(a, sbf, s);
+    case 1: return launch_int4_zs<NT, 1>(a, p, sbf, s);
+    case 2: return launch_int4_zs<NT, 2>(a, p, sbf, s);
+    default: return launch_int4_zs<NT, 4>(a, p, sbf, s);
   }
 }
 
@@ -776,13 +798,14 @@ extern "C" size_t sp_int4_linear_workspace_size(int64_t M, int64_t N, int64_t K,
   Int4Shape sh{};
   if (M <= 0 || int4_shape(sh, N, K, group)) return 0;
   if (M > 32) M = 32;
-  // with and without zero points (whose ring leaves less room for x)
+  // any number of rows up to that, with and without zero points (whose ring leaves less room)
   size_t most = 0;
-  for (int zp = 0; zp < 2; ++zp) {
-    const Int4Plan p = int4_plan(M, N, sh.c, (int)sh.gpc, ring_bytes((int)sh.gpc, zp));
-    if (p.part_bytes > most) most = p.part_bytes;
-  }
-  return (size_t)kI4Tiles * sizeof(int32_t) + most;
+  for (int64_t m = 1; m <= M; ++m)
+    for (int zp = 0; zp < 2; ++zp) {
+      const size_t need = workspace_of(int4_plan(m, N, sh.c, (int)sh.gpc, ring_bytes((int)sh.gpc, zp)));
+      if (need > most) most = need;
+    }
+  return most;
 }
 
 extern "C" int sp_int4_linear(const void* x, int64_t x_row_stride, int x_dtype,
@@ -814,7 +837,12 @@ extern "C" int sp_int4_linear(const void* x, int64_t x_row_stride, int x_dtype,
                      "weights and the workspace on 16", (long long)xa);
   if (M == 0) return SP_OK;
   if (int rc = require_sm100()) return rc;
-  if (!workspace || workspace_bytes < sp_int4_linear_workspace_size(M, N, K, group))
+  const int gpc = (int)sh.gpc;
+  const bool sbf = scale_dtype == SP_BF16;
+  // 32 rows of x at a time, and the rest
+  const Int4Plan full = M >= 32 ? planned(32, N, sh.c, gpc, z_packed != nullptr) : Int4Plan{};
+  const Int4Plan tail = M % 32 ? planned(M % 32, N, sh.c, gpc, z_packed != nullptr) : Int4Plan{};
+  if (!workspace || workspace_bytes < workspace_of(full) || workspace_bytes < workspace_of(tail))
     return set_error(SP_ERR_WORKSPACE, "int4 linear: workspace missing or too small");
   Int4Args a{};
   a.x_stride = x_row_stride;
@@ -827,19 +855,18 @@ extern "C" int sp_int4_linear(const void* x, int64_t x_row_stride, int x_dtype,
   a.N = (int)N, a.K = (int)K, a.C = (int)sh.c;
   a.x_dtype = x_dtype;
   a.out_dtype = out_dtype;
-  const bool sbf = scale_dtype == SP_BF16;
-  const int gpc = (int)sh.gpc;
   const int64_t xs = x_dtype == SP_E4M3 ? 1 : 2, ys = dtype_size(out_dtype);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  for (int64_t m = 0; m < M; m += 32) {  // 32 rows of x at a time
+  for (int64_t m = 0; m < M; m += 32) {
     a.x = static_cast<const uint8_t*>(x) + m * x_row_stride * xs;
     a.x_scale = x_scale ? x_scale + m : nullptr;
     a.y = static_cast<uint8_t*>(y) + m * N * ys;
     a.M = (int)(M - m < 32 ? M - m : 32);
+    const Int4Plan& p = a.M == 32 ? full : tail;
     int rc;
-    if (a.M <= 8) rc = launch_int4_g<1>(a, gpc, sbf, s);
-    else if (a.M <= 16) rc = launch_int4_g<2>(a, gpc, sbf, s);
-    else rc = launch_int4_g<4>(a, gpc, sbf, s);
+    if (a.M <= 8) rc = launch_int4_g<1>(a, p, gpc, sbf, s);
+    else if (a.M <= 16) rc = launch_int4_g<2>(a, p, gpc, sbf, s);
+    else rc = launch_int4_g<4>(a, p, gpc, sbf, s);
     if (rc) return rc;
   }
   return SP_OK;

@@ -167,8 +167,7 @@ class Int4Linear:
             tile = 8 if M <= 8 else 16 if M <= 16 else 32
             need = self._work_bytes.get(tile)
             if need is None:
-                need = self._work_bytes[tile] = max(self.workspace_size(m)
-                                                    for m in range(1, tile + 1))
+                need = self._work_bytes[tile] = self.workspace_size(tile)
             work = _workspaces.get(index, raw, need)
         else:
             work = (workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size())

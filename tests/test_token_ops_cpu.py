@@ -136,3 +136,11 @@ def test_rope_table_pairs():
             a = pos * 10000.0 ** (-2 * i / 8)
             want = torch.tensor([a, a - torch.pi / 2], dtype=torch.float64).cos()
             assert torch.allclose(t[pos, i], want, atol=2.0 ** -24)
+
+
+@pytest.mark.parametrize("N,K,group", [(144, 4096, 32), (32, 1408, 128), (5120, 13824, 32),
+                                       (235, 17472, 64), (20832, 4864, 128)])
+def test_int4_workspace_serves_any_number_of_rows(N, K, group):
+    # a call beyond 32 rows runs the rest as a call of its own
+    need = [L.sp_int4_linear_workspace_size(m, N, K, group) for m in range(1, 70)]
+    assert need == sorted(need) and len(set(need[31:])) == 1
