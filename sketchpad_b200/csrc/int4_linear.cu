@@ -30,7 +30,14 @@
 // of a slab) in turn, a group's warps every U-th chunk, and join at the tile's end in shared
 // memory; int4_plan chooses U and S for the shortest schedule.  With S > 1 a tile's slabs are
 // joined by whichever group comes last (a counter in the workspace), in slab order, so results
-// do not depend on timing.
+// do not depend on timing.  (Equal numbers of chunks for every group instead of whole tiles, the
+// cut tiles joined in memory, took 17.1 and 36.9 us for the first and last case below.)
+//
+// Measured: 4 x 27648 x 5120, e4m3, groups of 64 with zero points 16.2 us, 4.8 TB/s or 0.73 of
+// the measured copy bandwidth (issue slots 54 % busy, HBM 47 %: the unpacking and the start of
+// the blocks); 1 x 4096 x 4096 5.7 us (the start, two chunks per warp, the join); 13 x 5120 x
+// 13824, groups of 32 18.8 us (five slabs: x staged in each block, the joins, and two MMAs per
+// weight fragment).
 #include <type_traits>
 
 #include "common.cuh"
@@ -43,7 +50,10 @@ constexpr int kI4Warps = 16;
 constexpr int kI4Deep = 3;          // stages of a warp's ring, of a chunk (2 KB) each
 constexpr int kI4Tiles = 1 << 16;   // counters of the workspace: row tiles of a launch
 constexpr int kI4Smem = 226 * 1024; // shared memory of a block (the SM's, but for 1 KB)
-constexpr double kTileCost = 1.0, kSlabCost = 2.0, kWarpTime = 13;  // see int4_plan
+// See int4_plan.  us at 3 x 3007 x 12160 groups of 32, at 5344 x 2368 with 11 rows and at
+// 256 x 15040 with 11 rows: 8.6, 8.4, 6.5 with these; with costs 0.5 and 1 8.7, 9.4, 6.5; with
+// those and warp times of 11 and 15 11.2, 9.4, 6.5 and 8.7, 9.4, 7.2.
+constexpr double kTileCost = 1.0, kSlabCost = 2.0, kWarpTime = 13;
 constexpr int kRedRow = 36;         // row of the join: 32 values, 36 apart against bank conflicts
 constexpr int kRedBytes = kI4Warps * 8 * kRedRow * 4;
 

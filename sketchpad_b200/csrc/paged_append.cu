@@ -8,7 +8,9 @@
 // Bound by HBM for prompts (q read and written, k and v read and written once) and by latency
 // for single tokens.  One block per token: a thread owns eight values at one place of a head
 // and walks the heads, so the token's position, page and (cos, sin) pairs are loaded once for
-// all of its heads, and the first heads' values while those are looked up.
+// all of its heads, and the first heads' values while those are looked up.  8193 tokens of 40 + 8
+// + 8 heads of 128 into an e4m3 cache: 39.9 us, 0.85 of the measured copy bandwidth; 32 tokens of
+// 32 + 8 + 8: 2.35 us, the chain of lookups.
 #include <new>
 
 #include "common.cuh"
@@ -18,9 +20,16 @@
 namespace sp {
 namespace {
 
+// Threads of a block.  Long calls take fewer per token, which then share the lookups over more
+// heads (us with 256 / 128 / 64 threads): 8193 tokens of 56 heads of 128 49.8 / 40.4 / 39.9,
+// 6300 of 18 heads of 256 30.3 / 24.0 / 21.5, but 2160 of 144 heads of 128 27.5 / 27.4 / 28.6;
+// 32 tokens, whose blocks do not fill the GPU, 2.2 / 2.6 with 256 / 128.
 constexpr int kAppThreads = 256;
-constexpr int64_t kAppMany = 1024;
-constexpr int kAppHeads = 2;  // heads of q of a thread whose loads are under way together
+constexpr int64_t kAppMany = 1024;     // tokens of a long call
+constexpr int64_t kAppValues = 8192;   // values of a token up to which 64 threads take it there
+// Heads of q of a thread in a round; the next round's loads are under way meanwhile.  (8193
+// tokens, us: 48.8 with 1, 42.0 with 2, 40.4 with 3, 41.4 with 4; 45.5 with 2 and no round ahead.)
+constexpr int kAppHeads = 3;
 
 struct AppendArgs {
   PagedCache c;
@@ -57,13 +66,13 @@ __global__ void __launch_bounds__(kAppThreads, 4) paged_append_kernel(const Appe
     return *reinterpret_cast<const uint4*>(src);
   };
   uint4 kv, qx[kAppHeads];
-  auto load_q = [&](int h0) {
+  auto load_q = [&](uint4 (&x)[kAppHeads], int h0) {
 #pragma unroll
     for (int u = 0; u < kAppHeads; ++u)
       if (h0 + u * slots < a.hq)
-        qx[u] = *reinterpret_cast<const uint4*>(q + (h0 + u * slots) * a.q_head);
+        x[u] = *reinterpret_cast<const uint4*>(q + (h0 + u * slots) * a.q_head);
   };
-  load_q(slot);
+  load_q(qx, slot);
   if (slot < 2 * a.hkv) kv = load_kv(slot);
   const int32_t seq = a.seq_ids[t], pos = a.positions[t];
   bool live = pos >= 0 && seq >= 0 && seq < a.c.table_rows;
@@ -102,7 +111,8 @@ __global__ void __launch_bounds__(kAppThreads, 4) paged_append_kernel(const Appe
 
   T* qo = static_cast<T*>(a.q_out) + t * a.hq * a.D + d0;
   for (int h0 = slot; h0 < a.hq; h0 += kAppHeads * slots) {
-    if (h0 != slot) load_q(h0);
+    uint4 next[kAppHeads];
+    load_q(next, h0 + kAppHeads * slots);
 #pragma unroll
     for (int u = 0; u < kAppHeads; ++u) {
       const int h = h0 + u * slots;
@@ -116,13 +126,15 @@ __global__ void __launch_bounds__(kAppThreads, 4) paged_append_kernel(const Appe
         }
         *reinterpret_cast<uint4*>(qo + h * a.D) = qx[u];
       }
+      qx[u] = next[u];
     }
   }
   if (!live) return;
   const int64_t k_at = page * a.c.k_page + in_page * a.c.k_slot + d0;
   const int64_t v_at = page * a.c.v_page + in_page * a.c.v_slot + d0;
   for (int h = slot; h < 2 * a.hkv; h += slots) {
-    if (h != slot) kv = load_kv(h);
+    uint4 next;
+    if (h + slots < 2 * a.hkv) next = load_kv(h + slots);
     const bool is_k = h < a.hkv;
     const int hk = is_k ? h : h - a.hkv;
     const int64_t at = is_k ? k_at + hk * a.c.k_head : v_at + hk * a.c.v_head;
@@ -145,6 +157,7 @@ __global__ void __launch_bounds__(kAppThreads, 4) paged_append_kernel(const Appe
     } else {
       *reinterpret_cast<uint4*>(static_cast<T*>(is_k ? a.c.k : a.c.v) + at) = kv;
     }
+    kv = next;
   }
 }
 
@@ -275,9 +288,10 @@ extern "C" int sp_paged_kv_append(const void* cache, const void* q, const void* 
   const unsigned grid = (unsigned)tokens;
   const bool f8 = h->dtype == SP_E4M3;
   auto run = [&](auto kernel) {
-    // many tokens: fewer threads with more heads each, which share the lookups
-    return launch_overlapped("paged append", kernel, grid,
-                             tokens >= kAppMany ? kAppThreads / 2 : kAppThreads, 0, s, a);
+    const int threads = tokens < kAppMany                          ? kAppThreads
+                        : (a.hq + 2 * a.hkv) * a.D <= kAppValues ? kAppThreads / 4
+                                                                 : kAppThreads / 2;
+    return launch_overlapped("paged append", kernel, grid, threads, 0, s, a);
   };
   if (dtype == SP_F16)
     return f8 ? run(paged_append_kernel<__half, true>) : run(paged_append_kernel<__half, false>);
