@@ -38,7 +38,8 @@ namespace sp {
 namespace {
 
 // Wide steps per block from which a call counts as large.  From 2 to 8 nothing changes that was
-// measured; at 24, 38 sequences of 442 tokens (12 heads of 256) take 155 us instead of 109.
+// measured; with 24, 38 sequences up to 442 (12 heads of 256, 192 query heads) take 158 us
+// instead of 93 and 64 windows of 1024 50 instead of 40.
 constexpr int kLargeSteps = 8;
 constexpr int kMaxWide = 8;     // warps of a block on different vheads, at most
 
@@ -173,9 +174,10 @@ struct Geo {
   static constexpr int BOXES = CHUNKS / 8;         // of a granule
   static constexpr int TOK = DP * ES <= 128 ? 32 : 16;
   static constexpr int TILE = TOK * DP * ES;       // k or v
-  // As many warps as their registers allow (12 of 168: 32 sequences up to 8192, D 128, 103 us
-  // against 110 with 8 of 255); an e4m3 tile's unpacking spills at 168 (112 against 130 us on
-  // four sequences up to 65536 with 8 warps and 12).
+  // As many warps as their registers allow: 12 of 168 (32 sequences up to 8192, D 128, 99 us
+  // against 102 with 8 of 255; 64 windows of 1024, D 64, 40.4 against 44.8).  An e4m3 tile's
+  // unpacking spills at 168: 8 warps (four sequences up to 65536 111 us against 109 with 12, but
+  // 7 sequences up to 2594 9.9 against 12.8).
   static constexpr int WARPS = DP > 128 ? (E4M3 ? 8 : 4) : E4M3 ? 8 : 12;
   static constexpr int STAGES = DP > 128 && !E4M3 ? 3 : 2;
   static constexpr int RING = STAGES * 2 * TILE;   // per warp
@@ -862,9 +864,9 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
 }
 
 // Warps of a block on different vheads: as many as keep all warps busy, or nearly, and at most
-// `most_wide`: 8 for 16-bit caches (32 sequences up to 8192, 8 heads of 128: 103 us, 122 with 1;
-// 64 windows of 1024, 12 heads of 64: 41 against 53); 1 for e4m3, whose unpacking keeps it
-// below the HBM's rate either way, so the joins of many heads count (112 us, 124 with 4).
+// `most_wide`: 8 for 16-bit caches (32 sequences up to 8192, 8 heads of 128: 99 us, 114 with 1;
+// 64 windows of 1024, 12 heads of 64: 40 against 50); 1 for e4m3, whose unpacking keeps it
+// below the HBM's rate either way, so the joins of many heads count (111 us, 122 with 4).
 int heads_wide(int vheads, int warps, int most_wide) {
   int best = 1;
   double most = 0;
