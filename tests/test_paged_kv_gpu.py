@@ -311,6 +311,37 @@ def test_append(T, hq, hkv, D, dtype, cdt, rope):
         assert torch.equal(u8(now)[untouched], u8(before)[untouched])
 
 
+@pytest.mark.parametrize("hq,hkv,D", [(40, 8, 128), (14, 2, 256), (56, 8, 256), (5, 1, 80),
+                                      (0, 3, 64)])
+@pytest.mark.parametrize("cdt", [BF, E4M3])
+def test_append_long_calls(hq, hkv, D, cdt):
+    """Many tokens take fewer threads each: bit for bit what the same tokens give in short calls
+    (which test_append compares with 64 bits)."""
+    T, B, page = 1531, 3, 16
+    ca, cb = (make_cache(110, page, hkv, D, cdt) for _ in range(2))
+    table = make_table([T // B + 30] * B, page, 110)
+    seq = torch.arange(T, device="cuda").to(torch.int32) % B
+    pos = 7 + torch.arange(T, device="cuda").to(torch.int32) // B
+    pos[100] = -1
+    qkv = torch.randn(T, hq + 2 * hkv, D, generator=gen(hq), device="cuda").to(BF)
+    q = qkv[:, :hq].contiguous() if hq else None
+    k, v = qkv[:, hq:hq + hkv], qkv[:, hq + hkv:]
+    cs = rope_table(T, D)
+    want = []
+    for i in range(0, T, 500):
+        e = slice(i, i + 500)
+        want.append(ca.append(k[e], v[e], table, seq[e], pos[e], q=q[e] if hq else None, rope=cs))
+    got = cb.append(k, v, table, seq, pos, q=q, rope=cs)
+    for x, y in ((ca.k, cb.k), (ca.v, cb.v)):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+    if hq:
+        assert torch.equal(torch.cat(want), got) and not got[100].any()
+        assert cb.append(k, v, table, seq, pos, q=q, rope=cs, q_out=q) is q  # in place
+        assert torch.equal(q, got)
+    else:
+        assert got is None
+
+
 def test_append_padding_and_missing_pages():
     cache = make_cache(10, 8, 2, 64, BF)
     k0 = cache.k.clone()
