@@ -178,3 +178,16 @@ def test_refusals():
                 lambda: lin(h.cpu())):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("M", [40, 65, 96])
+@pytest.mark.parametrize("N,K,group", [(144, 8192, 32), (1000, 13824, 128)])
+def test_more_rows_than_a_launch_takes(M, N, K, group):
+    """Launches that follow one another in a call share its workspace: bit for bit what calls of
+    their rows give."""
+    q, s, z = weight(N, K, group, True, torch.float16)
+    layer = Int4Linear(q, s, z, group_size=group)
+    x = torch.randn(M, K, generator=torch.Generator("cuda").manual_seed(M), device="cuda").half()
+    want = torch.cat([layer(x[i:i + 32]) for i in range(0, M, 32)])
+    for _ in range(3):
+        assert torch.equal(layer(x), want)

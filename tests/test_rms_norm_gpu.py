@@ -159,3 +159,21 @@ def test_refusals():
         rms_norm(x.double(), w.double())
     with pytest.raises(ValueError):
         rms_norm_fp8(x[:, :0], w[:0])
+
+
+@pytest.mark.parametrize("rows,n", [(6000, 120), (1500, 5120), (3000, 1031), (700, 16000), (200, 20000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_blocks_that_walk_rows(rows, n, dtype):
+    """More rows than blocks fit: bit for bit what calls of a few rows give."""
+    x, w, r = inputs(rows, n, dtype, True, 5)
+    y, s = rms_norm(x, w, 1e-6, residual=r)
+    q, sc, s8 = rms_norm_fp8(x, w, 1e-6, residual=r)
+    for i in range(0, rows, 100):
+        e = slice(i, i + 100)
+        y1, s1 = rms_norm(x[e], w, 1e-6, residual=r[e])
+        q1, sc1, s81 = rms_norm_fp8(x[e], w, 1e-6, residual=r[e])
+        assert torch.equal(y[e], y1) and torch.equal(s[e], s1) and torch.equal(s8[e], s81)
+        assert torch.equal(q[e].view(torch.uint8), q1.view(torch.uint8))
+        assert torch.equal(sc[e], sc1)
+    out, kept = rms_norm(x, w, 1e-6, residual=r, out=x, residual_out=r)  # the stream in place
+    assert out is x and kept is r and torch.equal(out, y) and torch.equal(kept, s)
