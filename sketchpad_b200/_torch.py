@@ -61,21 +61,23 @@ def cuda_index(x: torch.Tensor, *others) -> int:
 
 class Workspaces:
     """Zero-initialised device workspaces, one per (device, stream): the kernels that use them
-    leave their counters zero again, so calls in one stream's order share one.  A workspace made
-    while its stream is being captured belongs to the graph alone (its zeroing is a node of the
-    graph) and is not kept."""
+    leave their counters zero again, so calls in one stream's order share one, which grows with
+    them.  A call that is being captured never gets the stream's: the graph would outlive it, and
+    replays would meet the stream's other calls in it.  It gets one of the graph's own memory,
+    zeroed by a node of the graph (a workspace that the caller keeps saves that node)."""
 
     def __init__(self):
         self._kept = {}
 
     def get(self, index: int, stream: int, nbytes: int):
         """(tensor to hold on to until the launch, pointer, bytes) of at least nbytes."""
-        w = self._kept.get((index, stream))
+        capturing = torch.cuda.is_current_stream_capturing()
+        w = None if capturing else self._kept.get((index, stream))
         if w is None or w[2] < nbytes:
             n = (nbytes + 3) // 4
             t = torch.zeros(n, dtype=torch.int32, device=torch.device("cuda", index))
             w = (t, t.data_ptr(), n * 4)
-            if not torch.cuda.is_current_stream_capturing():
+            if not capturing:
                 self._kept[index, stream] = w
         return w
 

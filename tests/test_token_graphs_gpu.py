@@ -1,0 +1,80 @@
+"""The token operators in CUDA graphs that outlive the calls around their capture."""
+import pytest
+import torch
+
+from sketchpad_b200 import Int4Linear, PagedKVCache
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def layer(N, K, group=128, seed=0, **kw):
+    g = torch.Generator("cuda").manual_seed(seed + N + K)
+    q = torch.randint(0, 256, (N, K // 2), generator=g, device="cuda", dtype=torch.uint8)
+    s = (torch.rand(K // group, N, generator=g, device="cuda") / 64).half()
+    return Int4Linear(q, s, group_size=group, **kw)
+
+
+def occupy(nbytes):
+    """Tensors of the sizes of freed workspaces, none of their bytes zero."""
+    return [torch.full((n,), 0x5a, dtype=torch.uint8, device="cuda")
+            for n in (nbytes, nbytes, nbytes // 2, nbytes // 2) for _ in range(8)]
+
+
+def test_linear_captured_on_a_stream_that_is_used_again():
+    small, large = layer(1024, 16384, 64), layer(40000, 16384, 64)
+    assert large.workspace_size(32) > small.workspace_size(16)
+    x = torch.randn(13, 16384, device="cuda").to(BF)
+    want = [small(x * f) for f in (1, 2, 3)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    xin, out = torch.zeros_like(x), torch.zeros_like(want[0])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        small(xin, out=out)
+        s.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            small(xin, out=out)
+        held = [large(torch.randn(32, 16384, device="cuda").to(BF))]
+        s.synchronize()
+        held += occupy(small.workspace_size(16))
+        for f, w in zip((1, 2, 3), want):
+            xin.copy_(x * f)
+            out.zero_()
+            g.replay()
+            small(x)  # the stream's own calls between replays
+            s.synchronize()
+            assert torch.equal(out, w)
+    assert all(bool((t == 0x5a).all()) for t in held[1:])
+
+
+def test_attention_captured_on_a_stream_that_is_used_again():
+    gen = torch.Generator("cuda").manual_seed(3)
+    k, v = (torch.randn(130, 16, 2, 128, generator=gen, device="cuda").to(BF) for _ in range(2))
+    cache = PagedKVCache(k, v)
+    table = torch.randperm(130, generator=gen, device="cuda").to(torch.int32)[None, :128].contiguous()
+    lens = torch.tensor([2000], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 4, 128, generator=gen, device="cuda").to(BF)
+    qw = torch.randn(1, 32, 128, generator=gen, device="cuda").to(BF)
+    assert cache.workspace_size(32) > cache.workspace_size(4)
+    want = [cache.attend(q, table, lens - d) for d in (0, 1, 700)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    ln, out = lens.clone(), torch.zeros_like(q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        cache.attend(q, table, ln, out=out)
+        s.synchronize()
+        with torch.cuda.graph(g, stream=s):
+            cache.attend(q, table, ln, out=out)
+        cache.attend(qw, table, lens)
+        s.synchronize()
+        held = occupy(cache.workspace_size(4))
+        for d, w in zip((0, 1, 700), want):
+            ln.copy_(lens - d)
+            out.zero_()
+            g.replay()
+            cache.attend(q, table, lens)
+            s.synchronize()
+            assert torch.equal(out, w)
+    assert all(bool((t == 0x5a).all()) for t in held)
