@@ -32,7 +32,8 @@ class Int4Linear:
     uint8 [K/group, N] with values 0..15 (None: 8, symmetric weights), bias [N].
 
     group_size: 32, 64 or a multiple of 128 that divides K.  The constructor lays the weight out
-    for the kernels once (a device copy; the given tensors are not kept)."""
+    for the kernels once, and the bias in each output type (device copies; the given tensors are
+    not kept, and changing them later changes no output)."""
 
     def __init__(self, qweight: torch.Tensor, scales: torch.Tensor,
                  zeros: Optional[torch.Tensor] = None, *, group_size: int,
@@ -54,8 +55,11 @@ class Int4Linear:
         zeros = None if zeros is None else zeros.contiguous()
         self.out_features, self.in_features, self.group_size = N, K, group_size
         self.scale_dtype = scales.dtype
-        self.bias = bias
-        self._bias, self._work_bytes = {}, {}
+        self.bias = None if bias is None else bias.detach().clone()
+        self._bias = {} if bias is None else {
+            dt: self.bias.to(dt).contiguous()
+            for dt in (torch.float32, torch.float16, torch.bfloat16)}
+        self._work_bytes = {}
         self.q = torch.empty(sizes[0], dtype=torch.uint8, device=dev)
         self.scale = torch.empty(sizes[1], dtype=torch.uint8, device=dev)
         self.zero = None if zeros is None else torch.empty(sizes[2], dtype=torch.uint8, device=dev)
@@ -159,9 +163,8 @@ class Int4Linear:
                 p, stride = x.data_ptr(), K
             elif M <= 1:
                 stride = K
-        b_ptr = 0
-        if self.bias is not None:
-            b_ptr = self._bias_as(dt).data_ptr()
+        code = dtype_code(dt)
+        b_ptr = self._bias[dt].data_ptr() if self._bias else 0
         raw = raw_stream(index)
         if workspace is None:
             tile = 8 if M <= 8 else 16 if M <= 16 else 32
@@ -172,19 +175,13 @@ class Int4Linear:
         else:
             work = (workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size())
         _linear(p, stride, xd, s_ptr, *self._weight_args, b_ptr, out.data_ptr(), M, N, K,
-                self.group_size, dtype_code(dt), work[1], work[2], raw)
+                self.group_size, code, work[1], work[2], raw)
         return out
 
     def workspace_size(self, rows: int) -> int:
         """Bytes of a workspace (zeros, any dtype) for a call of that many rows."""
         return _lib.load().sp_int4_linear_workspace_size(rows, self.out_features,
                                                          self.in_features, self.group_size)
-
-    def _bias_as(self, dt: torch.dtype) -> torch.Tensor:
-        b = self._bias.get(dt)
-        if b is None:
-            b = self._bias[dt] = self.bias.to(dt).contiguous()
-        return b
 
     __call__ = forward
 

@@ -78,3 +78,34 @@ def test_attention_captured_on_a_stream_that_is_used_again():
             s.synchronize()
             assert torch.equal(out, w)
     assert all(bool((t == 0x5a).all()) for t in held)
+
+
+def test_bias_of_a_first_call_under_capture():
+    # the cast to the output's type is not the graph's: calls before the first replay have it too
+    bias = torch.randn(512, device="cuda")
+    lin = layer(512, 1024, bias=bias)
+    plain = layer(512, 1024)
+    x = torch.randn(3, 1024, device="cuda").to(BF)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = lin(x)
+        junk = [torch.zeros(512, dtype=BF, device="cuda") for _ in range(8)]
+    err = (lin(x).double() - plain(x, out_dtype=torch.float32).double() - bias.to(BF).double()).abs()
+    bound = 2.0 ** -7 * (plain(x, out_dtype=torch.float32).double().abs() + bias.double().abs())
+    assert bool((err <= bound).all())
+    g.replay()
+    assert torch.equal(out, lin(x)) and len(junk) == 8
+
+
+def test_bias_is_the_layers_own():
+    # like the weights: later changes of the given tensor reach no output type
+    bias = torch.randn(512, device="cuda")
+    lin = layer(512, 1024, bias=bias)
+    x = torch.randn(3, 1024, device="cuda").to(BF)
+    types = (torch.float32, torch.float16, BF)
+    before = [lin(x, out_dtype=t) for t in types]
+    other = layer(512, 1024, bias=bias.clone())
+    bias.add_(1000)
+    assert all(torch.equal(lin(x, out_dtype=t), b) for t, b in zip(types, before))
+    assert all(torch.equal(other(x, out_dtype=t), b) for t, b in zip(types, before))
+    assert torch.equal(lin.bias, bias - 1000) or float((lin.bias - (bias - 1000)).abs().max()) < 1e-3
