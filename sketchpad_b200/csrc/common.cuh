@@ -53,7 +53,8 @@ int encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, uint32_t rank, const 
 // A launch whose blocks may come up while the last blocks of the stream's kernel before it run,
 // where that kernel allows it (programmatic dependent launch).  The kernel has to execute
 // griddepcontrol.wait in every thread before it reads or writes anything that earlier work of
-// the stream touches.
+// the stream touches, and to read that with ordinary loads: non-coherent ones (__ldg) are for
+// data that nobody writes while the kernel lives, and the kernel before may still be writing.
 template <typename... P, typename... A>
 int launch_overlapped(const char* what, void (*kernel)(P...), unsigned blocks, unsigned threads,
                       size_t smem, cudaStream_t s, A&&... args) {

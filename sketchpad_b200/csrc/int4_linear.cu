@@ -166,7 +166,7 @@ __device__ __forceinline__ void x_load(XVec<XD> (&v)[kXBatch], const XVec<XD>* r
                                        int live) {
 #pragma unroll
   for (int u = 0; u < kXBatch; ++u)
-    v[u] = i + u * step < live ? __ldg(row + i + u * step) : XVec<XD>{};
+    v[u] = i + u * step < live ? row[i + u * step] : XVec<XD>{};
 }
 
 // The largest magnitude of a batch of 16-bit values, which order like their bits.

@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kAppThreads, 4) paged_append_kernel(const Appe
   float cs[8] = {1.f, 0.f, 1.f, 0.f, 1.f, 0.f, 1.f, 0.f};
   if (a.rope && live) {
     const float4* r = reinterpret_cast<const float4*>(a.rope + (int64_t)pos * (a.D >> 1)) + 2 * lane;
-    const float4 r0 = __ldg(r), r1 = __ldg(r + 1);
+    const float4 r0 = r[0], r1 = r[1];
     cs[0] = r0.x, cs[1] = r0.y, cs[2] = r0.z, cs[3] = r0.w;
     cs[4] = r1.x, cs[5] = r1.y, cs[6] = r1.z, cs[7] = r1.w;
   }

@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
           const int32_t col = a.c.page_size.div(tok);
           r.slot = tok - col * a.c.page_size.d;
           r.bits = bits;
-          r.page = __ldg(a.c.table + lk.b * a.c.table_stride + col);
+          r.page = a.c.table[lk.b * a.c.table_stride + col];
         }
       }
       advance(lk);
