@@ -12,18 +12,16 @@
 //    slots of the warp's ring in shared memory (cp.async), so four to six KB per warp are in
 //    flight without holding registers.  32 rows, because the x operand that they share comes
 //    from shared memory, which 16 rows would keep busier than the weights keep HBM.
-//  - A 4-bit value in the low bits of an f16 is the subnormal q 2^-24, exactly, and the tensor
-//    cores take subnormals: two values per AND, no subtraction, no multiplication.  Bits 4-7
-//    are 16 q 2^-24; the inputs that meet those are staged as x / 16.  The f32 sums are scaled
-//    back by 2^24 at the end.
-//  - The zero point leaves the products: sum (q - z) x = sum q x - z sum x, where sum x of a
-//    group comes from one MMA per 16 inputs with a matrix of ones, once per block; -z sum x is
-//    what a group's accumulator starts from.  (|q x| is at most twice |(q - z) x| for a middle
-//    zero point, so the f32 sums lose a bit at most.)
+//  - A 4-bit value in the low bits of an f16 of exponent 10 is 1024 + q, in bits 4-7 1024 + 16 q:
+//    two values per AND-OR, and one f16x2 instruction takes off 1024 + z, or multiplies by 1/16
+//    and takes off 64 + z, both exactly.  So the MMA's operand is q - z itself.  (Values left as
+//    f16 subnormals q 2^-24, with z sum x taken off the sums, saved two of those instructions in
+//    nine, but the tensor cores align a product by its factors' exponent fields, 2^-14 for every
+//    subnormal: sums lost ten bits, and a large input that meets q = z did not cancel.)
 //  - x is staged in shared memory as f16, each row scaled by a power of two that brings its
-//    largest value of the block's inputs to [2^14, 2^15): exact for f16 and bf16 but for values
-//    below 2^-35 of that, and e4m3 values fit as they are.  A row with an infinity or a NaN
-//    gives infinities or NaNs.
+//    largest value of the block's inputs to [2^14, 2^15): what f16 cannot hold there is at most
+//    2^-39 of that value per input (f16's subnormals, 2^-25 at most from 2^14), and e4m3 values
+//    fit as they are.  A row with an infinity or a NaN gives infinities or NaNs.
 //
 // The launch is one block of 16 warps per SM.  Where a block cannot hold all of x, the inputs
 // are cut into S slabs, each with its own blocks.  Groups of U warps take whole tiles (32 rows
@@ -31,12 +29,12 @@
 // memory; int4_plan chooses U and S for the shortest schedule.  With S > 1 a tile's slabs are
 // joined by whichever group comes last (a counter in the workspace), in slab order, so results
 // do not depend on timing.  (Equal numbers of chunks for every group instead of whole tiles, the
-// cut tiles joined in memory, took 17.1 and 36.9 us for the first and last case below.)
+// cut tiles joined in memory, was 1.06 and 1.96 times slower for the first and last case below.)
 //
-// Measured: 4 x 27648 x 5120, e4m3, groups of 64 with zero points 16.2 us, 4.8 TB/s or 0.73 of
-// the measured copy bandwidth (issue slots 54 % busy, HBM 47 %: the unpacking and the start of
-// the blocks); 1 x 4096 x 4096 5.7 us (the start, two chunks per warp, the join); 13 x 5120 x
-// 13824, groups of 32 18.8 us (five slabs: x staged in each block, the joins, and two MMAs per
+// Measured: 4 x 27648 x 5120, e4m3, groups of 64 with zero points 16.6 us, 4.7 TB/s or 0.72 of
+// the measured copy bandwidth (issue slots 58 % busy: the unpacking, and the start of the
+// blocks); 1 x 4096 x 4096 5.7 us (the start, two chunks per warp, the join); 13 x 5120 x
+// 13824, groups of 32 18.0 us (five slabs: x staged in each block, the joins, and two MMAs per
 // weight fragment).
 #include <type_traits>
 
@@ -50,10 +48,10 @@ constexpr int kI4Warps = 16;
 constexpr int kI4Deep = 3;          // stages of a warp's ring, of a chunk (2 KB) each
 constexpr int kI4Tiles = 1 << 16;   // counters of the workspace: row tiles of a launch
 constexpr int kI4Smem = 226 * 1024; // shared memory of a block (the SM's, but for 1 KB)
-// See int4_plan.  us at 3 x 3007 x 12160 groups of 32, at 5344 x 2368 with 11 rows and at
-// 256 x 15040 with 11 rows: 8.6, 8.4, 6.5 with these; with costs 0.5 and 1 8.7, 9.4, 6.5; with
-// those and warp times of 11 and 15 11.2, 9.4, 6.5 and 8.7, 9.4, 7.2.
-constexpr double kTileCost = 1.0, kSlabCost = 2.0, kWarpTime = 13;
+// See int4_plan.  us at 13 x 5120 x 13824 groups of 32, 1 x 20832 x 4864 and 11 x 5344 x 2368:
+// 18.0, 15.8, 7.0 with these; with a slab cost of 1 21.9, 15.8, 8.9; with costs of 1 and 2 and warp
+// times of 13, 11 and 9 18.3, 17.3, 7.0, then 21.9, 15.8, 7.0 and 21.9, 17.9, 7.3.
+constexpr double kTileCost = 1.0, kSlabCost = 3.0, kWarpTime = 12;
 constexpr int kRedRow = 36;         // row of the join: 32 values, 36 apart against bank conflicts
 constexpr int kRedBytes = kI4Warps * 8 * kRedRow * 4;
 
@@ -92,6 +90,24 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
 }
 __device__ __forceinline__ void prefetch_l2(const void* p) {
   asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+// (v & MASK) | 0x64006400 in one instruction: 4-bit values as mantissas of exponent 10
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t mantissas(uint32_t v) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "n"(MASK), "r"(0x64006400u));
+  return r;
+}
+// f16 pairs: a + b; a / 16 + b
+__device__ __forceinline__ uint32_t add2h(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t sixteenth2h(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0x2c002c00u), "r"(b));
+  return r;
 }
 // t[0..1] += s a[0..1], one instruction
 __device__ __forceinline__ void fma2(float* t, const float* a, float s) {
@@ -190,27 +206,19 @@ __device__ __forceinline__ void x_max_row(uint32_t mx, uint32_t* amax) {
                         : __float_as_uint(__half2float(__ushort_as_half((unsigned short)h))));
 }
 
-// A batch into shared memory as f16 times the row's power of two, pairs 1 and 3 of each 16-byte
-// group also by 1/16.
+// A batch into shared memory as f16 times the row's power of two.
 template <int XD>
 __device__ __forceinline__ void x_put(const XVec<XD> (&v)[kXBatch], float mul, uint8_t* dst, int i,
                                       int step, int groups) {
-  const float mul16 = mul * 0.0625f;
 #pragma unroll
   for (int u = 0; u < kXBatch; ++u) {
     uint32_t o[4];
     if constexpr (XD == SP_E4M3) {
       const uint32_t in[2] = {v[u].x, v[u].y};
-      const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
 #pragma unroll
-      for (int h = 0; h < 4; ++h) {
+      for (int h = 0; h < 4; ++h)
         asm("cvt.rn.f16x2.e4m3x2 %0, %1;"
             : "=r"(o[h]) : "h"((uint16_t)(in[h >> 1] >> (16 * (h & 1)))));
-        if (h & 1) {
-          const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&o[h]), sixteenth);
-          o[h] = *reinterpret_cast<const uint32_t*>(&r);
-        }
-      }
     } else {
       const uint32_t in[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
@@ -220,8 +228,7 @@ __device__ __forceinline__ void x_put(const XVec<XD> (&v)[kXBatch], float mul, u
           f = make_float2(__uint_as_float(in[h] << 16), __uint_as_float(in[h] & 0xffff0000u));
         else
           f = __half22float2(*reinterpret_cast<const __half2*>(&in[h]));
-        const float c = h & 1 ? mul16 : mul;
-        const __half2 r = __floats2half2_rn(f.x * c, f.y * c);
+        const __half2 r = __floats2half2_rn(f.x * mul, f.y * mul);
         o[h] = *reinterpret_cast<const uint32_t*>(&r);
       }
     }
@@ -282,8 +289,8 @@ __device__ __forceinline__ void group_sync(int id, int U) {
 
 // The end of a tile for eight rows of x: thread gt of the group's 32 U adds up the warps' sums in
 // `gred` for values gt, gt + 32 U, ... (output o & 31 of the tile, row o >> 5 of the eight).
-__device__ __forceinline__ void join_rows(const Int4Args& a, const float* gred, const float* back,
-                                       float* part, int n, int gt, int tile) {
+__device__ __forceinline__ void join_rows(const Int4Args& a, const float* gred,
+                                       const uint32_t* amax, float* part, int n, int gt, int tile) {
 #pragma unroll 1
   for (int o = gt; o < 256; o += a.U * 32) {
     const int m = n * 8 + (o >> 5), row = tile * 32 + (o & 31);
@@ -291,7 +298,7 @@ __device__ __forceinline__ void join_rows(const Int4Args& a, const float* gred, 
     float v = 0.f;
 #pragma unroll 4
     for (int k = 0; k < a.U; ++k) v += p[k * 8 * kRedRow];
-    v *= back[m];
+    v *= __uint_as_float((254u - row_exponent(amax[m])) << 23);  // the staged row's power of two
     if (a.S > 1) __stcg(part + n * 256 + o, v);
     else if (m < a.M && row < a.N) store_y(a, m, row, v);
   }
@@ -331,7 +338,6 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1)
   constexpr int TM = 8 * NT;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ uint32_t amax[TM];
-  __shared__ float back[TM];
   __shared__ float red[kI4Warps * 8 * kRedRow];
   __shared__ int last_flag[kI4Warps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -346,9 +352,7 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1)
   const int tile0 = blockIdx.x / a.S + group * slab_blocks;
   const int tile_step = slab_blocks * (kI4Warps / U);
   const uint32_t ring = smem_u32(smem) + warp * R::WARP;
-  // the groups' sums of x, [cs, GPC, TM / 2, 4]: two rows' sums twice, an accumulator's layout
-  float* xsum = reinterpret_cast<float*>(smem + R::BLOCK);
-  uint8_t* xsm = smem + R::BLOCK + cs * GPC * TM * 8;
+  uint8_t* xsm = smem + R::BLOCK;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -401,8 +405,6 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1)
     if (a.x_dtype == SP_E4M3) x_stage<SP_E4M3>(a, mrows, k0, groups16, live, amax, xsm, xrow);
     else if (a.x_dtype == SP_BF16) x_stage<SP_BF16>(a, mrows, k0, groups16, live, amax, xsm, xrow);
     else x_stage<SP_F16>(a, mrows, k0, groups16, live, amax, xsm, xrow);
-    // what undoes the staged row's power of two and the weights' 2^-24
-    if (tid < TM) back[tid] = __uint_as_float((254u - row_exponent(amax[tid])) << 23) * 0x1p24f;
   }
 
   // lanes beyond the last row of x repeat it: their MMA columns are never stored
@@ -411,30 +413,6 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1)
   for (int n = 0; n < NT; ++n)
     xbase[n] = xsm + min(n * 8 + g, mrows - 1) * xrow + t4 * 16;
   const float zero4[4] = {0.f, 0.f, 0.f, 0.f};
-  // ---- the groups' sums of x, in the accumulators' unit 2^-24 and times -8 (symmetric) or
-  // -1 (to be multiplied by the zero point)
-  for (int i = warp; i < cs; i += kI4Warps) {
-    const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x4c004c00u, 0x4c004c00u};  // 1, 16
-    const float unit = ZP ? -0x1p-24f : -0x1p-21f;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      float acc[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        constexpr int JPG = 4 / GPC;
-        uint32_t b[4];
-        lds<16>(b, xbase[n] + i * 256 + j * 64);
-        if (j % JPG == 0) mma_f16(acc, ones, b[0], b[1], zero4);
-        else mma_f16(acc, ones, b[0], b[1], acc);
-        mma_f16(acc, ones, b[2], b[3], acc);
-        if (j % JPG == JPG - 1 && g == 0)
-          *reinterpret_cast<float4*>(xsum + ((i * GPC + j / JPG) * TM + n * 8 + t4 * 2) * 2) =
-              make_float4(acc[0] * unit, acc[1] * unit, acc[0] * unit, acc[1] * unit);
-      }
-    }
-  }
-  __syncthreads();
-
   const uint8_t* ring_p = smem + warp * R::WARP;
   uint32_t stage = 0, refill = (kI4Deep - 1) * R::STAGE;  // offsets in the ring
   for (int tile = tile0; tile < n_tiles; tile += tile_step) {
@@ -445,7 +423,6 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1)
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) tot[rt][n][e] = 0.f;
-    const uint8_t* xs = reinterpret_cast<const uint8_t*>(xsum) + t4 * 16 + gw * (GPC * TM * 8);
     uint32_t xo = gw * 256;
 
     for (int c = gw; c < cs; c += U) {
@@ -460,42 +437,30 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1)
       refill = stage;
       stage = stage + R::STAGE == R::WARP ? 0 : stage + R::STAGE;
       float acc[2][NT][4];
+      uint32_t low[4], high[4];  // -(1024 + z), -(64 + z) of the group, f16 pairs
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         constexpr int JPG = 4 / GPC;  // words per group
         const int grp = j / JPG;
-        // what the group's accumulators start from
-        float c0[2][NT][4];
-        if (j % JPG == 0) {
-          float z[4];
-          if constexpr (ZP) {
+        if constexpr (ZP) {
+          if (j % JPG == 0)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {  // byte -> f32 through the mantissa of 2^23
+            for (int r = 0; r < 4; ++r) {  // the zero point in the low byte of 1024, twice
               const int zi = r * GPC + grp;
-              z[r] = __uint_as_float(__byte_perm(zm[zi >> 2], 0x4b000000u, 0x7540 | (zi & 3))) -
-                     8388608.f;
+              low[r] = __byte_perm(zm[zi >> 2], 0xe4e4e4e4u, 0x4040 | (zi & 3) * 0x101);
+              high[r] = add2h(low[r], 0x63806380u);  // + 960
             }
-          }
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint32_t v[4];
-            lds<16>(v, xs + (grp * TM + n * 8) * 8);
-#pragma unroll
-            for (int rt = 0; rt < 2; ++rt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                c0[rt][n][e] = __uint_as_float(v[e]);
-                if constexpr (ZP) c0[rt][n][e] *= z[rt * 2 + (e >> 1)];
-              }
-          }
         }
         // nibbles 0, 1 and, eight bits down, 2, 3 of each half
         uint32_t p[4][4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
+          const uint32_t l = ZP ? low[r] : 0xe408e408u, h = ZP ? high[r] : 0xd480d480u;
           const uint32_t v = w[r][j] >> 8;
-          p[r][0] = w[r][j] & 0x000f000fu, p[r][1] = w[r][j] & 0x00f000f0u;
-          p[r][2] = v & 0x000f000fu, p[r][3] = v & 0x00f000f0u;
+          p[r][0] = add2h(mantissas<0x000f000f>(w[r][j]), l);
+          p[r][1] = sixteenth2h(mantissas<0x00f000f0>(w[r][j]), h);
+          p[r][2] = add2h(mantissas<0x000f000f>(v), l);
+          p[r][3] = sixteenth2h(mantissas<0x00f000f0>(v), h);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -505,7 +470,7 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1)
           for (int rt = 0; rt < 2; ++rt) {
             const uint32_t a0[4] = {p[rt * 2][0], p[rt * 2 + 1][0], p[rt * 2][1], p[rt * 2 + 1][1]};
             const uint32_t a1[4] = {p[rt * 2][2], p[rt * 2 + 1][2], p[rt * 2][3], p[rt * 2 + 1][3]};
-            if (j % JPG == 0) mma_f16(acc[rt][n], a0, b[0], b[1], c0[rt][n]);
+            if (j % JPG == 0) mma_f16(acc[rt][n], a0, b[0], b[1], zero4);
             else mma_f16(acc[rt][n], a0, b[0], b[1], acc[rt][n]);
             mma_f16(acc[rt][n], a1, b[2], b[3], acc[rt][n]);
           }
@@ -527,7 +492,6 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1)
           }
         }
       }
-      xs += U * (GPC * TM * 8);
       xo += U * 256;
     }
 
@@ -544,7 +508,7 @@ __global__ void __launch_bounds__(kI4Warps * 32, 1)
         for (int e = 0; e < 4; ++e)
           gred[(gw * 8 + t4 * 2 + (e & 1)) * kRedRow + rt * 16 + (e >> 1) * 8 + g] = tot[rt][n][e];
       group_sync(group, U);
-      join_rows(a, gred, back, parts + slab * (NT * 256), n, gt, tile);
+      join_rows(a, gred, amax, parts + slab * (NT * 256), n, gt, tile);
     }
     if (a.S > 1) {
       // one thread's release covers the group's stores, which the barrier orders before it
@@ -642,10 +606,10 @@ struct Int4Plan {
 // that is kept busy: a block's chunks, or kWarpTime times those of its busiest warp if that is
 // more (fewer than kWarpTime warps do not keep an SM busy), each tile with the cost of its join,
 // in chunks of each of its warps.
-Int4Plan int4_plan(int64_t M, int64_t N, int64_t C, int gpc, int ring_bytes) {
+Int4Plan int4_plan(int64_t M, int64_t N, int64_t C, int ring_bytes) {
   const int NT = M <= 8 ? 1 : M <= 16 ? 2 : 4;
   const int64_t tokens = M < 8 * NT ? M : 8 * NT, n_tiles = (N + 31) / 32;
-  const int64_t per_chunk = tokens * 256 + gpc * 8 * NT * 8;
+  const int64_t per_chunk = tokens * 256;
   const int64_t fixed = 1024 + kRedBytes + ring_bytes + tokens * 64;
   const int64_t sms = num_sms(), fit = (kI4Smem - fixed) / per_chunk;
   const int64_t s_min = (C + fit - 1) / fit, s_max = s_min < 8 ? 16 : 2 * s_min;
@@ -695,7 +659,7 @@ const Int4Plan& planned(int64_t M, int64_t N, int64_t C, int gpc, bool zp) {
   Entry& e = table[h >> 58];
   for (int i = 0; i < 5; ++i)
     if (e.key[i] != key[i]) {
-      e.plan = int4_plan(M, N, C, gpc, ring_bytes(gpc, zp));
+      e.plan = int4_plan(M, N, C, ring_bytes(gpc, zp));
       for (int k = 0; k < 5; ++k) e.key[k] = key[k];
       break;
     }
@@ -812,7 +776,7 @@ extern "C" size_t sp_int4_linear_workspace_size(int64_t M, int64_t N, int64_t K,
   size_t most = 0;
   for (int64_t m = 1; m <= M; ++m)
     for (int zp = 0; zp < 2; ++zp) {
-      const size_t need = workspace_of(int4_plan(m, N, sh.c, (int)sh.gpc, ring_bytes((int)sh.gpc, zp)));
+      const size_t need = workspace_of(int4_plan(m, N, sh.c, ring_bytes((int)sh.gpc, zp)));
       if (need > most) most = need;
     }
   return most;
