@@ -25,7 +25,7 @@
 // Measured, heads of 128: 32 sequences of 1 to 8192 tokens (32 heads over 8, bf16) 99 us, 5.4 TB/s
 // or 0.83 of the measured copy bandwidth; 4 of 50001 to 65536 (64 over 8, e4m3) 111 us, 0.65 (two
 // conversions and two MMAs per register of e4m3, 8 warps of 246 registers: the dependences
-// between them); 64 windows of 1024 (12 heads of 64, f16) 40.5 us, 0.76; one sequence of 4097
+// between them); 64 windows of 1024 (12 heads of 64, f16) 41.7 us, 0.74; one sequence of 4097
 // (40 over 8) 15.8 us, two steps of a block and the joins' two round trips.
 #include <type_traits>
 
@@ -38,8 +38,8 @@ namespace sp {
 namespace {
 
 // Wide steps per block from which a call counts as large.  From 2 to 8 nothing changes that was
-// measured; with 24, 38 sequences up to 442 (12 heads of 256, 192 query heads) take 158 us
-// instead of 93 and 64 windows of 1024 50 instead of 40.
+// measured; with 24, 38 sequences up to 442 (12 heads of 256, 192 query heads) take 161 us
+// instead of 96 and 64 windows of 1024 53 instead of 42.
 constexpr int kLargeSteps = 8;
 constexpr int kMaxWide = 8;     // warps of a block on different vheads, at most
 
@@ -175,7 +175,7 @@ struct Geo {
   static constexpr int TOK = DP * ES <= 128 ? 32 : 16;
   static constexpr int TILE = TOK * DP * ES;       // k or v
   // As many warps as their registers allow: 12 of 168 (32 sequences up to 8192, D 128, 99 us
-  // against 102 with 8 of 255; 64 windows of 1024, D 64, 40.4 against 44.8).  An e4m3 tile's
+  // against 102 with 8 of 255; 64 windows of 1024, D 64, 41.7 against 47.6).  An e4m3 tile's
   // unpacking spills at 168: 8 warps (four sequences up to 65536 111 us against 109 with 12, but
   // 7 sequences up to 2594 9.9 against 12.8).
   static constexpr int WARPS = DP > 128 ? (E4M3 ? 8 : 4) : E4M3 ? 8 : 12;
@@ -603,14 +603,29 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
           l[r] += sc[n][2 * r] + sc[n][2 * r + 1];
         }
 
-      // ---- o += p v
-      if constexpr (E4M3) {
+      // ---- o += p v.  p is rounded to the MMA's type.  Where that shows beside the output's own
+      // rounding, p's rounding error goes through a second MMA, so that p counts with 16 bits
+      // (bf16) or 21: all but e4m3 values for bf16 output, to whose error of 2^-9 f16's 2^-12 adds
+      // a fiftieth.
+      constexpr bool kSplit = !(E4M3 && std::is_same_v<T, __nv_bfloat16>);
 #pragma unroll
-        for (int h = 0; h < G::TOK / 16; ++h) {
-          const uint32_t pf[4] = {pack2<MT>(sc[2 * h][0], sc[2 * h][1]),
-                                  pack2<MT>(sc[2 * h][2], sc[2 * h][3]),
-                                  pack2<MT>(sc[2 * h + 1][0], sc[2 * h + 1][1]),
-                                  pack2<MT>(sc[2 * h + 1][2], sc[2 * h + 1][3])};
+      for (int h = 0; h < G::TOK / 16; ++h) {
+        uint32_t pf[4], pe[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = sc[2 * h + (i >> 1)][(i & 1) * 2];
+          const float y = sc[2 * h + (i >> 1)][(i & 1) * 2 + 1];
+          pf[i] = pack2<MT>(x, y);
+          if constexpr (kSplit) {
+            const MT* e = reinterpret_cast<const MT*>(&pf[i]);
+            pe[i] = pack2<MT>(x - to_f32(e[0]), y - to_f32(e[1]));
+          }
+        }
+        auto add = [&](float (&c)[4], uint32_t b0, uint32_t b1) {
+          mma16816<MT>(c, pf, b0, b1);
+          if constexpr (kSplit) mma16816<MT>(c, pe, b0, b1);
+        };
+        if constexpr (E4M3) {
 #pragma unroll
           for (int n = 0; n < DP / 32; ++n) {
             // two chunks of 16 values of d: a register of the transposed 16-bit read has values
@@ -623,40 +638,19 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
             for (int i = 0; i < 4; ++i) vf[i] = __byte_perm(vf[i], 0, 0x3120);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              mma16816<MT>(o[n * 4 + c * 2], pf, e4m3x2_to_f16x2(vf[c * 2]),
-                           e4m3x2_to_f16x2(vf[c * 2 + 1]));
-              mma16816<MT>(o[n * 4 + c * 2 + 1], pf, e4m3x2_to_f16x2(vf[c * 2] >> 16),
-                           e4m3x2_to_f16x2(vf[c * 2 + 1] >> 16));
+              add(o[n * 4 + c * 2], e4m3x2_to_f16x2(vf[c * 2]), e4m3x2_to_f16x2(vf[c * 2 + 1]));
+              add(o[n * 4 + c * 2 + 1], e4m3x2_to_f16x2(vf[c * 2] >> 16),
+                  e4m3x2_to_f16x2(vf[c * 2 + 1] >> 16));
             }
           }
-        }
-      } else {
-        // p rounded to T; for bf16 its rounding error goes through a second MMA, so p counts
-        // with 16 bits and the output is as near as its own type allows
-#pragma unroll
-        for (int h = 0; h < G::TOK / 16; ++h) {
-          uint32_t pf[4], pe[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x = sc[2 * h + (i >> 1)][(i & 1) * 2];
-            const float y = sc[2 * h + (i >> 1)][(i & 1) * 2 + 1];
-            pf[i] = pack2<MT>(x, y);
-            if constexpr (!std::is_same_v<MT, __half>) {
-              const T* e = reinterpret_cast<const T*>(&pf[i]);
-              pe[i] = pack2<MT>(x - to_f32(e[0]), y - to_f32(e[1]));
-            }
-          }
+        } else {
 #pragma unroll
           for (int n = 0; n < DP / 16; ++n) {
             uint32_t vf[4];  // d 0-7 (tokens 0-7, 8-15), d 8-15 (tokens 0-7, 8-15)
             ldsm4t(vf, ((vt + vofs) ^ ((n * 2 & 7) << 4)) +
                            ((h * 2 * G::BOXES + (n * 2 >> 3)) << 10));
-            mma16816<MT>(o[2 * n], pf, vf[0], vf[1]);
-            mma16816<MT>(o[2 * n + 1], pf, vf[2], vf[3]);
-            if constexpr (!std::is_same_v<MT, __half>) {
-              mma16816<MT>(o[2 * n], pe, vf[0], vf[1]);
-              mma16816<MT>(o[2 * n + 1], pe, vf[2], vf[3]);
-            }
+            add(o[2 * n], vf[0], vf[1]);
+            add(o[2 * n + 1], vf[2], vf[3]);
           }
         }
       }
@@ -865,7 +859,7 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
 
 // Warps of a block on different vheads: as many as keep all warps busy, or nearly, and at most
 // `most_wide`: 8 for 16-bit caches (32 sequences up to 8192, 8 heads of 128: 99 us, 114 with 1;
-// 64 windows of 1024, 12 heads of 64: 40 against 50); 1 for e4m3, whose unpacking keeps it
+// 64 windows of 1024, 12 heads of 64: 42 against 53); 1 for e4m3, whose unpacking keeps it
 // below the HBM's rate either way, so the joins of many heads count (111 us, 122 with 4).
 int heads_wide(int vheads, int warps, int most_wide) {
   int best = 1;
