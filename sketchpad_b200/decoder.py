@@ -127,17 +127,33 @@ class Decoder:
              seq_lens: torch.Tensor) -> torch.Tensor:
         """One new token per sequence: hidden [sequences, hidden] its embedding, seq_lens (int32)
         the tokens before it, which its own joins (seq_lens is advanced).  A sequence of
-        negative length is padding and stays so.  Returns the normalised output."""
+        negative length is padding and stays so.  One that has no room for the token stays as it
+        is, too: its length is not advanced, nothing is stored, and its row of the output, which
+        attends to nothing, is not a token's.  (No room: max_positions or the block table's
+        columns are used up, or the table names no page of the cache at the token's position; with
+        the page filled in, the next step goes on.)  Returns the normalised output."""
         B = hidden.shape[0]
-        live = (seq_lens >= 0).to(torch.int32)
-        positions = seq_lens.clone()
-        seq_lens += live
+        positions, attended = self._advance(seq_lens, block_table)
         seq_ids = torch.arange(B, dtype=torch.int32, device=hidden.device)
         x, residual = hidden, None
         for layer, cache in zip(self.layers, self.caches):
             x, residual = layer.step(x, residual, cache, block_table, seq_ids, positions,
-                                     seq_lens, self.rope)
+                                     attended, self.rope)
         return rms_norm(x, self.norm, self.config.eps, residual=residual)[0]
+
+
+    def _advance(self, seq_lens: torch.Tensor, block_table: torch.Tensor):
+        """Advances seq_lens where the new token has room; (its position or -1, the tokens to
+        attend to, its own among them, or 0)."""
+        page_size = min(c.page_size for c in self.caches)
+        pages = min(c.pages for c in self.caches)
+        end = min(self.config.max_positions, block_table.shape[1] * page_size)
+        at = seq_lens.clamp(0, end - 1)
+        page = block_table.gather(1, (at // page_size).long()[:, None])[:, 0]
+        live = (at == seq_lens) & (page.clamp(0, pages - 1) == page)
+        positions = torch.where(live, seq_lens, -1)
+        seq_lens += live
+        return positions, positions + 1
 
 
 class DecoderGraph:
