@@ -105,8 +105,10 @@ class Decoder:
 
     def __init__(self, config: DecoderConfig, layers: List[DecoderLayer], norm: torch.Tensor,
                  caches: List[PagedKVCache]):
-        if len(layers) != len(caches):
-            raise ValueError("one cache per layer")
+        if not layers or len(layers) != len(caches):
+            raise ValueError("at least one layer, and one cache per layer")
+        if any(c.page_size != caches[0].page_size or c.pages != caches[0].pages for c in caches):
+            raise ValueError("the caches share a block table: as many pages each, of one size")
         self.config, self.layers, self.norm, self.caches = config, layers, norm, caches
         self.rope = rope_table(config, norm.device)
 
@@ -145,8 +147,7 @@ class Decoder:
     def _advance(self, seq_lens: torch.Tensor, block_table: torch.Tensor):
         """Advances seq_lens where the new token has room; (its position or -1, the tokens to
         attend to, its own among them, or 0)."""
-        page_size = min(c.page_size for c in self.caches)
-        pages = min(c.pages for c in self.caches)
+        pages, page_size = self.caches[0].pages, self.caches[0].page_size
         end = min(self.config.max_positions, block_table.shape[1] * page_size)
         at = seq_lens.clamp(0, end - 1)
         page = block_table.gather(1, (at // page_size).long()[:, None])[:, 0]
