@@ -15,7 +15,7 @@ can be captured into a CUDA graph once and replayed for every token.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, NamedTuple, Optional
 
 import torch
 
@@ -51,6 +51,12 @@ def rope_table(config: DecoderConfig, device="cuda") -> torch.Tensor:
     return rope_pair_table(ang.cos(), ang.sin()).to(device)
 
 
+class StepWorkspaces(NamedTuple):
+    """What the steps of one graph, or one stream, share: their linears' and their attention's."""
+    linear: torch.Tensor
+    attend: torch.Tensor
+
+
 class DecoderLayer:
     """Weights: float tensors in the linears' [out, in] layout, quantized here to 4 bits.
 
@@ -81,23 +87,28 @@ class DecoderLayer:
 
     def step(self, x: torch.Tensor, residual: Optional[torch.Tensor], cache: PagedKVCache,
              block_table: torch.Tensor, seq_ids: torch.Tensor, positions: torch.Tensor,
-             seq_lens: torch.Tensor, rope: torch.Tensor):
+             seq_lens: torch.Tensor, rope: torch.Tensor,
+             workspaces: Optional[StepWorkspaces] = None):
         """x [sequences, hidden]: the layer before's output, residual: the stream it has not been
-        added to yet (None: x is the stream).  Returns the same pair for the next layer."""
+        added to yet (None: x is the stream).  workspaces: those of `Decoder.new_workspaces` (else
+        the stream's).  Returns the same pair for the next layer."""
         c = self.config
+        wl, wa = workspaces or (None, None)
         B = x.shape[0]
         if residual is None:
             xq, xs = rms_norm_fp8(x, self.norm1, c.eps)
             residual = x
         else:
             xq, xs, residual = rms_norm_fp8(x, self.norm1, c.eps, residual=residual)
-        qkv = self.qkv(xq, xs, out_dtype=x.dtype).view(B, c.heads + 2 * c.kv_heads, c.head_dim)
+        qkv = self.qkv(xq, xs, out_dtype=x.dtype, workspace=wl).view(B, c.heads + 2 * c.kv_heads, c.head_dim)
         q, k, v = qkv.split((c.heads, c.kv_heads, c.kv_heads), 1)
         q = cache.append(k, v, block_table, seq_ids, positions, q=q, rope=rope)
-        o = cache.attend(q, block_table, seq_lens, window=c.window, sinks=c.sinks)
-        x = self.out(o.view(B, c.heads * c.head_dim))
+        o = cache.attend(q, block_table, seq_lens, window=c.window, sinks=c.sinks,
+                         workspace=wa)
+        x = self.out(o.view(B, c.heads * c.head_dim), workspace=wl)
         xq, xs, residual = rms_norm_fp8(x, self.norm2, c.eps, residual=residual)
-        return self.down(swiglu(self.gate_up(xq, xs, out_dtype=x.dtype))), residual
+        h = swiglu(self.gate_up(xq, xs, out_dtype=x.dtype, workspace=wl))
+        return self.down(h, workspace=wl), residual
 
 
 class Decoder:
@@ -125,8 +136,16 @@ class Decoder:
         norm = torch.ones(config.hidden, dtype=torch.bfloat16, device=device)
         return cls(config, layers, norm, caches)
 
-    def step(self, hidden: torch.Tensor, block_table: torch.Tensor,
-             seq_lens: torch.Tensor) -> torch.Tensor:
+    def new_workspaces(self, batch: int) -> StepWorkspaces:
+        """Workspaces for steps of up to `batch` sequences, one after another."""
+        dev = self.norm.device
+        need = max(lin.workspace_size(batch) for la in self.layers
+                   for lin in (la.qkv, la.out, la.gate_up, la.down))
+        return StepWorkspaces(torch.zeros((need + 3) // 4, dtype=torch.int32, device=dev),
+                              self.caches[0].new_workspace(self.config.heads))
+
+    def step(self, hidden: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+             workspaces: Optional[StepWorkspaces] = None) -> torch.Tensor:
         """One new token per sequence: hidden [sequences, hidden] its embedding, seq_lens (int32)
         the tokens before it, which its own joins (seq_lens is advanced).  A sequence of
         negative length is padding and stays so.  One that has no room for the token stays as it
@@ -140,7 +159,7 @@ class Decoder:
         x, residual = hidden, None
         for layer, cache in zip(self.layers, self.caches):
             x, residual = layer.step(x, residual, cache, block_table, seq_ids, positions,
-                                     attended, self.rope)
+                                     attended, self.rope, workspaces)
         return rms_norm(x, self.norm, self.config.eps, residual=residual)[0]
 
 
@@ -159,21 +178,26 @@ class Decoder:
 
 class DecoderGraph:
     """A decoder's step captured for a batch: replayed with the contents of `hidden`,
-    `block_table` and `seq_lens` of the moment; `output` holds the result."""
+    `block_table` and `seq_lens` of the moment; `output` holds the result.
+
+    The graph has workspaces of its own, zeroed once (a captured call without them zeroes one in
+    every replay, between kernels that would overlap)."""
 
     def __init__(self, decoder: Decoder, batch: int, max_pages: int):
         dev = decoder.norm.device
         self.hidden = torch.zeros(batch, decoder.config.hidden, dtype=torch.bfloat16, device=dev)
         self.block_table = torch.full((batch, max_pages), -1, dtype=torch.int32, device=dev)
         self.seq_lens = torch.full((batch,), -1, dtype=torch.int32, device=dev)
+        self.workspaces = decoder.new_workspaces(batch)
         side = torch.cuda.Stream(dev)
         side.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(side):  # padding only: nothing enters the caches
-            decoder.step(self.hidden, self.block_table, self.seq_lens)
+            decoder.step(self.hidden, self.block_table, self.seq_lens, self.workspaces)
         torch.cuda.current_stream(dev).wait_stream(side)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
-            self.output = decoder.step(self.hidden, self.block_table, self.seq_lens)
+            self.output = decoder.step(self.hidden, self.block_table, self.seq_lens,
+                                       self.workspaces)
 
     def replay(self) -> torch.Tensor:
         self.graph.replay()
@@ -202,7 +226,8 @@ def main() -> None:
           f"{ms * 1e3:.0f} us a step, {batch / ms * 1e3:.0f} tokens/s")
 
 
-__all__ = ["DecoderConfig", "DecoderLayer", "Decoder", "DecoderGraph", "rope_table"]
+__all__ = ["DecoderConfig", "DecoderLayer", "Decoder", "DecoderGraph", "StepWorkspaces",
+           "rope_table"]
 
 if __name__ == "__main__":
     main()

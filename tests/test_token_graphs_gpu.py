@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from sketchpad_b200 import Int4Linear, PagedKVCache
+from sketchpad_b200 import Int4Linear, PagedKVCache, _torch
+from sketchpad_b200.decoder import Decoder, DecoderConfig, DecoderGraph
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -109,3 +110,33 @@ def test_bias_is_the_layers_own():
     assert all(torch.equal(lin(x, out_dtype=t), b) for t, b in zip(types, before))
     assert all(torch.equal(other(x, out_dtype=t), b) for t, b in zip(types, before))
     assert torch.equal(lin.bias, bias - 1000) or float((lin.bias - (bias - 1000)).abs().max()) < 1e-3
+
+
+def test_a_captured_step_zeroes_no_workspaces(monkeypatch):
+    c = DecoderConfig(hidden=512, intermediate=768, heads=8, kv_heads=2, head_dim=64, layers=2,
+                      group_size=64, max_positions=64)
+    dec = Decoder.random(c, pages=8, page_size=16)
+    made, get = [], _torch.Workspaces.get
+
+    def record(self, *a):
+        made.append(a)
+        return get(self, *a)
+
+    monkeypatch.setattr(_torch.Workspaces, "get", record)
+    g = DecoderGraph(dec, 2, 4)
+    assert not made
+    monkeypatch.undo()
+    table = torch.arange(8, dtype=torch.int32, device="cuda").view(2, 4)
+    lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    g.block_table.copy_(table)
+    g.seq_lens.zero_()
+    hidden = torch.randn(20, 2, c.hidden, device="cuda").to(BF)
+    outs = []
+    for h in hidden:
+        g.hidden.copy_(h)
+        outs.append(g.replay().clone())
+    w = g.workspaces
+    torch.cuda.synchronize()
+    assert not w.linear[:1 << 16].any() and not w.attend[:1 << 18].any()  # the counters
+    for h, out in zip(hidden, outs):
+        assert torch.equal(dec.step(h, table, lens), out)
