@@ -185,7 +185,8 @@ class DecoderGraph:
 
     def __init__(self, decoder: Decoder, batch: int, max_pages: int):
         dev = decoder.norm.device
-        self.hidden = torch.zeros(batch, decoder.config.hidden, dtype=torch.bfloat16, device=dev)
+        self.hidden = torch.zeros(batch, decoder.config.hidden, dtype=decoder.norm.dtype,
+                                  device=dev)
         self.block_table = torch.full((batch, max_pages), -1, dtype=torch.int32, device=dev)
         self.seq_lens = torch.full((batch,), -1, dtype=torch.int32, device=dev)
         self.workspaces = decoder.new_workspaces(batch)

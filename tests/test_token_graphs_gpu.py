@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from sketchpad_b200 import Int4Linear, PagedKVCache, _torch
-from sketchpad_b200.decoder import Decoder, DecoderConfig, DecoderGraph
+from sketchpad_b200.decoder import Decoder, DecoderConfig, DecoderGraph, DecoderLayer
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -140,3 +140,21 @@ def test_a_captured_step_zeroes_no_workspaces(monkeypatch):
     assert not w.linear[:1 << 16].any() and not w.attend[:1 << 18].any()  # the counters
     for h, out in zip(hidden, outs):
         assert torch.equal(dec.step(h, table, lens), out)
+
+
+def test_a_graph_of_an_f16_decoder():
+    c = DecoderConfig(hidden=256, intermediate=256, heads=4, kv_heads=2, head_dim=64,
+                      group_size=64, max_positions=64)
+    HF = torch.float16
+    k, v = (torch.zeros(4, 16, 2, 64, dtype=HF, device="cuda") for _ in range(2))
+    dec = Decoder(c, [DecoderLayer.random(c, dtype=HF)], torch.ones(256, dtype=HF, device="cuda"),
+                  [PagedKVCache(k, v)])
+    g = DecoderGraph(dec, 1, 4)
+    assert g.hidden.dtype == g.output.dtype == HF
+    g.block_table.copy_(torch.arange(4, dtype=torch.int32)[None])
+    g.seq_lens.zero_()
+    lens = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for h in torch.randn(5, 1, 256, device="cuda").to(HF):
+        g.hidden.copy_(h)
+        out = g.replay().clone()
+        assert torch.equal(dec.step(h, g.block_table, lens), out)
