@@ -82,6 +82,13 @@ class Workspaces:
         return w
 
 
+def given_workspace(t: torch.Tensor):
+    """What Workspaces.get returns, of a workspace that the caller gives."""
+    if not t.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    return t, t.data_ptr(), t.numel() * t.element_size()
+
+
 def ptr(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 

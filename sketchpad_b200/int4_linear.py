@@ -18,7 +18,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._torch import Workspaces, cuda_index, dtype_code, ptr, raw_stream, require_cuda, stream_ptr
+from ._torch import (Workspaces, cuda_index, dtype_code, given_workspace, ptr, raw_stream,
+                     require_cuda, stream_ptr)
 
 _linear = _lib.Entry("sp_int4_linear")
 _workspaces = Workspaces()
@@ -173,7 +174,7 @@ class Int4Linear:
                 need = self._work_bytes[tile] = self.workspace_size(tile)
             work = _workspaces.get(index, raw, need)
         else:
-            work = (workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size())
+            work = given_workspace(workspace)
         _linear(p, stride, xd, s_ptr, *self._weight_args, b_ptr, out.data_ptr(), M, N, K,
                 self.group_size, code, work[1], work[2], raw)
         return out

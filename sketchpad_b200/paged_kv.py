@@ -20,7 +20,8 @@ from typing import Dict, Optional
 import torch
 
 from . import _lib
-from ._torch import Workspaces, cuda_index, dtype_code, ptr, raw_stream, require_cuda
+from ._torch import (Workspaces, cuda_index, dtype_code, given_workspace, ptr, raw_stream,
+                     require_cuda)
 
 _append = _lib.Entry("sp_paged_kv_append")
 _attend = _lib.Entry("sp_paged_attention")
@@ -191,7 +192,7 @@ class PagedKVCache:
                 need = self._work_bytes[hq] = self.workspace_size(hq)
             work = _workspaces.get(index, stream, need)
         else:
-            work = (workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size())
+            work = given_workspace(workspace)
         _attend(self._handle, q_ptr, q_seq, q_head, table.data_ptr(), cols,
                 max(table.stride(0), cols), seq_lens.data_ptr(), out.data_ptr(), B, hq, window,
                 sinks, scale or 0.0, code, work[1], work[2], stream)

@@ -1,0 +1,27 @@
+"""Calls of the token operators that are refused on the host, before anything is launched."""
+import pytest
+import torch
+
+from sketchpad_b200 import Int4Linear, PagedKVCache
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def test_workspaces_that_are_not_contiguous():
+    lin = Int4Linear(torch.zeros(64, 64, dtype=torch.uint8, device="cuda"),
+                     torch.ones(1, 64, dtype=torch.float16, device="cuda"), group_size=128)
+    w = torch.zeros(lin.workspace_size(1) // 4, 2, dtype=torch.int32, device="cuda")[:, 0]
+    x = torch.zeros(1, 128, dtype=BF, device="cuda")
+    with pytest.raises(ValueError):
+        lin(x, workspace=w)
+    assert not lin(x, workspace=w.contiguous()).any()
+    t = torch.zeros(2, 16, 1, 64, dtype=BF, device="cuda")
+    cache = PagedKVCache(t, t.clone())
+    w = torch.zeros(cache.workspace_size(1) // 4 + 1, 2, dtype=torch.int32, device="cuda")[:, 0]
+    q = torch.zeros(1, 1, 64, dtype=BF, device="cuda")
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    n = torch.ones(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        cache.attend(q, table, n, workspace=w)
+    assert not cache.attend(q, table, n, workspace=w.contiguous()).any()

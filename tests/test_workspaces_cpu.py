@@ -37,3 +37,12 @@ def test_a_capture_never_gets_the_streams_workspace(host):
     assert w.get(0, 7, 100)[1] == kept[1]  # nor does the stream get the graph's
     larger = w.get(0, 7, 1000)
     assert larger[1] not in (kept[1], inside[1])
+
+
+def test_a_given_workspace_is_contiguous():
+    # its bytes are counted from its values, which must not lie further apart
+    t = torch.zeros(64, 4, dtype=torch.int32)
+    assert _torch.given_workspace(t)[1:] == (t.data_ptr(), 1024)
+    for bad in (t[:, :2], t[::2], t.t()):
+        with pytest.raises(ValueError):
+            _torch.given_workspace(bad)
