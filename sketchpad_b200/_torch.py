@@ -41,6 +41,12 @@ except AttributeError:  # a torch built without CUDA: the operators raise before
     def _raw_stream(index: int) -> int:
         return torch.cuda.current_stream(index).cuda_stream
 
+try:
+    _current_device = torch._C._cuda_getDevice
+except AttributeError:
+    def _current_device() -> int:
+        return torch.cuda.current_device()
+
 
 def raw_stream(index: int) -> int:
     """The handle of the device's current stream as an int (stream_ptr builds a Stream object
@@ -49,10 +55,14 @@ def raw_stream(index: int) -> int:
 
 
 def cuda_index(x: torch.Tensor, *others) -> int:
-    """The device index that x and the others (None: absent) share; ValueError as require_cuda."""
+    """The device index that x and the others (None: absent) share, which has to be the current
+    one (kernels are launched there); ValueError as require_cuda."""
     i = x.get_device()
     if i < 0:
         raise ValueError("sketchpad_b200 ops take CUDA tensors (there is no CPU path)")
+    if i != _current_device():
+        raise ValueError(f"the tensors are on cuda:{i} and the current device is "
+                         f"cuda:{_current_device()} (torch.cuda.set_device)")
     for t in others:
         if t is not None and t.get_device() != i:
             require_cuda(x, *others)

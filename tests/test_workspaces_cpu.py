@@ -46,3 +46,22 @@ def test_a_given_workspace_is_contiguous():
     for bad in (t[:, :2], t[::2], t.t()):
         with pytest.raises(ValueError):
             _torch.given_workspace(bad)
+
+
+class OnDevice:
+    def __init__(self, index):
+        self.index = index
+
+    def get_device(self):
+        return self.index
+
+
+def test_operators_run_on_the_current_device(monkeypatch):
+    # a default stream's handle is the same on every device: the kernel would run on the current
+    # one, with addresses of another
+    monkeypatch.setattr(_torch, "_current_device", lambda: 1, raising=False)
+    assert _torch.cuda_index(OnDevice(1), None, OnDevice(1)) == 1
+    with pytest.raises(ValueError):
+        _torch.cuda_index(OnDevice(0), OnDevice(0))
+    with pytest.raises(ValueError):
+        _torch.cuda_index(OnDevice(-1))
