@@ -156,8 +156,9 @@ class PagedKVCache:
         """softmax(scale q k^T) v of one new token per sequence: q [sequences, heads, head_dim]
         over the seq_lens[b] (int32) tokens of sequence b, its own among them; query head h reads
         cache head h // (heads / kv_heads).  window: only the last `window` tokens and the first
-        `sinks`.  scale: 1 / sqrt(head_dim) unless given.  A sequence of length 0, or without a
-        page that is there, gives zeros."""
+        `sinks`.  scale: positive, 1 / sqrt(head_dim) unless given.  Lengths beyond the block
+        table are cut, tokens on pages that are not there are not seen, and a sequence that sees
+        none gives zeros."""
         index = cuda_index(q, block_table, seq_lens, out, workspace, self.k)
         D, hkv = self.head_dim, self.kv_heads
         if q.dim() != 3:
@@ -180,6 +181,10 @@ class PagedKVCache:
             raise ValueError("window must be at least 1")
         if sinks < 0:
             raise ValueError("sinks must not be negative")
+        if scale is None:
+            scale = 0.0  # the entry's own 1 / sqrt(head_dim)
+        elif not 2.0 ** -126 <= scale < float("inf"):
+            raise ValueError("scale must be positive and finite (None: 1 / sqrt(head_dim))")
         if out is None:
             out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, hq, D))
         elif out.shape != (B, hq, D) or out.dtype != q.dtype or not out.is_contiguous():
@@ -195,7 +200,7 @@ class PagedKVCache:
             work = given_workspace(workspace)
         _attend(self._handle, q_ptr, q_seq, q_head, table.data_ptr(), cols,
                 max(table.stride(0), cols), seq_lens.data_ptr(), out.data_ptr(), B, hq, window,
-                sinks, scale or 0.0, code, work[1], work[2], stream)
+                sinks, scale, code, work[1], work[2], stream)
         return out
 
 

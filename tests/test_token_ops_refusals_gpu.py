@@ -25,3 +25,15 @@ def test_workspaces_that_are_not_contiguous():
     with pytest.raises(ValueError):
         cache.attend(q, table, n, workspace=w)
     assert not cache.attend(q, table, n, workspace=w.contiguous()).any()
+
+
+def test_scales_that_the_entry_would_replace():
+    t = torch.randn(2, 16, 1, 64, device="cuda").to(BF)
+    cache = PagedKVCache(t, t.clone())
+    q = torch.randn(1, 1, 64, device="cuda").to(BF)
+    table = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    n = torch.full((1,), 9, dtype=torch.int32, device="cuda")
+    for scale in (0.0, -0.125, float("nan"), float("inf"), 1e-45):
+        with pytest.raises(ValueError):
+            cache.attend(q, table, n, scale=scale)
+    assert torch.equal(cache.attend(q, table, n), cache.attend(q, table, n, scale=0.125))
