@@ -80,6 +80,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float = 1e-6,
         raise ValueError("out must be contiguous and have x's shape and dtype")
     else:
         cuda_index(x, out)
+        if out.data_ptr() == ro_ptr and rows:
+            raise ValueError("out and residual_out must be different memory")
     _norm(xr[1], xr[2], rr[1], rr[2], w_ptr, out.data_ptr(), ro_ptr, rows, n, eps, code,
           raw_stream(index))
     return out if residual is None else (out, residual_out)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from sketchpad_b200 import Int4Linear, PagedKVCache
+from sketchpad_b200 import Int4Linear, PagedKVCache, rms_norm
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -37,3 +37,13 @@ def test_scales_that_the_entry_would_replace():
         with pytest.raises(ValueError):
             cache.attend(q, table, n, scale=scale)
     assert torch.equal(cache.attend(q, table, n), cache.attend(q, table, n, scale=0.125))
+
+
+def test_norm_and_stream_into_one_memory():
+    x, r = torch.randn(2, 3, 64, device="cuda").to(BF)
+    buf = torch.empty_like(x)
+    for kw in (dict(out=buf, residual_out=buf), dict(out=x, residual_out=x)):
+        with pytest.raises(ValueError):
+            rms_norm(x, None, residual=r, **kw)
+    y, s = rms_norm(x, None, residual=r, out=buf)
+    assert y is buf and torch.equal(s, x + r)
