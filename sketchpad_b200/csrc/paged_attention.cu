@@ -179,6 +179,8 @@ struct Geo {
   // unpacking spills at 168: 8 warps (four sequences up to 65536 111 us against 109 with 12, but
   // 7 sequences up to 2594 9.9 against 12.8).
   static constexpr int WARPS = DP > 128 ? (E4M3 ? 8 : 4) : E4M3 ? 8 : 12;
+  // heads_wide() gives each warp a vhead of its own only where all warps get one
+  static constexpr bool ALONE = !E4M3 && WARPS <= kMaxWide;
   static constexpr int STAGES = DP > 128 && !E4M3 ? 3 : 2;
   static constexpr int RING = STAGES * 2 * TILE;   // per warp
   static constexpr int THREADS = WARPS * 32;
@@ -682,7 +684,7 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
       n = min(16, a.group - r0);
       return static_cast<T*>(a.out) + ((int64_t)at.b * a.hq + k * a.group + r0) * a.D;
     };
-    if (TG == 1) {
+    if (G::ALONE && TG == 1) {
       // a warp has its vhead alone: its rows go out as they are
       if (my_h < heads && my_t == 0) {
         int k, n;
@@ -692,36 +694,20 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
         for (int r = 0; r < 2; ++r) {
           const int row = g + 8 * r;
           const float lr = r ? l[1] : l[0];
-          const float inv = lr == 0.f ? 0.f : (E4M3 ? a.c.v_scale[k] : 1.f) / lr;
+          const float inv = lr == 0.f ? 0.f : 1.f / lr;
           if (row >= n) break;
           if (n_parts > 1 && t4 == 0)
             __stcg(reinterpret_cast<float2*>(p + a.part_rows * a.D + 2 * row),
                    make_float2(r ? m[1] : m[0], lr));
-          auto val = [&](int e, int i) { return r ? o[e][2 + i] : o[e][i]; };
-          if constexpr (E4M3) {
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) {
-              const int d = c * 16 + t4 * 4;
-              if (d >= a.D) continue;
-              const float4 v = make_float4(val(2 * c, 0), val(2 * c + 1, 0), val(2 * c, 1),
-                                           val(2 * c + 1, 1));
-              if (n_parts > 1)
-                __stcg(reinterpret_cast<float4*>(p + row * a.D + d), v);
-              else
-                *reinterpret_cast<uint2*>(outp + row * a.D + d) =
-                    make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < DP / 8; ++e) {
-              const int d = e * 8 + t4 * 2;
-              if (d >= a.D) continue;
-              const float x = val(e, 0), y = val(e, 1);
-              if (n_parts > 1)
-                __stcg(reinterpret_cast<float2*>(p + row * a.D + d), make_float2(x, y));
-              else
-                *reinterpret_cast<uint32_t*>(outp + row * a.D + d) = pack2<T>(x * inv, y * inv);
-            }
+          for (int e = 0; e < DP / 8; ++e) {
+            const int d = e * 8 + t4 * 2;
+            if (d >= a.D) continue;
+            const float x = r ? o[e][2] : o[e][0], y = r ? o[e][3] : o[e][1];
+            if (n_parts > 1)
+              __stcg(reinterpret_cast<float2*>(p + row * a.D + d), make_float2(x, y));
+            else
+              *reinterpret_cast<uint32_t*>(outp + row * a.D + d) = pack2<T>(x * inv, y * inv);
           }
         }
       }
