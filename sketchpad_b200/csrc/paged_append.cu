@@ -21,12 +21,15 @@ namespace sp {
 namespace {
 
 // Threads of a block.  Long calls take fewer per token, which then share the lookups over more
-// heads (us with 256 / 128 / 64 threads): 8193 tokens of 56 heads of 128 49.8 / 40.4 / 39.9,
-// 6300 of 18 heads of 256 30.3 / 24.0 / 21.5, but 2160 of 144 heads of 128 27.5 / 27.4 / 28.6;
-// 32 tokens, whose blocks do not fill the GPU, 2.2 / 2.6 with 256 / 128.
+// heads.  us with 256 / 128 / 64 threads, 56 heads of 128: 32 tokens 2.4 / 2.7 / 3.7, 512 tokens
+// 3.9 / 4.6 / 6.4, 768 5.3 / 5.4 / 6.5, 1024 6.4 / 6.0 / 8.5, 1536 11.5 / 10.3 / 10.6, 2048 15.3 /
+// 12.7 / 12.4, 4096 27.4 / 22.9 / 22.3; 18 heads of 256: 512 3.3 / 4.1 / 5.0, 768 4.6 / 4.4 / 5.1,
+// 1536 7.4 / 6.1 / 6.9, 2048 11.5 / 8.9 / 8.0; but 144 heads of 128: 1024 14.9 / 14.6 / 18.1,
+// 2048 26.7 / 26.5 / 27.6.
 constexpr int kAppThreads = 256;
-constexpr int64_t kAppMany = 1024;     // tokens of a long call
-constexpr int64_t kAppValues = 8192;   // values of a token up to which 64 threads take it there
+constexpr int64_t kAppLong = 768;      // tokens of a call from which 128 threads take a token
+constexpr int64_t kAppLonger = 2048;   // ... and 64, where a token has up to
+constexpr int64_t kAppValues = 8192;   // this many values
 // Heads of q of a thread in a round; the next round's loads are under way meanwhile.  (8193
 // tokens, us: 48.8 with 1, 42.0 with 2, 40.4 with 3, 41.4 with 4; 45.5 with 2 and no round ahead.)
 constexpr int kAppHeads = 3;
@@ -288,9 +291,8 @@ extern "C" int sp_paged_kv_append(const void* cache, const void* q, const void* 
   const unsigned grid = (unsigned)tokens;
   const bool f8 = h->dtype == SP_E4M3;
   auto run = [&](auto kernel) {
-    const int threads = tokens < kAppMany                          ? kAppThreads
-                        : (a.hq + 2 * a.hkv) * a.D <= kAppValues ? kAppThreads / 4
-                                                                 : kAppThreads / 2;
+    const bool few = tokens >= kAppLonger && (a.hq + 2 * a.hkv) * a.D <= kAppValues;
+    const int threads = few ? kAppThreads / 4 : tokens >= kAppLong ? kAppThreads / 2 : kAppThreads;
     return launch_overlapped("paged append", kernel, grid, threads, 0, s, a);
   };
   if (dtype == SP_F16)
