@@ -22,11 +22,11 @@
 // page sizes take those 16-byte copies.  The query heads of a cache head are the 16 rows of the
 // warp's m16n8k16 MMAs (rows beyond hq / hkv are zeros).
 //
-// Measured, heads of 128: 32 sequences of 1 to 8192 tokens (32 heads over 8, bf16) 99 us, 5.4 TB/s
-// or 0.83 of the measured copy bandwidth; 4 of 50001 to 65536 (64 over 8, e4m3) 111 us, 0.65 (two
+// Measured, heads of 128: 32 sequences of 1 to 8192 tokens (32 heads over 8, bf16) 97 us, 5.5 TB/s
+// or 0.85 of the measured copy bandwidth; 4 of 50001 to 65536 (64 over 8, e4m3) 110 us, 0.66 (two
 // conversions and two MMAs per register of e4m3, 8 warps of 246 registers: the dependences
 // between them); 64 windows of 1024 (12 heads of 64, f16) 41.7 us, 0.74; one sequence of 4097
-// (40 over 8) 15.8 us, two steps of a block and the joins' two round trips.
+// (40 over 8) 15.1 us, two steps of a block and the joins' two round trips.
 #include <type_traits>
 
 #include "common.cuh"
@@ -194,6 +194,20 @@ struct Geo {
   }
 };
 
+// The sequences that show nothing come out as zeros: a warp of each block takes every nblk-th.
+// (512 of them, 128 heads of 128: 10.7 us; a lane to a sequence 117.)
+template <typename T>
+__device__ __forceinline__ void clear_unseen(const AttnArgs& a, int64_t capacity) {
+#pragma unroll 1
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    if (visible_of(a, b, capacity).granules != 0) continue;
+    T* o = static_cast<T*>(a.out) + (int64_t)b * a.hq * a.D;
+#pragma unroll 1
+    for (int i = (threadIdx.x & 31) * 8; i < a.hq * a.D; i += 256)
+      *reinterpret_cast<uint4*>(o + i) = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // A place in the list of steps: step `step` of `steps` of head block hb of sequence b.
 struct Cursor {
   int b, hb, step, steps;
@@ -237,8 +251,8 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
   // that at neighbouring tokens.  Large calls take HB = heads_wide, so that a block reads what
   // lies together in memory (a token's heads; 256 bytes of a head at a time cost the HBM a
   // fifth of its rate, 128 bytes a third); small ones HB = 1, which has fewer parts to join.
-  // Sequences that show nothing come out as zeros.
   const int tg_wide = G::WARPS / a.heads_wide;
+  if (warp == G::WARPS - 1) clear_unseen<T>(a, capacity);
   // (Every warp scans the lengths by itself: no barrier.)
   int32_t wide = 0, narrow = 0;  // steps of an item, over the sequences
   int first_granules = 0;        // of sequence `lane`
@@ -249,12 +263,6 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
     if (base == 0) first_granules = n;
     wide += (n + tg_wide * NG - 1) / (tg_wide * NG);
     narrow += (n + G::WARPS * NG - 1) / (G::WARPS * NG);
-    if (n == 0 && warp == 0 && b < a.B && b % nblk == blockIdx.x) {
-      T* o = static_cast<T*>(a.out) + (int64_t)b * a.hq * a.D;
-#pragma unroll 1
-      for (int i = 0; i < a.hq * a.D; i += 8)
-        *reinterpret_cast<uint4*>(o + i) = make_uint4(0, 0, 0, 0);
-    }
   }
   wide = __reduce_add_sync(0xffffffffu, wide);
   narrow = __reduce_add_sync(0xffffffffu, narrow);
@@ -307,9 +315,10 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
     cc.hb = (unit0 - seq_unit) / cc.steps;  // head blocks in order within the sequence
     cc.step = unit0 - seq_unit - cc.hb * cc.steps;
   }
-  // To the next step of the list (only while one is left).  True at an item's end.
-  auto advance = [&](Cursor& c) {
+  // To the next step of the list, if there is `more` of it for this block.  True at an item's end.
+  auto advance = [&](Cursor& c, bool more) {
     if (++c.step < c.steps) return false;
+    if (!more) return true;
     c.step = 0;
     if (++c.hb == items_per_seq) {
       c.hb = 0;
@@ -357,7 +366,7 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
           r.page = a.c.table[lk.b * a.c.table_stride + col];
         }
       }
-      advance(lk);
+      advance(lk, looked + 1 < n_steps);
     }
     ++looked;
   };
@@ -660,7 +669,7 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
 
     // ---- the item's end, or the share's
     const Cursor at = cc;
-    const bool item_end = advance(cc);
+    const bool item_end = advance(cc, s + 1 < n_steps);
     if (!item_end && s + 1 < n_steps) continue;
     fresh = true;
 #pragma unroll

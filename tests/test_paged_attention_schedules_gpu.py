@@ -119,3 +119,18 @@ def test_tables_of_more_steps_than_a_launch_takes():
     ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
     q = torch.randn(B, heads, 16, generator=gen(4), device="cuda").to(BF)
     check_attend(cache.attend(q, table, ln), q, cache, table, lens)  # one page is there
+
+
+@pytest.mark.parametrize("hq,hkv,D,cdt", [(8, 2, 128, BF), (8, 4, 256, BF), (16, 16, 64, E4M3)])
+@pytest.mark.parametrize("live", [(0, 1, 299), (150,), (149, 296, 297), ()])
+def test_padding_among_the_sequences(hq, hkv, D, cdt, live):
+    lens = [0] * 300
+    for i, b in enumerate(live):
+        lens[b] = 40 + 333 * i
+    cache = make_cache(80, 16, hkv, D, cdt)
+    table = make_table(lens, 16, 80, width=45)
+    q = torch.randn(300, hq, D, generator=gen(5), device="cuda").to(BF)
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, float("nan"))
+    cache.attend(q, table, ln, out=out)
+    check_attend(out, q, cache, table, lens)
