@@ -1,5 +1,6 @@
 // numeric.cuh -- element conversions shared by the token-decoding kernels (rms_norm.cu,
-// int4_linear.cu, paged_kv.cu): f32 <-> {f32, f16, bf16} and f32 -> e4m3 by value.
+// int4_linear.cu, paged_append.cu, paged_attention.cu): f32 <-> {f32, f16, bf16} and f32 -> e4m3
+// by value.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -24,8 +25,8 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// Two e4m3 bytes (a low) of two f32 values: round to nearest even, finite values saturate at
-// +-448, NaN stays NaN.
+// Two e4m3 bytes (a low) of two f32 values: round to nearest even, larger ones and
+// infinities saturate at +-448, NaN stays NaN.
 __device__ __forceinline__ uint16_t e4m3x2_from_f32(float a, float b) {
   return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }

@@ -3,8 +3,8 @@
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q.k_j - m)   over the visible tokens j:
 //   all of the sequence's, or its last `window` and its first `sinks`.
 //
-// Bound by HBM: every visible key and value is read once and meets only the hq / hkv query heads
-// that share it (at most 2 hq/hkv flop per byte of 16-bit cache).  The work is the list of steps
+// Bound by HBM: every visible key and value is read once (once per 16 query heads that share it,
+// the rows of an MMA) and meets only the hq / hkv query heads that share it (at most 2 hq/hkv flop per byte of 16-bit cache).  The work is the list of steps
 // (a tile per warp) of every (sequence, cache head) in order; the blocks, one per SM, take equal
 // shares of that list whatever the lengths are, so one long sequence uses the whole GPU and a
 // ragged batch is even.  Shares cut (sequence, head) items: a block leaves such a part's
@@ -973,7 +973,8 @@ extern "C" int sp_paged_attention(const void* cache, const void* q, int64_t q_se
   a.parts = reinterpret_cast<float*>(a.counters + kItems);
   const int32_t* table = a.c.table;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // sequences of a launch: the item table holds theirs, and steps count in 31 bits
+  // sequences of a launch: the workspace's counters, one per item, hold theirs, and steps count
+  // in 31 bits
   const int64_t granules = (table_cols * h->page_size + 7) / 8;
   if (granules * vheads > 2147483647LL - 65536)
     return set_error(SP_ERR_SHAPE, "paged attention: a sequence of too many tokens x heads");

@@ -60,7 +60,8 @@ class StepWorkspaces(NamedTuple):
 class DecoderLayer:
     """Weights: float tensors in the linears' [out, in] layout, quantized here to 4 bits.
 
-    qkv [(heads + 2 kv_heads) head_dim, hidden] (queries, keys, values), out [hidden, heads
+    qkv [(heads + 2 kv_heads) head_dim, hidden] (queries, keys, values; each head's rows in the
+    rotary pairs' order (2 i, 2 i + 1), see PagedKVCache.append), out [hidden, heads
     head_dim], gate_up [2 intermediate, hidden] (gate, up), down [hidden, intermediate], and the
     two norms [hidden]."""
 

@@ -127,8 +127,9 @@ class Int4Linear:
         x bf16 or f16, or float8_e4m3fn with x_scale f32 [...].  The output's type is
         out_dtype, else out's, else x's (bf16 for e4m3).
 
-        The layers share one workspace per stream; a call captured into a graph that is replayed
-        beside other work of its stream needs one of its own (`workspace_size` zero bytes)."""
+        The layers share one workspace per stream.  A call that is captured into a graph gets one
+        of the graph's, zeroed in every replay, unless it is given one (`workspace_size` zero
+        bytes), which must not be used by work beside the replays."""
         index = cuda_index(x, self.q, x_scale, out, workspace)
         N, K = self.out_features, self.in_features
         xd = _X.get(x.dtype)

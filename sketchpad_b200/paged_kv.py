@@ -32,8 +32,9 @@ _16BIT = {torch.float16: _lib.SP_F16, torch.bfloat16: _lib.SP_BF16}
 class PagedKVCache:
     """k and v tensors of equal shape; k_scale and v_scale f32 [kv_heads] for e4m3 ones.
 
-    The calls of `attend` share one device workspace per stream; a call captured into a graph
-    that is replayed beside other work of its stream needs one of its own (`new_workspace`)."""
+    The calls of `attend` share one device workspace per stream.  A call that is captured into a
+    graph gets one of the graph's, zeroed in every replay, unless it is given one (`new_workspace`),
+    which must not be used by work beside the replays."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None):
@@ -97,7 +98,9 @@ class PagedKVCache:
         ready for attention.
 
         rope: f32 [positions, head_dim / 2, 2] (cos, sin) from `rope_pair_table`; k and q are
-        rotated by their position (interleaved pairs).  A token whose sequence, position or page
+        rotated by their position, in interleaved pairs (2 i, 2 i + 1).  (Projections made for
+        pairs (i, i + head_dim / 2) have their rows put in that order first: row 2 i + h of a head
+        from row i + h head_dim / 2.)  A token whose sequence, position or page
         does not exist (a position of -1, say) is padding: nothing is stored, its q is zeros."""
         index = cuda_index(k, v, block_table, seq_ids, positions, q, rope, q_out, self.k)
         T = k.shape[0]
