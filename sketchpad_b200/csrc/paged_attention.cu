@@ -23,9 +23,9 @@
 // warp's m16n8k16 MMAs (rows beyond hq / hkv are zeros).
 //
 // Measured, heads of 128: 32 sequences of 1 to 8192 tokens (32 heads over 8, bf16) 97 us, 5.5 TB/s
-// or 0.85 of the measured copy bandwidth; 4 of 50001 to 65536 (64 over 8, e4m3) 110 us, 0.66 (two
+// or 0.85 of the measured copy bandwidth; 4 of 50001 to 65536 (64 over 8, e4m3) 109 us, 0.66 (two
 // conversions and two MMAs per register of e4m3, 8 warps of 246 registers: the dependences
-// between them); 64 windows of 1024 (12 heads of 64, f16) 41.7 us, 0.74; one sequence of 4097
+// between them); 64 windows of 1024 (12 heads of 64, f16) 41.6 us, 0.74; one sequence of 4097
 // (40 over 8) 15.1 us, two steps of a block and the joins' two round trips.
 #include <type_traits>
 
@@ -39,7 +39,7 @@ namespace {
 
 // Wide steps per block from which a call counts as large.  From 2 to 8 nothing changes that was
 // measured; with 24, 38 sequences up to 442 (12 heads of 256, 192 query heads) take 161 us
-// instead of 96 and 64 windows of 1024 53 instead of 42.
+// instead of 97 and 64 windows of 1024 53 instead of 42.
 constexpr int kLargeSteps = 8;
 constexpr int kMaxWide = 8;     // warps of a block on different vheads, at most
 
@@ -174,10 +174,10 @@ struct Geo {
   static constexpr int BOXES = CHUNKS / 8;         // of a granule
   static constexpr int TOK = DP * ES <= 128 ? 32 : 16;
   static constexpr int TILE = TOK * DP * ES;       // k or v
-  // As many warps as their registers allow: 12 of 168 (32 sequences up to 8192, D 128, 99 us
-  // against 102 with 8 of 255; 64 windows of 1024, D 64, 41.7 against 47.6).  An e4m3 tile's
-  // unpacking spills at 168: 8 warps (four sequences up to 65536 111 us against 109 with 12, but
-  // 7 sequences up to 2594 9.9 against 12.8).
+  // As many warps as their registers allow: 12 of 168 (32 sequences up to 8192, D 128, 97 us
+  // against 103 with 8 of 255; 64 windows of 1024, D 64, 41.6 against 47.4).  An e4m3 tile's
+  // unpacking spills at 168: 8 warps (four sequences up to 65536 109 us against 108 with 12, but
+  // 7 sequences up to 2594 9.9 against 13.0).
   static constexpr int WARPS = DP > 128 ? (E4M3 ? 8 : 4) : E4M3 ? 8 : 12;
   // heads_wide() gives each warp a vhead of its own only where all warps get one
   static constexpr bool ALONE = !E4M3 && WARPS <= kMaxWide;
@@ -853,9 +853,9 @@ __global__ void __launch_bounds__(Geo<T, E4M3, DP>::THREADS, 1)
 }
 
 // Warps of a block on different vheads: as many as keep all warps busy, or nearly, and at most
-// `most_wide`: 8 for 16-bit caches (32 sequences up to 8192, 8 heads of 128: 99 us, 114 with 1;
+// `most_wide`: 8 for 16-bit caches (32 sequences up to 8192, 8 heads of 128: 97 us, 110 with 1;
 // 64 windows of 1024, 12 heads of 64: 42 against 53); 1 for e4m3, whose unpacking keeps it
-// below the HBM's rate either way, so the joins of many heads count (111 us, 122 with 4).
+// below the HBM's rate either way, so the joins of many heads count (109 us, 119 with 4).
 int heads_wide(int vheads, int warps, int most_wide) {
   int best = 1;
   double most = 0;
