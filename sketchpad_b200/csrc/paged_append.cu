@@ -9,7 +9,7 @@
 // for single tokens.  One block per token: a thread owns eight values at one place of a head
 // and walks the heads, so the token's position, page and (cos, sin) pairs are loaded once for
 // all of its heads, and the first heads' values while those are looked up.  8193 tokens of 40 + 8
-// + 8 heads of 128 into an e4m3 cache: 39.9 us, 0.85 of the measured copy bandwidth; 32 tokens of
+// + 8 heads of 128 into an e4m3 cache: 40.0 us, 0.84 of the measured copy bandwidth; 32 tokens of
 // 32 + 8 + 8: 2.35 us, the chain of lookups.
 #include <new>
 

@@ -1,9 +1,9 @@
 """The 4-bit linear at the ends of the types' ranges, and with channels far above the rest.
 
-x is staged in f16, a row's largest value at 2^14 or above, a quarter of the inputs at 1/16 of
-that: what f16 cannot hold is at most 2^-25 * 2^4 / 2^14 = 2^-35 of the row's largest value per
-input, 2^-35 max|x| sum |w| in all.  The rest is the bound of the ordinary sizes, and where the
-results come near f32's subnormals their quantum, once per slab of the inputs (64 at most here)."""
+x is staged in f16, a row's largest value at 2^14 or above: what f16 cannot hold is at most
+2^-25 / 2^14 = 2^-39 of the row's largest value per input; 2^-35 max|x| sum |w| in all is allowed.
+The rest is the bound of the ordinary sizes, and where the results come near f32's subnormals
+their quantum, once per slab of the inputs (64 at most here)."""
 import pytest
 import torch
 
