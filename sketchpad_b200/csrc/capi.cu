@@ -125,12 +125,14 @@ cudaMemPool_t scratch_pool() {
   return st == 2 ? pools[dev] : nullptr;
 }
 
-bool first_time_on_device(unsigned long long* flag_bits) {
+bool ready_on_device(const unsigned long long* flag_bits) {
   const int dev = current_device();
-  if (dev < 0 || dev >= 64) return true;
-  const unsigned long long bit = 1ull << dev;
-  const unsigned long long old = __atomic_fetch_or(flag_bits, bit, __ATOMIC_ACQ_REL);
-  return (old & bit) == 0;
+  return dev >= 0 && dev < 64 && (__atomic_load_n(flag_bits, __ATOMIC_ACQUIRE) >> dev & 1) != 0;
+}
+
+void set_ready_on_device(unsigned long long* flag_bits) {
+  const int dev = current_device();
+  if (dev >= 0 && dev < 64) __atomic_fetch_or(flag_bits, 1ull << dev, __ATOMIC_RELEASE);
 }
 
 int encode_tiled(CUtensorMap* map, CUtensorMapDataType dt, uint32_t rank, const void* base,

@@ -39,9 +39,12 @@ int num_sms();
 // Current device index (cudaGetDevice; 0 on failure).
 int current_device();
 
-// True once per (flag, device): lets a launcher set a kernel attribute the first time it
-// runs on a device instead of on every call.
-bool first_time_on_device(unsigned long long* flag_bits);
+// Let a launcher set a kernel attribute the first time it runs on a device instead of on every
+// call: ready_on_device is true once set_ready_on_device has been called for the current device,
+// which the launcher does after it has set the attribute.  (Threads whose first calls meet each
+// set it; none launches before it is set.)
+bool ready_on_device(const unsigned long long* flag_bits);
+void set_ready_on_device(unsigned long long* flag_bits);
 cudaMemPool_t scratch_pool();
 
 // cuTensorMapEncodeTiled obtained through cudaGetDriverEntryPoint (no libcuda link).

@@ -517,18 +517,18 @@ int launch_fa(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& m
   auto kern = fa_fwd_kernel<NBQ, NBV, STAGES>;
   static_assert(L::kAlloc <= 232448, "flash_attn smem budget");
   static unsigned long long attr_set = 0;
-  if (first_time_on_device(&attr_set)) {
+  if (!ready_on_device(&attr_set)) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
     cudaFuncAttributes fa{};
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, kern);
     if (e != cudaSuccess || fa.maxThreadsPerBlock < kThreads) {
-      __atomic_fetch_and(&attr_set, ~(1ull << current_device()), __ATOMIC_ACQ_REL);
       return set_error(SP_ERR_LAUNCH,
                        "flash_attn: kernel cannot launch %d threads (%s; regs/thread %d, max threads "
                        "%d, dynamic smem %d of %d)",
                        kThreads, cudaGetErrorString(e), fa.numRegs, fa.maxThreadsPerBlock, L::kAlloc,
                        fa.maxDynamicSharedSizeBytes);
     }
+    set_ready_on_device(&attr_set);
   }
   const int tiles = p.single ? 1 : 2;
   dim3 grid((unsigned)((p.Sq + tiles * kBM - 1) / (tiles * kBM)), (unsigned)p.H, (unsigned)B);
@@ -768,13 +768,13 @@ int launch_attn_short_mma(const void* q, const void* k, const void* v, void* out
   auto kern = attn_short_mma_kernel<T, DH, OUT>;
   const int smem = kShortWarps * 3 * kShortMax * (DH + kSmRow) * (int)sizeof(T);
   static unsigned long long attr_set = 0;
-  if (smem > 48 * 1024 && first_time_on_device(&attr_set)) {
+  if (smem > 48 * 1024 && !ready_on_device(&attr_set)) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) {
-      __atomic_fetch_and(&attr_set, ~(1ull << current_device()), __ATOMIC_ACQ_REL);
       return set_error(SP_ERR_LAUNCH, "flash_attn: short-sequence smem attribute: %s",
                        cudaGetErrorString(e));
     }
+    set_ready_on_device(&attr_set);
   }
   const unsigned grid = (unsigned)((a.BH + kShortWarps - 1) / kShortWarps);
   kern<<<grid, kShortWarps * 32, smem, s>>>(static_cast<const T*>(q), static_cast<const T*>(k),

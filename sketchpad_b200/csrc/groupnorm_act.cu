@@ -1001,13 +1001,13 @@ template <typename T, int VPT>
 int launch_cluster(const GnParams& p, int cs, int64_t BG, cudaStream_t stream) {
   auto kern = gn_cluster_kernel<T, VPT>;
   static unsigned long long attr_set = 0;
-  if (cs > 8 && first_time_on_device(&attr_set)) {
+  if (cs > 8 && !ready_on_device(&attr_set)) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) {
-      __atomic_fetch_and(&attr_set, ~(1ull << current_device()), __ATOMIC_ACQ_REL);
       return set_error(SP_ERR_LAUNCH, "groupnorm: cluster size %d not allowed: %s", cs,
                        cudaGetErrorString(e));
     }
+    set_ready_on_device(&attr_set);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cs, (unsigned)BG, 1);
@@ -1054,14 +1054,14 @@ template <typename T>
 int launch_slices(GnSliceParams p, void* ws, cudaStream_t stream) {
   auto kern = gn_slice_kernel<T>;
   static unsigned long long attr_set = 0;
-  if (first_time_on_device(&attr_set)) {
+  if (!ready_on_device(&attr_set)) {
     const cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SlRoles<T>::kSmem);
     if (e != cudaSuccess) {
-      __atomic_fetch_and(&attr_set, ~(1ull << current_device()), __ATOMIC_ACQ_REL);
       return set_error(SP_ERR_LAUNCH, "groupnorm: kernel attribute failed: %s",
                        cudaGetErrorString(e));
     }
+    set_ready_on_device(&attr_set);
   }
   // resident CTAs per SM, found once per device: the grid is exactly the resident set
   // (cooperative launch), so every CTA a pass-1 unit waits on is running

@@ -970,14 +970,14 @@ static int launch_cluster_nhwc(const NhwcClusterParams& p, const ClusterPlan& pl
                         : gn_nhwc_cluster_reg_kernel<T, 1>;
   if (pl.R > kClRegRows) {
     static unsigned long long attr_set = 0;
-    if (first_time_on_device(&attr_set)) {
+    if (!ready_on_device(&attr_set)) {
       cudaError_t e = cudaFuncSetAttribute(gn_nhwc_cluster_kernel<T>,
                                            cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
       if (e != cudaSuccess) {
-        __atomic_fetch_and(&attr_set, ~(1ull << current_device()), __ATOMIC_ACQ_REL);
         return set_error(SP_ERR_LAUNCH, "groupnorm (channels-last): smem attribute failed: %s",
                          cudaGetErrorString(e));
       }
+      set_ready_on_device(&attr_set);
     }
   }
   cudaLaunchConfig_t cfg = {};

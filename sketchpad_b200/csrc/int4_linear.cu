@@ -670,11 +670,13 @@ template <int NT, int GPC, bool ZP, bool SBF>
 int launch_int4(Int4Args a, const Int4Plan& p, cudaStream_t s) {
   auto kernel = int4_linear_kernel<NT, GPC, ZP, SBF>;
   static unsigned long long flags = 0;
-  if (first_time_on_device(&flags) &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           kI4Smem - 1024 - kRedBytes) != cudaSuccess)
-    return set_error(SP_ERR_LAUNCH, "int4 linear: shared memory attribute: %s",
-                     cudaGetErrorString(cudaGetLastError()));
+  if (!ready_on_device(&flags)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kI4Smem - 1024 - kRedBytes) != cudaSuccess)
+      return set_error(SP_ERR_LAUNCH, "int4 linear: shared memory attribute: %s",
+                       cudaGetErrorString(cudaGetLastError()));
+    set_ready_on_device(&flags);
+  }
   a.S = p.S, a.cs = p.cs, a.U = p.U;
   return launch_overlapped("int4 linear", kernel, p.blocks, kI4Warps * 32, p.smem, s, a);
 }

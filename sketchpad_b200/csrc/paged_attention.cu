@@ -873,11 +873,13 @@ int launch_attn_tma(AttnArgs a, const CacheHandle* h, cudaStream_t s) {
   a.heads_wide = heads_wide(a.vheads, G::WARPS, E4M3 ? 1 : kMaxWide);
   auto kernel = paged_attn_kernel<T, E4M3, DP, TMA>;
   static unsigned long long flags = 0;
-  if (first_time_on_device(&flags) &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM) !=
-          cudaSuccess)
-    return set_error(SP_ERR_LAUNCH, "paged attention: shared memory attribute: %s",
-                     cudaGetErrorString(cudaGetLastError()));
+  if (!ready_on_device(&flags)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM) !=
+        cudaSuccess)
+      return set_error(SP_ERR_LAUNCH, "paged attention: shared memory attribute: %s",
+                       cudaGetErrorString(cudaGetLastError()));
+    set_ready_on_device(&flags);
+  }
   const int blocks = num_sms();
   return launch_overlapped("paged attention", kernel, blocks, G::THREADS, G::SMEM, s, a, h->kmap,
                            h->vmap);

@@ -993,14 +993,14 @@ int launch_qlinear_small(const void* x, const void* w, const QlParams& p, cudaSt
   }
   auto kern = qlinear_small_kernel<BN>;
   static unsigned long long attr_set = 0;
-  if (first_time_on_device(&attr_set)) {
+  if (!ready_on_device(&attr_set)) {
     const cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kAlloc);
     if (e != cudaSuccess) {
-      __atomic_fetch_and(&attr_set, ~(1ull << current_device()), __ATOMIC_ACQ_REL);
       return set_error(SP_ERR_LAUNCH, "bf16 linear: smem attribute failed: %s",
                        cudaGetErrorString(e));
     }
+    set_ready_on_device(&attr_set);
   }
   QlParams q = p;
   q.ws = nullptr;
@@ -1109,15 +1109,15 @@ int launch_qlinear(const void* x, const void* w8, const QlParams& p, cudaStream_
   auto kern1 = qlinear_kernel<WF, false>;
   auto kern2 = qlinear_kernel<WF, WF != W_BF16>;  // (bf16 weights never pair)
   static unsigned long long attr_set[2] = {0, 0};
-  if (first_time_on_device(&attr_set[pair])) {
+  if (!ready_on_device(&attr_set[pair])) {
     cudaError_t e = pair ? cudaFuncSetAttribute(kern2, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                 kSmem2)
                          : cudaFuncSetAttribute(kern1, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                 kSmem1);
     if (e != cudaSuccess) {
-      __atomic_fetch_and(&attr_set[pair], ~(1ull << current_device()), __ATOMIC_ACQ_REL);
       return set_error(SP_ERR_LAUNCH, "quantized linear: smem attribute failed: %s", cudaGetErrorString(e));
     }
+    set_ready_on_device(&attr_set[pair]);
   }
   // a paired tile is 512 x rows (two CTAs of 256), an unpaired one 256
   const int m_rows = pair ? 2 * kQBM : kQBM, cta_per_tile = pair ? 2 : 1;
